@@ -356,6 +356,83 @@ int ogx_attention_fwd_e4m3_to_peers(const void* q, const void* k, const void* v,
                                     void* const* peer_bases, int peers, int64_t tokens_per_peer,
                                     int64_t out_stride_t, void* stream);
 
+/* ---- Training pass of the attention (the reference only infers; these are additions of this library): the
+ * attention that keeps what its backward pass needs, attention's gradients, and the Q/K norm + rotation with
+ * its gradients.  All results are summed in a fixed order: the same inputs give the same bits. */
+
+/* Attention with masks and shared key/value heads, keeping the softmax statistics.  q [batch, q_tokens,
+ * heads*128], k and v [batch, kv_tokens, kv_heads*128] bf16 with token and batch strides (multiples of 8
+ * elements); query head h reads key/value head h / (heads / kv_heads).  Query i sees key j when
+ *   i < q_lengths[b], j < kv_lengths[b] (int32 device arrays, clamped to [0, tokens]; NULL: full length), and
+ *   causal_block == 0 or j / causal_block <= floor((i + kv_tokens - q_tokens) / causal_block):
+ * causal_block 1 is the token-causal mask with both sequences ending together, n a mask over blocks of n
+ * positions (the tokens of a latent frame).  out: bf16 [batch, q_tokens, heads*128]; lse: f32 [batch, heads,
+ * q_tokens], the natural log of each row's sum of exponentials.  A row that sees no key gets out = 0 and lse =
+ * -inf.  Keys and values past kv_lengths may hold anything (NaN included). */
+int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
+                          int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
+                          int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t, float softmax_scale,
+                          int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
+                          int64_t out_stride_b, int64_t out_stride_t, float* lse, void* stream);
+
+/* Bytes of device workspace that ogx_attention_bwd needs for these sizes. */
+int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads,
+                                int64_t* bytes);
+
+/* Gradients of ogx_attention_fwd_lse: from dout (the gradient of out), the forward's inputs, out and lse, dq
+ * [batch, q_tokens, heads*128] and dk, dv [batch, kv_tokens, kv_heads*128] (bf16, own strides, dk and dv
+ * sharing theirs), every element written.  The probabilities are recomputed from lse.  Rows past q_lengths and
+ * rows that see no key get dq = 0 and give nothing to dk and dv (their q and dout may hold anything); keys past
+ * kv_lengths get dk = dv = 0.  workspace: device memory, 16-byte aligned, overwritten; calls that may run at the
+ * same time need one each. */
+int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                      const float* lse, int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
+                      int64_t kv_heads, int64_t head_dim, int64_t dout_stride_b, int64_t dout_stride_t,
+                      int64_t q_stride_b, int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t,
+                      int64_t out_stride_b, int64_t out_stride_t, float softmax_scale, int64_t causal_block,
+                      const int* q_lengths, const int* kv_lengths, void* workspace, int64_t workspace_bytes, void* dq,
+                      int64_t dq_stride_b, int64_t dq_stride_t, void* dk, void* dv, int64_t dkv_stride_b,
+                      int64_t dkv_stride_t, void* stream);
+
+/* What the RMSNorm of ogx_qk_norm_rope runs over. */
+#define OGX_NORM_NONE 0 /* no norm: the rotation alone */
+#define OGX_NORM_HEAD 1 /* each head by itself, weights [head_dim] */
+#define OGX_NORM_ROW 2  /* all heads of a row together, weights [heads * head_dim] */
+
+/* Q/K RMSNorm (with weight) and rotation in one pass, fp32 math, one bf16 rounding.  q [batch, tokens,
+ * heads*head_dim] and k [batch, tokens, kv_heads*head_dim] bf16 with batch and token strides (multiples of 8
+ * elements), head_dim 64 or 128, heads + kv_heads <= 128.  The first `rotary` columns of each head (a multiple of
+ * 16) turn by the token's angles: columns (j, j + rotary/2), or (2j, 2j + 1) with interleaved != 0, by entry j of
+ * cos and sin.  The tables are bf16 or f32 with unit column stride and strides cs_stride_b (0: shared by the
+ * batch), cs_stride_h (0: shared by the heads; otherwise heads == kv_heads) and cs_stride_t, multiples of 8.
+ * The outputs may be the inputs (in place).  With OGX_NORM_ROW and the half layout this is the arithmetic of
+ * ogx_video_qk_rmsnorm_rope at other widths, batches and head counts. */
+int ogx_qk_norm_rope(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                     int64_t head_dim, int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
+                     const void* q_weight, const void* k_weight, int weight_dtype, int norm, float eps,
+                     const void* cos, const void* sin, int cs_dtype, int64_t rotary, int interleaved,
+                     int64_t cs_stride_b, int64_t cs_stride_h, int64_t cs_stride_t, void* q_out, int64_t q_out_stride_b,
+                     int64_t q_out_stride_t, void* k_out, int64_t k_out_stride_b, int64_t k_out_stride_t,
+                     void* stream);
+
+/* Bytes of device workspace that ogx_qk_norm_rope_bwd needs for these sizes on the current device (0 for
+ * OGX_NORM_NONE). */
+int ogx_qk_norm_rope_bwd_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                   int norm, int64_t* bytes);
+
+/* Gradients of ogx_qk_norm_rope: from those of its outputs (dq_out, dk_out) and its inputs, dq and dk (bf16, own
+ * strides; they may be dq_out and dk_out) and the weights' dq_weight, dk_weight (f32, summed over all rows; not
+ * written for OGX_NORM_NONE).  workspace as for ogx_attention_bwd (may be NULL for OGX_NORM_NONE). */
+int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq_out_stride_t, const void* dk_out,
+                         int64_t dk_out_stride_b, int64_t dk_out_stride_t, const void* q, const void* k, int64_t batch,
+                         int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
+                         int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, const void* q_weight,
+                         const void* k_weight, int weight_dtype, int norm, float eps, const void* cos, const void* sin,
+                         int cs_dtype, int64_t rotary, int interleaved, int64_t cs_stride_b, int64_t cs_stride_h,
+                         int64_t cs_stride_t, void* dq, int64_t dq_stride_b, int64_t dq_stride_t, void* dk,
+                         int64_t dk_stride_b, int64_t dk_stride_t, float* dq_weight, float* dk_weight, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,9 @@ DTYPE_F32 = 1
 DTYPE_F16 = 2
 QUANT_TORCH = 0
 QUANT_SINGLE = 1
+NORM_NONE = 0
+NORM_HEAD = 1
+NORM_ROW = 2
 
 # name -> argument types (restype is c_int for all entry points but ogx_last_error)
 _SIGNATURES: dict[str, list] = {
@@ -130,6 +133,33 @@ _SIGNATURES: dict[str, list] = {
     "ogx_attention_fwd_e4m3_to_peers": [
         c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p, c_int, c_int64,
         c_int64, c_void_p,
+    ],
+    "ogx_attention_fwd_lse": [
+        c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+        c_int64, c_int64, c_float, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+    ],
+    "ogx_attention_bwd_workspace": [
+        c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+    ],
+    "ogx_attention_bwd": [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+        c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
+        c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+        c_int64, c_int64, c_void_p,
+    ],
+    "ogx_qk_norm_rope": [
+        c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+        c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_int64, c_int, c_int64, c_int64,
+        c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+    ],
+    "ogx_qk_norm_rope_bwd_workspace": [
+        c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p,
+    ],
+    "ogx_qk_norm_rope_bwd": [
+        c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+        c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int, c_float,
+        c_void_p, c_void_p, c_int, c_int64, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64,
+        c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
     ],
 }
 

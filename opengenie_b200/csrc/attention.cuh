@@ -74,7 +74,50 @@ struct Params {
   // over NVLink instead of out_q.
   uint8_t* out_peer[8];
   int peer_tokens;
+  // MASKED kernels only (Visibility below has the masks' meaning)
+  float* lse;                  // [batch, heads, L]: natural log of each row's sum of exponentials
+  int heads_per_kv;            // query heads that share a key/value head
+  int causal_block;            // 0: every key is visible
+  const int* q_lengths;        // [batch] or null
+  const int* kv_lengths;       // [batch] or null
 };
+
+// Which keys a query sees.  Queries from q_len on see none; keys from kv_len on are seen by none.  With
+// block > 0 the sequences end together: query i stands at position i + shift, shift = L_kv - L, and sees the
+// keys of its own block of `block` positions and of all earlier blocks (block 1: the token-causal mask; the
+// tokens of a latent frame: a frame-causal one).  Both forms below are prefixes, so a tile needs comparing
+// only at its border.
+struct Visibility {
+  int q_len, kv_len, block, shift;
+  // keys [0, limit) are visible to query i
+  __device__ __forceinline__ int limit(int i) const {
+    if (i >= q_len) return 0;
+    if (block == 0) return kv_len;
+    const int at = i + shift;
+    if (at < 0) return 0;
+    const int64_t end = static_cast<int64_t>(at) - at % block + block;
+    return end < kv_len ? static_cast<int>(end) : kv_len;
+  }
+  // queries [first(j), q_len) see key j < kv_len
+  __device__ __forceinline__ int first(int j) const { return block == 0 ? 0 : j - j % block - shift; }
+};
+
+__device__ __forceinline__ int clamp_length(const int* lengths, int batch, int full) {
+  if (lengths == nullptr) return full;
+  const int n = lengths[batch];
+  return n < 0 ? 0 : (n > full ? full : n);
+}
+
+// Zeroes rows [row0, rows) of a tile of 128-byte rows (both 64-column halves) that a TMA load wrote, by one
+// warp: rows past a sequence's length hold whatever the caller's memory holds there, and 0 * NaN in the
+// product that sums over these rows would reach every output.  The caller has waited for the load and
+// signals the MMA issuer afterwards.  (A 128-byte row stays its own 128 bytes under the swizzle.)
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int half_bytes, int row0, int rows, uint32_t lane) {
+  for (int i = static_cast<int>(lane); i < (rows - row0) * 8; i += 32) {
+    *reinterpret_cast<uint4*>(tile + row0 * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(tile + half_bytes + row0 * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
 
 struct SharedState {
   uint64_t q_full;
@@ -85,6 +128,9 @@ struct SharedState {
   uint64_t o_ready[NQ];    // completes once per PV_q(j)
   uint64_t o_done[NQ];     // the last PV_q completed
   uint64_t drained;
+  // MASKED: the MMA issuer asks warp 2 to zero the rows past the keys in the last V tile, and its answer.  (A
+  // warp that waited for that tile's load by parity alone could take an earlier load of the stage for it.)
+  uint64_t v_fix_request, v_fixed;
   uint32_t tmem_base;
   int abort;
 };
@@ -144,7 +190,9 @@ __device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* map, 
   tma_load_4d(dst + half_bytes, map, bar, 64, head, row0, batch);
 }
 
-template <bool OUT_E4M3>
+// MASKED adds per-batch lengths, a block-causal mask, shared key/value heads and the softmax statistics that
+// the backward pass reads (bf16 output only); without it the code is the dense kernel's.
+template <bool OUT_E4M3, bool MASKED = false>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                     const __grid_constant__ CUtensorMap tv, Params p) {
@@ -162,8 +210,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t lane = threadIdx.x & 31;
   const int head = blockIdx.y;
   const int batch = blockIdx.z;
-  const int q_block0 = blockIdx.x * (NQ * BQ);
-  const int nkv = (p.L_kv + BKV - 1) / BKV;
+  // causal rows get longer with their index: the longest blocks start first
+  const int q_block0 = (MASKED ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * (NQ * BQ);
+  const int kv_head = MASKED ? head / p.heads_per_kv : head;
 
   if (threadIdx.x == 0) {
     mbar_init(&st.q_full, 1);
@@ -182,6 +231,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&st.o_done[q], 1);
     }
     mbar_init(&st.drained, 1);
+    if (MASKED) {
+      mbar_init(&st.v_fix_request, 1);
+      mbar_init(&st.v_fixed, 1);
+    }
     st.abort = 0;
     fence_mbar_init();
   }
@@ -190,6 +243,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
   }
   pdl_wait();  // everything above touches only this CTA's shared memory and TMEM
+  int nkv = (p.L_kv + BKV - 1) / BKV;
+  Visibility vis{};
+  int fix_tile = -1;  // the V tile whose last rows lie past the keys' length
+  if constexpr (MASKED) {
+    vis = Visibility{clamp_length(p.q_lengths, batch, p.L), clamp_length(p.kv_lengths, batch, p.L_kv), p.causal_block,
+                     p.L_kv - p.L};
+    const int last = min(q_block0 + NQ * BQ, vis.q_len) - 1;  // limit() grows with the row
+    nkv = last < q_block0 ? 0 : (vis.limit(last) + BKV - 1) / BKV;
+    if (vis.kv_len < p.L_kv && vis.kv_len % BKV != 0 && vis.kv_len / BKV < nkv) fix_tile = vis.kv_len / BKV;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -198,7 +261,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     reg_dealloc<kRegsProducer>();
-    if (warp == 0 && elect_one()) {
+    if (MASKED && nkv == 0) {
+      // no row of this block sees a key: nothing to load or multiply
+    } else if (MASKED && warp == 2 && fix_tile >= 0) {
+      if (mbar_wait(&st.v_fix_request, 0, abort) &&
+          mbar_wait(&st.v_full[fix_tile % KV_STAGES], (fix_tile / KV_STAGES) & 1, abort)) {
+        zero_rows(v_tiles + (fix_tile % KV_STAGES) * KV_TILE_BYTES, KV_HALF_BYTES, vis.kv_len % BKV, BKV, lane);
+        fence_async_shared();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&st.v_fixed);
+    } else if (warp == 0 && elect_one()) {
       // ---------------------------------------------------------- TMA producer
       tma_prefetch_desc(&tq);
       tma_prefetch_desc(&tk);
@@ -212,11 +285,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t ph = (j / KV_STAGES) & 1;
         if (!mbar_wait(&st.k_empty[s], ph ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.k_full[s], KV_TILE_BYTES);
-        load_rows(k_tiles + s * KV_TILE_BYTES, &tk, &st.k_full[s], KV_HALF_BYTES, head, j * BKV, batch);
+        load_rows(k_tiles + s * KV_TILE_BYTES, &tk, &st.k_full[s], KV_HALF_BYTES, kv_head, j * BKV, batch);
         ++issued;
         if (!mbar_wait(&st.v_empty[s], ph ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.v_full[s], KV_TILE_BYTES);
-        load_rows(v_tiles + s * KV_TILE_BYTES, &tv, &st.v_full[s], KV_HALF_BYTES, head, j * BKV, batch);
+        load_rows(v_tiles + s * KV_TILE_BYTES, &tv, &st.v_full[s], KV_HALF_BYTES, kv_head, j * BKV, batch);
         ++issued;
       }
       if (*abort) {
@@ -278,6 +351,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int j2 = j + 2;
         const int s2 = j2 % KV_STAGES;
         if (!mbar_wait(&st.v_full[s], ph, abort) || !mbar_wait(&st.p_full[0][j & 1], pph, abort)) { ok = false; break; }
+        if (MASKED && j == fix_tile) {
+          mbar_arrive(&st.v_fix_request);
+          if (!mbar_wait(&st.v_fixed, 0, abort)) { ok = false; break; }
+        }
         tc_fence_after();
         issue_pv(0, j);
         if (j2 < nkv) {
@@ -309,6 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m_run = -INFINITY;  // running max, already multiplied by c
     float l_run = 0.f;
     bool ok = true;
+    const int limit = MASKED ? vis.limit(q_block0 + q * BQ + row) : p.L_kv;
     for (int j = 0; j < nkv; ++j) {
       const int b = j & 1;
       const uint32_t s_tmem = tmem + lane_off + TMEM_S + q * 128 + b * 64;
@@ -319,8 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
       tmem_ld_wait();
       float* sf = reinterpret_cast<float*>(sr);
-      const int kv_valid = p.L_kv - j * BKV;
-      if (kv_valid < BKV) {
+      const int kv_valid = limit - j * BKV;
+      if (MASKED ? __any_sync(0xffffffffu, kv_valid < BKV) : kv_valid < BKV) {
 #pragma unroll
         for (int i = 0; i < BKV; ++i)
           if (i >= kv_valid) sf[i] = -INFINITY;
@@ -341,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float alpha = 1.f;
       bool rescale = false;
       if (j == 0) {
-        m_use = m_tile;
+        m_use = (MASKED && limit <= 0) ? 0.f : m_tile;  // key 0 is visible to every row that sees any
       } else if (m_tile > m_run + kRescaleThreshold) {
         m_use = m_tile;
         alpha = ex2(m_run - m_tile);
@@ -388,10 +466,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       mbar_arrive(&st.p_full[q][b]);
     }
-    if (ok && mbar_wait(&st.o_done[q], 0, abort)) {
+    if (MASKED && nkv == 0) {
+      const int token = q_block0 + q * BQ + row;
+      if (token < p.L) {
+        uint4* dst = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(batch) * p.out_stride_b +
+                                              static_cast<int64_t>(token) * p.out_stride_t +
+                                              static_cast<int64_t>(head) * HD);
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+        p.lse[(static_cast<int64_t>(batch) * gridDim.y + head) * p.L + token] = -INFINITY;
+      }
+    } else if (ok && mbar_wait(&st.o_done[q], 0, abort)) {
       tc_fence_after();
       const int token = q_block0 + q * BQ + row;
       const float inv_l = 1.f / l_run;
+      if constexpr (MASKED) {
+        if (token < p.L)
+          p.lse[(static_cast<int64_t>(batch) * gridDim.y + head) * p.L + token] =
+              limit <= 0 ? -INFINITY : (m_run + log2f(l_run)) * 0.6931471805599453f;
+      }
       if constexpr (OUT_E4M3) {
         // e4m3 rows are 128 bytes.  Each thread owns one row, so storing straight from registers
         // would scatter 32 rows per instruction; instead the warp stages its 32 quantised rows in
@@ -459,7 +552,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int v8 = 0; v8 < 4; ++v8) {
               float f[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(orr[v8 * 8 + i]) * inv_l;
+              for (int i = 0; i < 8; ++i)
+                f[i] = (MASKED && limit <= 0) ? 0.f : __uint_as_float(orr[v8 * 8 + i]) * inv_l;
               *reinterpret_cast<uint4*>(p.out + base + v8 * 8) = pack8(f);
             }
           }

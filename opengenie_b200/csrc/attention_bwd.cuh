@@ -1,0 +1,666 @@
+// Gradients of attention, head_dim 128, bf16 in and out, fp32 softmax and accumulation.  With c the softmax
+// scale, S = c Q K^T, P = exp(S - lse) (recomputed from the row statistics the forward pass kept) and
+// delta_i = dO_i . O_i:
+//   dV = P^T dO,   dP = dO V^T,   dS = P o (dP - delta),   dQ = c dS K,   dK = c dS^T Q;
+// dK and dV of a shared key/value head sum over its query heads.
+//
+// Two launches.  attn_bwd_stats_kernel writes per query row -lse * log2(e) and -delta.  attn_bwd_kernel has a
+// CTA for every tile of 128 keys of a key/value head (dK and dV, over all query tiles of its query heads)
+// and a CTA for every tile of 128 queries of a head (dQ, over all key tiles).  S and dP are computed in both:
+// seven tile products instead of five.  In return every gradient is summed in one CTA's tensor memory in a
+// fixed order: no fp32 buffer for dQ, no atomics, and the same bits on every run.  The five-product form adds
+// its dQ tiles to HBM (a 64 KB reduction per tile pair, in whatever order the CTAs reach it).
+#pragma once
+
+#include "attention.cuh"
+#include "rows.cuh"
+
+namespace ogx {
+namespace attn {
+
+constexpr int BT = 128;                        // queries or keys per tile
+constexpr int T_HALF_BYTES = BT * 64 * 2;      // 64-column half of a tile (128-byte rows, 128-byte swizzle)
+constexpr int T_BYTES = 2 * T_HALF_BYTES;
+constexpr int STAT_FLOATS = 2 * BT;            // a query tile's statistics: 128 x -lse*log2e, 128 x -delta
+constexpr int STAT_BYTES = STAT_FLOATS * 4;
+constexpr int B_STAGES = 2;                    // ring of the operands a CTA streams
+constexpr int DQ_K_STAGES = 3;                 // K tiles of a dQ CTA: S of the next tile but one needs its K early
+constexpr int BWD_SMEM_DKDV = (2 + 2 * B_STAGES) * T_BYTES + B_STAGES * STAT_BYTES;
+constexpr int BWD_SMEM_DQ = (2 + B_STAGES + DQ_K_STAGES) * T_BYTES;
+constexpr int BWD_SMEM = (BWD_SMEM_DKDV > BWD_SMEM_DQ ? BWD_SMEM_DKDV : BWD_SMEM_DQ) + 1024;
+constexpr int kBwdThreads = 384;               // TMA, MMA, row-zeroing and one idle warp; two softmax groups
+
+struct BwdParams {
+  int L, L_kv;
+  int heads, kv_heads, heads_per_kv;
+  int q_tiles, kv_tiles;
+  unsigned dkdv_ctas;  // CTAs [0, dkdv_ctas) make dK and dV, the rest dQ
+  int causal_block;
+  float scale, scale_log2;
+  const int* q_lengths;
+  const int* kv_lengths;
+  const float* stats;  // [batch][heads][q_tiles][2][128]
+  __nv_bfloat16 *dq, *dk, *dv;
+  int64_t dq_stride_b, dq_stride_t, dkv_stride_b, dkv_stride_t;
+};
+
+struct BwdShared {
+  uint64_t fixed_full;                             // the operands a CTA keeps: K and V, or Q and dO
+  uint64_t a_full[DQ_K_STAGES], a_empty[DQ_K_STAGES];  // Q and statistics (dK/dV), K (dQ)
+  uint64_t b_full[B_STAGES], b_empty[B_STAGES];        // dO (dK/dV), V (dQ)
+  uint64_t zero_request, zeroed;  // the MMA issuer asks warp 2 to zero rows past the sequence's length; its answer
+  uint64_t s_full[2], p_full, dp_full, dp_read, ds_full[2];
+  uint64_t done;
+  uint32_t tmem_base;
+  int abort;
+};
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// D[128 x 128] (+)= A B^T, both tiles in shared memory with the 128 columns of d as the summed axis.
+__device__ __forceinline__ void mma_tile_ss(uint32_t d, uint32_t a, uint32_t b) {
+  constexpr uint32_t idesc = make_idesc(1, 1, 0, 0, BT, BT);
+#pragma unroll
+  for (int kk = 0; kk < HD / 16; ++kk) {
+    const uint32_t off = (kk >> 2) * T_HALF_BYTES + (kk & 3) * 32;
+    mma_f16_ss(d, make_sdesc_sw128(a + off, 16, 1024), make_sdesc_sw128(b + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+  }
+}
+
+// D[128 x 128] (+)= A B with A (bf16, 128 x 128) in tensor memory: each softmax group writes its 64 columns over
+// the start of the fp32 columns it has read, so columns [0, 64) lie at a and columns [64, 128) at a + 64.  B's
+// rows are the summed axis.
+__device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
+  constexpr uint32_t idesc = make_idesc(1, 1, 0, 1, BT, HD);
+#pragma unroll
+  for (int kk = 0; kk < BT / 16; ++kk)
+    mma_f16_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, make_sdesc_sw128(b + kk * 2048, T_HALF_BYTES, 1024), idesc,
+               (accumulate || kk > 0) ? 1u : 0u);
+}
+
+// A row's 128 fp32 columns in tensor memory, or `columns` of them, times `scale`, as bf16 to global memory.
+__device__ __forceinline__ void store_row(uint32_t taddr, int columns, float scale, __nv_bfloat16* dst, bool valid) {
+#pragma unroll 1
+  for (int oc = 0; oc < columns / 32; ++oc) {
+    uint32_t r[32];
+    tmem_ld32(taddr + oc * 32, r);
+    tmem_ld_wait();
+    if (valid) {
+#pragma unroll
+      for (int v8 = 0; v8 < 4; ++v8) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[v8 * 8 + i]) * scale;
+        *reinterpret_cast<uint4*>(dst + oc * 32 + v8 * 8) = pack8(f);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void zero_row(__nv_bfloat16* dst, int columns) {
+  for (int i = 0; i < columns / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// 64 scores of a row to probabilities: exp2(score * c + offset), three quarters on the MUFU and one on the FMA pipe.
+template <typename Offset>
+__device__ __forceinline__ void probabilities(float (&s)[64], float c, Offset offset) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const f2 a = fma2(f2{s[2 * i], s[2 * i + 1]}, f2{c, c}, offset(2 * i));
+    const f2 pr = ((kPolyChunkMask >> (i / 8)) & 1u) ? ex2_poly2(a) : f2{ex2(a.x), ex2(a.y)};
+    s[2 * i] = pr.x;
+    s[2 * i + 1] = pr.y;
+  }
+}
+
+// ------------------------------------------------------------------------------------------- row statistics
+// 16 lanes per (token, head) row.  Rows past the sequence's length and rows that saw no key get -lse = -inf, so
+// their probabilities are 0; the tiles' padding rows too.
+struct StatsParams {
+  const __nv_bfloat16 *dout, *out;
+  int64_t dout_stride_b, dout_stride_t, out_stride_b, out_stride_t;
+  const float* lse;
+  const int* q_lengths;
+  float* stats;
+  int L, heads, q_tiles;
+  int64_t rows;  // batch * q_tiles * 128 * heads
+};
+
+__global__ void __launch_bounds__(256) attn_bwd_stats_kernel(StatsParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int sub = threadIdx.x & 15;
+  // whole warps stay together: the reduction below names all 32 lanes
+  const int64_t per_block = blockDim.x / 16;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per_block; r0 < p.rows; r0 += gridDim.x * per_block) {
+    const int64_t r = r0 + threadIdx.x / 16;
+    const bool in = r < p.rows;
+    const int64_t rr = in ? r : 0;
+    const int head = static_cast<int>(rr % p.heads);
+    const int64_t bt = rr / p.heads;
+    const int padded = p.q_tiles * BT;
+    const int token = static_cast<int>(bt % padded);
+    const int batch = static_cast<int>(bt / padded);
+    const bool live = in && token < clamp_length(p.q_lengths, batch, p.L);
+    float d = 0.f;
+    if (live) {
+      float a[8], b[8];
+      unpack8(*reinterpret_cast<const uint4*>(p.dout + batch * p.dout_stride_b + token * p.dout_stride_t +
+                                              static_cast<int64_t>(head) * HD + sub * 8),
+              a);
+      unpack8(*reinterpret_cast<const uint4*>(p.out + batch * p.out_stride_b + token * p.out_stride_t +
+                                              static_cast<int64_t>(head) * HD + sub * 8),
+              b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d = fmaf(a[i], b[i], d);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (in && sub == 0) {
+      const int64_t bh = static_cast<int64_t>(batch) * p.heads + head;
+      const float lse = live ? p.lse[bh * p.L + token] : -INFINITY;
+      const bool empty = lse == -INFINITY;
+      float* dst = p.stats + (bh * p.q_tiles + token / BT) * STAT_FLOATS + token % BT;
+      dst[0] = empty ? -INFINITY : -lse * 1.4426950408889634f;
+      dst[BT] = empty ? 0.f : -d;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------- dK and dV
+// One tile of 128 keys; keys are the rows (TMEM lanes) of every product, so P^T and dS^T feed the dV and dK
+// products from tensor memory and a softmax thread owns one key.
+//   TMEM: S^T [0,128), dP^T [128,256), dV [256,384), dK [384,512); bf16 P^T over S^T, dS^T over dP^T.
+// Per query tile the MMA issuer runs dV += P dO, S(next), dK += dS Q, dP(next): while the softmax groups turn S
+// into P the tensor pipe does the previous tile's dK and this tile's dP, and while they turn dP into dS it does
+// dV and the next S.
+__device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv,
+                                         const CUtensorMap* tdo, const BwdParams& p, BwdShared& st, uint8_t* smem,
+                                         uint32_t tmem) {
+  uint8_t* k_tile = smem;
+  uint8_t* v_tile = smem + T_BYTES;
+  uint8_t* q_tiles = smem + 2 * T_BYTES;
+  uint8_t* do_tiles = q_tiles + B_STAGES * T_BYTES;
+  uint8_t* stat_tiles = do_tiles + B_STAGES * T_BYTES;
+  const uint32_t warp = warp_idx();
+  const uint32_t lane = threadIdx.x & 31;
+  volatile int* abort = &st.abort;
+
+  const unsigned idx = blockIdx.x;
+  const int kt = static_cast<int>(idx % p.kv_tiles);
+  const int bh = static_cast<int>(idx / p.kv_tiles);
+  const int kv_head = bh % p.kv_heads;
+  const int batch = bh / p.kv_heads;
+  const int k0 = kt * BT;
+  const Visibility vis{clamp_length(p.q_lengths, batch, p.L), clamp_length(p.kv_lengths, batch, p.L_kv),
+                       p.causal_block, p.L_kv - p.L};
+  const int first_tile = max(vis.first(k0), 0) / BT;
+  const int end_tile = (vis.q_len + BT - 1) / BT;
+  const int per_head = (k0 >= vis.kv_len || end_tile <= first_tile) ? 0 : end_tile - first_tile;
+  const int n = per_head * p.heads_per_kv;
+  // the last query tile of each head has rows past the sequence's length, holding the caller's memory
+  const bool fix = vis.q_len < p.L && vis.q_len % BT != 0;
+
+  if (n == 0) {
+    if (warp >= 4) {
+      const int key = k0 + static_cast<int>((warp & 3) * 32 + lane);
+      __nv_bfloat16* base = warp < 8 ? p.dv : p.dk;
+      if (key < p.L_kv)
+        zero_row(base + batch * p.dkv_stride_b + key * p.dkv_stride_t + static_cast<int64_t>(kv_head) * HD, HD);
+    }
+    return;
+  }
+
+  if (warp == 0) {
+    if (elect_one()) {
+      // ---------------------------------------------------------- TMA producer
+      mbar_arrive_expect_tx(&st.fixed_full, 2 * T_BYTES);
+      load_rows(k_tile, tk, &st.fixed_full, T_HALF_BYTES, kv_head, k0, batch);
+      load_rows(v_tile, tv, &st.fixed_full, T_HALF_BYTES, kv_head, k0, batch);
+      int a_issued = 0, b_issued = 0;
+      int head = kv_head * p.heads_per_kv, tile = first_tile;
+      for (int j = 0; j < n; ++j) {
+        const int s = j % B_STAGES;
+        const uint32_t ph = (j / B_STAGES) & 1;
+        if (!mbar_wait(&st.a_empty[s], ph ^ 1u, abort)) break;
+        mbar_arrive_expect_tx(&st.a_full[s], T_BYTES + STAT_BYTES);
+        load_rows(q_tiles + s * T_BYTES, tq, &st.a_full[s], T_HALF_BYTES, head, tile * BT, batch);
+        rows::bulk_load(stat_tiles + s * STAT_BYTES,
+                        p.stats + ((static_cast<int64_t>(batch) * p.heads + head) * p.q_tiles + tile) * STAT_FLOATS,
+                        STAT_BYTES, &st.a_full[s]);
+        ++a_issued;
+        if (!mbar_wait(&st.b_empty[s], ph ^ 1u, abort)) break;
+        mbar_arrive_expect_tx(&st.b_full[s], T_BYTES);
+        load_rows(do_tiles + s * T_BYTES, tdo, &st.b_full[s], T_HALF_BYTES, head, tile * BT, batch);
+        ++b_issued;
+        if (++tile == end_tile) {
+          tile = first_tile;
+          ++head;
+        }
+      }
+      if (*abort) {  // let the copies in flight land before the CTA exits
+        mbar_wait(&st.fixed_full, 0, nullptr);
+        for (int j = a_issued - 1; j >= 0 && j >= a_issued - B_STAGES; --j)
+          mbar_wait(&st.a_full[j % B_STAGES], (j / B_STAGES) & 1, nullptr);
+        for (int j = b_issued - 1; j >= 0 && j >= b_issued - B_STAGES; --j)
+          mbar_wait(&st.b_full[j % B_STAGES], (j / B_STAGES) & 1, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      // ---------------------------------------------------------- MMA issuer
+      const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+      const uint32_t k_addr = smem_u32(k_tile), v_addr = smem_u32(v_tile);
+      const uint32_t q_addr = smem_u32(q_tiles), do_addr = smem_u32(do_tiles);
+      uint32_t requests = 0;
+      // Q of tile j in shared memory; in a head's last tile with its rows and dO's past the length zeroed
+      auto q_ready = [&](int j) {
+        const int s = j % B_STAGES;
+        if (!mbar_wait(&st.a_full[s], (j / B_STAGES) & 1, abort)) return false;
+        if (fix && (j + 1) % per_head == 0) {
+          if (!mbar_wait(&st.b_full[s], (j / B_STAGES) & 1, abort)) return false;
+          mbar_arrive(&st.zero_request);
+          if (!mbar_wait(&st.zeroed, requests++ & 1, abort)) return false;
+        }
+        tc_fence_after();
+        return true;
+      };
+      auto issue_s = [&](int j) {
+        mma_tile_ss(t_s, k_addr, q_addr + (j % B_STAGES) * T_BYTES);
+        mma_commit(&st.s_full[0]);
+      };
+      auto issue_dp = [&](int j) {
+        mma_tile_ss(t_dp, v_addr, do_addr + (j % B_STAGES) * T_BYTES);
+        mma_commit(&st.dp_full);
+      };
+      bool ok = mbar_wait(&st.fixed_full, 0, abort) && q_ready(0);
+      if (ok) issue_s(0);
+      ok = ok && mbar_wait(&st.b_full[0], 0, abort);
+      if (ok) {
+        tc_fence_after();
+        issue_dp(0);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const int s = j % B_STAGES;
+        if (!mbar_wait(&st.p_full, j & 1, abort)) break;
+        tc_fence_after();
+        mma_tile_ts(t_dv, t_s, do_addr + s * T_BYTES, j > 0);
+        mma_commit(&st.b_empty[s]);
+        if (j + 1 < n) {
+          if (!q_ready(j + 1)) break;
+          issue_s(j + 1);
+        }
+        if (!mbar_wait(&st.ds_full[0], j & 1, abort)) break;
+        tc_fence_after();
+        mma_tile_ts(t_dk, t_dp, q_addr + s * T_BYTES, j > 0);
+        mma_commit(&st.a_empty[s]);
+        if (j + 1 < n) {
+          const int s1 = (j + 1) % B_STAGES;
+          if (!mbar_wait(&st.b_full[s1], ((j + 1) / B_STAGES) & 1, abort)) break;
+          tc_fence_after();
+          issue_dp(j + 1);
+        }
+      }
+      mma_commit(&st.done);
+      mbar_wait(&st.done, 0, nullptr);
+    }
+  } else if (warp == 2) {
+    if (fix) {
+      // ---------------------------------------------------------- zeroes the rows past the queries' length
+      uint32_t request = 0;
+      for (int j = per_head - 1; j < n; j += per_head) {
+        const int s = j % B_STAGES;
+        const uint32_t ph = (j / B_STAGES) & 1;
+        if (!mbar_wait(&st.zero_request, request++ & 1, abort)) break;
+        if (!mbar_wait(&st.a_full[s], ph, abort) || !mbar_wait(&st.b_full[s], ph, abort)) break;
+        zero_rows(q_tiles + s * T_BYTES, T_HALF_BYTES, vis.q_len % BT, BT, lane);
+        zero_rows(do_tiles + s * T_BYTES, T_HALF_BYTES, vis.q_len % BT, BT, lane);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&st.zeroed);
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax groups
+    const int g = static_cast<int>(warp - 4) >> 2;  // query columns [64g, 64g + 64)
+    const uint32_t quarter = warp & 3;
+    const int key = k0 + static_cast<int>(quarter * 32 + lane);
+    const uint32_t lane_off = (quarter * 32u) << 16;
+    const uint32_t s_tmem = tmem + lane_off + g * 64;
+    const uint32_t dp_tmem = s_tmem + 128;
+    const bool key_ok = key < vis.kv_len;
+    const int first = vis.first(key);
+    // every key row of the tile sees the queries from here on
+    const int all_from = vis.first(min(k0 + BT, vis.kv_len) - 1);
+    const bool ragged_keys = k0 + BT > vis.kv_len;
+    bool ok = true;
+    int tile = first_tile;
+    for (int j = 0; j < n; ++j) {
+      const int s = j % B_STAGES;
+      const int q0 = tile * BT;
+      if (++tile == end_tile) tile = first_tile;
+      const bool masked = ragged_keys || q0 < all_from || q0 + BT > vis.q_len;
+      const int lo = key_ok ? first - q0 - g * 64 : 64;
+      const int hi = vis.q_len - q0 - g * 64;
+      const float* stat = reinterpret_cast<const float*>(stat_tiles + s * STAT_BYTES) + g * 64;
+      if (!mbar_wait(&st.a_full[s], (j / B_STAGES) & 1, abort) || !mbar_wait(&st.s_full[0], j & 1, abort)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float pr[64];
+      tmem_ld32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(&pr[0]));
+      tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&pr[32]));
+      tmem_ld_wait();
+      probabilities(pr, p.scale_log2, [&](int i) { return *reinterpret_cast<const f2*>(stat + i); });
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (i < lo || i >= hi) pr[i] = 0.f;
+      }
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) {
+        uint32_t pk[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pk[i] = pack_bf16x2(pr[cc * 16 + 2 * i], pr[cc * 16 + 2 * i + 1]);
+        tmem_st8(s_tmem + cc * 8, pk);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&st.p_full);
+
+      if (!mbar_wait(&st.dp_full, j & 1, abort)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float dp[32];
+        tmem_ld32(dp_tmem + half * 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int col = half * 32 + 2 * i;
+          const f2 nd = *reinterpret_cast<const f2*>(stat + BT + col);
+          const f2 ds = mul2(f2{pr[col], pr[col + 1]}, add2(f2{dp[2 * i], dp[2 * i + 1]}, nd));
+          dp[2 * i] = ds.x;
+          dp[2 * i + 1] = ds.y;
+        }
+        if (masked) {  // dP of a masked pair may be anything
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (half * 32 + i < lo || half * 32 + i >= hi) dp[i] = 0.f;
+        }
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          uint32_t pk[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pk[i] = pack_bf16x2(dp[cc * 16 + 2 * i], dp[cc * 16 + 2 * i + 1]);
+          tmem_st8(dp_tmem + half * 16 + cc * 8, pk);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&st.ds_full[0]);
+    }
+    if (ok && mbar_wait(&st.done, 0, abort)) {
+      tc_fence_after();
+      __nv_bfloat16* base = g == 0 ? p.dv : p.dk;
+      store_row(tmem + lane_off + (g == 0 ? 256 : 384), HD, g == 0 ? 1.f : p.scale,
+                base + batch * p.dkv_stride_b + key * p.dkv_stride_t + static_cast<int64_t>(kv_head) * HD,
+                key < p.L_kv);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------- dQ
+// One tile of 128 queries; a softmax thread owns one query, so its statistics are two registers.
+//   TMEM: S in two buffers [0,128) [128,256), dP [256,384), dQ [384,512); bf16 dS over its S buffer.
+// P never leaves the registers here.  With two score buffers S(j+1) is ready before the softmax of tile j ends,
+// and dP(j+1) runs as soon as dP(j) is in registers.
+__device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv,
+                                       const CUtensorMap* tdo, const BwdParams& p, BwdShared& st, uint8_t* smem,
+                                       uint32_t tmem) {
+  uint8_t* q_tile = smem;
+  uint8_t* do_tile = smem + T_BYTES;
+  uint8_t* k_tiles = smem + 2 * T_BYTES;
+  uint8_t* v_tiles = k_tiles + DQ_K_STAGES * T_BYTES;
+  const uint32_t warp = warp_idx();
+  const uint32_t lane = threadIdx.x & 31;
+  volatile int* abort = &st.abort;
+
+  const unsigned idx = blockIdx.x - p.dkdv_ctas;
+  const int qt = p.q_tiles - 1 - static_cast<int>(idx % p.q_tiles);  // causal rows get longer with their index
+  const int bh = static_cast<int>(idx / p.q_tiles);
+  const int head = bh % p.heads;
+  const int batch = bh / p.heads;
+  const int kv_head = head / p.heads_per_kv;
+  const int q0 = qt * BT;
+  const Visibility vis{clamp_length(p.q_lengths, batch, p.L), clamp_length(p.kv_lengths, batch, p.L_kv),
+                       p.causal_block, p.L_kv - p.L};
+  const int last = min(q0 + BT, vis.q_len) - 1;
+  const int n = last < q0 ? 0 : (vis.limit(last) + BT - 1) / BT;
+  const int fix_tile = (vis.kv_len < p.L_kv && vis.kv_len % BT != 0 && vis.kv_len / BT < n) ? vis.kv_len / BT : -1;
+
+  if (n == 0) {
+    if (warp >= 4) {
+      const int token = q0 + static_cast<int>((warp & 3) * 32 + lane);
+      if (token < p.L)
+        zero_row(p.dq + batch * p.dq_stride_b + token * p.dq_stride_t + static_cast<int64_t>(head) * HD +
+                     (warp < 8 ? 0 : 64),
+                 64);
+    }
+    return;
+  }
+
+  if (warp == 0) {
+    if (elect_one()) {
+      // ---------------------------------------------------------- TMA producer
+      mbar_arrive_expect_tx(&st.fixed_full, 2 * T_BYTES);
+      load_rows(q_tile, tq, &st.fixed_full, T_HALF_BYTES, head, q0, batch);
+      load_rows(do_tile, tdo, &st.fixed_full, T_HALF_BYTES, head, q0, batch);
+      int a_issued = 0, b_issued = 0;
+      for (int j = 0; j < n; ++j) {
+        const int sk = j % DQ_K_STAGES, sv = j % B_STAGES;
+        if (!mbar_wait(&st.a_empty[sk], ((j / DQ_K_STAGES) & 1) ^ 1u, abort)) break;
+        mbar_arrive_expect_tx(&st.a_full[sk], T_BYTES);
+        load_rows(k_tiles + sk * T_BYTES, tk, &st.a_full[sk], T_HALF_BYTES, kv_head, j * BT, batch);
+        ++a_issued;
+        if (!mbar_wait(&st.b_empty[sv], ((j / B_STAGES) & 1) ^ 1u, abort)) break;
+        mbar_arrive_expect_tx(&st.b_full[sv], T_BYTES);
+        load_rows(v_tiles + sv * T_BYTES, tv, &st.b_full[sv], T_HALF_BYTES, kv_head, j * BT, batch);
+        ++b_issued;
+      }
+      if (*abort) {  // let the copies in flight land before the CTA exits
+        mbar_wait(&st.fixed_full, 0, nullptr);
+        for (int j = a_issued - 1; j >= 0 && j >= a_issued - DQ_K_STAGES; --j)
+          mbar_wait(&st.a_full[j % DQ_K_STAGES], (j / DQ_K_STAGES) & 1, nullptr);
+        for (int j = b_issued - 1; j >= 0 && j >= b_issued - B_STAGES; --j)
+          mbar_wait(&st.b_full[j % B_STAGES], (j / B_STAGES) & 1, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      // ---------------------------------------------------------- MMA issuer
+      const uint32_t t_dp = tmem + 256, t_dq = tmem + 384;
+      const uint32_t q_addr = smem_u32(q_tile), do_addr = smem_u32(do_tile);
+      const uint32_t k_addr = smem_u32(k_tiles), v_addr = smem_u32(v_tiles);
+      auto issue_s = [&](int j) {
+        if (!mbar_wait(&st.a_full[j % DQ_K_STAGES], (j / DQ_K_STAGES) & 1, abort)) return false;
+        if (j == fix_tile) {
+          mbar_arrive(&st.zero_request);
+          if (!mbar_wait(&st.zeroed, 0, abort)) return false;
+        }
+        tc_fence_after();
+        mma_tile_ss(tmem + (j & 1) * 128, q_addr, k_addr + (j % DQ_K_STAGES) * T_BYTES);
+        mma_commit(&st.s_full[j & 1]);
+        return true;
+      };
+      auto issue_dp = [&](int j) {
+        if (!mbar_wait(&st.b_full[j % B_STAGES], (j / B_STAGES) & 1, abort)) return false;
+        tc_fence_after();
+        mma_tile_ss(t_dp, do_addr, v_addr + (j % B_STAGES) * T_BYTES);
+        mma_commit(&st.dp_full);
+        mma_commit(&st.b_empty[j % B_STAGES]);
+        return true;
+      };
+      bool ok = mbar_wait(&st.fixed_full, 0, abort) && issue_s(0) && issue_dp(0) && (n < 2 || issue_s(1));
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) {
+          if (!mbar_wait(&st.dp_read, j & 1, abort)) break;
+          if (!issue_dp(j + 1)) break;
+        }
+        if (!mbar_wait(&st.ds_full[j & 1], (j >> 1) & 1, abort)) break;
+        tc_fence_after();
+        mma_tile_ts(t_dq, tmem + (j & 1) * 128, k_addr + (j % DQ_K_STAGES) * T_BYTES, j > 0);
+        mma_commit(&st.a_empty[j % DQ_K_STAGES]);
+        if (j + 2 < n && !issue_s(j + 2)) break;
+      }
+      mma_commit(&st.done);
+      mbar_wait(&st.done, 0, nullptr);
+    }
+  } else if (warp == 2) {
+    if (fix_tile >= 0) {
+      // ---------------------------------------------------------- zeroes the K rows past the keys' length
+      const int s = fix_tile % DQ_K_STAGES;
+      if (mbar_wait(&st.zero_request, 0, abort) && mbar_wait(&st.a_full[s], (fix_tile / DQ_K_STAGES) & 1, abort)) {
+        zero_rows(k_tiles + s * T_BYTES, T_HALF_BYTES, vis.kv_len % BT, BT, lane);
+        fence_async_shared();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&st.zeroed);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax groups
+    const int g = static_cast<int>(warp - 4) >> 2;  // key columns [64g, 64g + 64)
+    const uint32_t quarter = warp & 3;
+    const int row = static_cast<int>(quarter * 32 + lane);
+    const int token = q0 + row;
+    const uint32_t lane_off = (quarter * 32u) << 16;
+    const uint32_t dp_tmem = tmem + lane_off + 256 + g * 64;
+    const float* stat = p.stats + ((static_cast<int64_t>(batch) * p.heads + head) * p.q_tiles + qt) * STAT_FLOATS + row;
+    const float nl = stat[0], nd = stat[BT];
+    const int limit = vis.limit(token);
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int b = j & 1;
+      const uint32_t s_tmem = tmem + lane_off + b * 128 + g * 64;
+      const int valid = limit - j * BT - g * 64;  // columns of this thread's 64 that its query sees
+      const bool masked = __any_sync(0xffffffffu, valid < 64);
+      if (!mbar_wait(&st.s_full[b], (j >> 1) & 1, abort)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float pr[64];
+      tmem_ld32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(&pr[0]));
+      tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&pr[32]));
+      tmem_ld_wait();
+      probabilities(pr, p.scale_log2, [&](int) { return f2{nl, nl}; });
+      if (!mbar_wait(&st.dp_full, j & 1, abort)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float dp[32];
+        tmem_ld32(dp_tmem + half * 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
+        tmem_ld_wait();
+        if (half == 1) {
+          tc_fence_before();
+          mbar_arrive(&st.dp_read);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int col = half * 32 + 2 * i;
+          const f2 ds = mul2(f2{pr[col], pr[col + 1]}, add2(f2{dp[2 * i], dp[2 * i + 1]}, f2{nd, nd}));
+          dp[2 * i] = ds.x;
+          dp[2 * i + 1] = ds.y;
+        }
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (half * 32 + i >= valid) dp[i] = 0.f;
+        }
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          uint32_t pk[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pk[i] = pack_bf16x2(dp[cc * 16 + 2 * i], dp[cc * 16 + 2 * i + 1]);
+          tmem_st8(s_tmem + half * 16 + cc * 8, pk);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&st.ds_full[b]);
+    }
+    if (ok && mbar_wait(&st.done, 0, abort)) {
+      tc_fence_after();
+      store_row(tmem + lane_off + 384 + g * 64, 64, p.scale,
+                p.dq + batch * p.dq_stride_b + token * p.dq_stride_t + static_cast<int64_t>(head) * HD + g * 64,
+                token < p.L);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                    const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo, BwdParams p) {
+  pdl_trigger();
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ BwdShared st;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t warp = warp_idx();
+  if (threadIdx.x == 0) {
+    mbar_init(&st.fixed_full, 1);
+    for (int s = 0; s < DQ_K_STAGES; ++s) {
+      mbar_init(&st.a_full[s], 1);
+      mbar_init(&st.a_empty[s], 1);
+    }
+    for (int s = 0; s < B_STAGES; ++s) {
+      mbar_init(&st.b_full[s], 1);
+      mbar_init(&st.b_empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&st.s_full[b], 1);
+      mbar_init(&st.ds_full[b], 256);
+    }
+    mbar_init(&st.p_full, 256);
+    mbar_init(&st.dp_full, 1);
+    mbar_init(&st.dp_read, 256);
+    mbar_init(&st.zero_request, 1);
+    mbar_init(&st.zeroed, 1);
+    mbar_init(&st.done, 1);
+    st.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&st.tmem_base, TMEM_COLS);
+    tmem_relinquish();
+  }
+  pdl_wait();  // everything above touches only this CTA's shared memory and TMEM
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = st.tmem_base;
+  if (blockIdx.x < p.dkdv_ctas)
+    bwd_dkdv(&tq, &tk, &tv, &tdo, p, st, smem, tmem);
+  else
+    bwd_dq(&tq, &tk, &tv, &tdo, p, st, smem, tmem);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+}  // namespace attn
+}  // namespace ogx

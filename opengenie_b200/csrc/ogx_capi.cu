@@ -20,6 +20,8 @@
 #include "../../include/ogx.h"
 #include "elementwise.cuh"
 #include "attention.cuh"
+#include "attention_bwd.cuh"
+#include "qk_norm.cuh"
 #include "rows.cuh"
 #include "fp8_gemm.cuh"
 #include "peer.cuh"
@@ -902,6 +904,18 @@ int attention_common(const void* q, const void* k, const void* v, int64_t batch,
   return make_map(mv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v, kvdims, kvstrides, vbox);
 }
 
+// The softmax warpgroups raise their register limit with setmaxnreg, drawing on the registers the
+// launch reserved; only launch a build whose per-thread count is the one the split was sized for.
+int attn_register_split_ok(const void* kern) {
+  cudaFuncAttributes attr;
+  int rc = check_cuda(cudaFuncGetAttributes(&attr, kern), "cudaFuncGetAttributes");
+  if (rc) return rc;
+  if (attr.numRegs != ogx::attn::kLaunchRegs)
+    return fail(OGX_ECUDA, "attention kernel built with %d registers per thread, the register split needs %d", attr.numRegs,
+                ogx::attn::kLaunchRegs);
+  return OGX_OK;
+}
+
 template <bool E4M3>
 int attention_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, int64_t batch,
                      int64_t tokens, int64_t heads, const ogx::attn::Params& p, cudaStream_t s) {
@@ -919,14 +933,7 @@ int attention_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtenso
   auto kern = ogx::attn::attn_fwd_kernel<E4M3>;
   int rc = ensure_smem(kern, ogx::attn::SMEM_BYTES);
   if (rc) return rc;
-  // The softmax warpgroups raise their register limit with setmaxnreg, drawing on the registers the
-  // launch reserved; only launch a build whose per-thread count is the one the split was sized for.
-  cudaFuncAttributes attr;
-  rc = check_cuda(cudaFuncGetAttributes(&attr, kern), "cudaFuncGetAttributes");
-  if (rc) return rc;
-  if (attr.numRegs != ogx::attn::kLaunchRegs)
-    return fail(OGX_ECUDA, "attention kernel built with %d registers per thread, the register split needs %d", attr.numRegs,
-                ogx::attn::kLaunchRegs);
+  if ((rc = attn_register_split_ok(reinterpret_cast<const void*>(kern)))) return rc;
   const dim3 grid(static_cast<unsigned>((tokens + 255) / 256), static_cast<unsigned>(heads),
                   static_cast<unsigned>(batch));
   launch(kern, grid, ogx::attn::kThreads, ogx::attn::SMEM_BYTES, s, mq, mk, mv, p);
@@ -1419,6 +1426,408 @@ int ogx_peer_barrier_static(int rank, int world, const int* devices, unsigned in
   return check_cuda(cudaMemcpyAsync(count_out, local + ogx::kPeerCountWord, sizeof(unsigned int),
                                     cudaMemcpyDeviceToDevice, s),
                     "cudaMemcpyAsync");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------- training pass: attention with statistics, gradients
+namespace {
+
+// {d, head, token, batch} map of bf16 rows of heads * 128 columns; a box is 64 columns of `box_rows` tokens.
+int token_map(CUtensorMap* map, const void* base, int64_t heads, int64_t tokens, int64_t batch, int64_t stride_t,
+              int64_t stride_b, int box_rows) {
+  const uint64_t dims[4] = {128, static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens),
+                            static_cast<uint64_t>(batch)};
+  const uint64_t strides[3] = {256, static_cast<uint64_t>(stride_t) * 2, static_cast<uint64_t>(stride_b) * 2};
+  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(box_rows), 1};
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box);
+}
+
+bool row_strides_ok(int64_t width, int64_t tokens, int64_t batch, int64_t stride_t, int64_t stride_b) {
+  if (stride_t % 8 || stride_b % 8 || stride_t < width || stride_b < 0) return false;
+  // a tensor map holds strides below 2^40 bytes
+  return stride_t < (int64_t{1} << 38) && (batch == 1 || stride_b < (int64_t{1} << 38)) && tokens > 0;
+}
+
+int masked_attention_guard(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
+                           int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
+                           int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t, float softmax_scale,
+                           int64_t causal_block) {
+  if (q == nullptr || k == nullptr || v == nullptr) return fail(OGX_EINVAL, "null_pointer");
+  if (head_dim != 128) return fail(OGX_EINVAL, "head_dim: only 128 is supported");
+  if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1 || kv_heads < 1) return fail(OGX_EINVAL, "shape");
+  // positions and tile ends stay below 2^31
+  constexpr int64_t kMost = int64_t{1} << 29;
+  if (q_tokens > kMost || kv_tokens > kMost || heads > 65535 || batch > 65535) return fail(OGX_EINVAL, "shape");
+  if (heads % kv_heads) return fail(OGX_EINVAL, "kv_heads: heads must be a multiple of kv_heads");
+  if (causal_block < 0 || causal_block > kMost) return fail(OGX_EINVAL, "causal_block");
+  if (!(softmax_scale > 0.f) || softmax_scale > 3.0e38f) return fail(OGX_EINVAL, "softmax_scale");
+  if (!row_strides_ok(heads * 128, q_tokens, batch, q_stride_t, q_stride_b) ||
+      !row_strides_ok(kv_heads * 128, kv_tokens, batch, kv_stride_t, kv_stride_b))
+    return fail(OGX_EINVAL, "stride");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return fail(OGX_EINVAL, "alignment");
+  return OGX_OK;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int64_t bwd_tiles(int64_t tokens) { return (tokens + ogx::attn::BT - 1) / ogx::attn::BT; }
+
+int64_t bwd_stats_bytes(int64_t batch, int64_t q_tokens, int64_t heads) {
+  return batch * heads * bwd_tiles(q_tokens) * ogx::attn::STAT_BYTES;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
+                          int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
+                          int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t, float softmax_scale,
+                          int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
+                          int64_t out_stride_b, int64_t out_stride_t, float* lse, void* stream) {
+  int rc = masked_attention_guard(q, k, v, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, q_stride_b,
+                                  q_stride_t, kv_stride_b, kv_stride_t, softmax_scale, causal_block);
+  if (rc) return rc;
+  if (out == nullptr || !aligned16(out) || !row_strides_ok(heads * 128, q_tokens, batch, out_stride_t, out_stride_b))
+    return fail(OGX_EINVAL, "output");
+  if (lse == nullptr || !aligned4(lse)) return fail(OGX_EINVAL, "lse");
+  if (!aligned4(q_lengths) || !aligned4(kv_lengths)) return fail(OGX_EINVAL, "lengths");
+  CUtensorMap mq, mk, mv;
+  if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BQ))) return rc;
+  if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, kv_stride_t, kv_stride_b, ogx::attn::BKV))) return rc;
+  if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, kv_stride_t, kv_stride_b, ogx::attn::BKV))) return rc;
+  ogx::attn::Params p{};
+  p.L = static_cast<int>(q_tokens);
+  p.L_kv = static_cast<int>(kv_tokens);
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_stride_b = out_stride_b;
+  p.out_stride_t = out_stride_t;
+  p.lse = lse;
+  p.heads_per_kv = static_cast<int>(heads / kv_heads);
+  p.causal_block = static_cast<int>(causal_block);
+  p.q_lengths = q_lengths;
+  p.kv_lengths = kv_lengths;
+  auto kern = ogx::attn::attn_fwd_kernel<false, true>;
+  if ((rc = attn_register_split_ok(reinterpret_cast<const void*>(kern)))) return rc;
+  if ((rc = ensure_smem(kern, ogx::attn::SMEM_BYTES))) return rc;
+  const dim3 grid(static_cast<unsigned>((q_tokens + 255) / 256), static_cast<unsigned>(heads),
+                  static_cast<unsigned>(batch));
+  launch(kern, grid, ogx::attn::kThreads, ogx::attn::SMEM_BYTES, static_cast<cudaStream_t>(stream), mq, mk, mv, p);
+  return check_launch("attn_fwd_kernel");
+}
+
+int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads,
+                                int64_t* bytes) {
+  if (bytes == nullptr) return fail(OGX_EINVAL, "null_pointer");
+  if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1 || kv_heads < 1) return fail(OGX_EINVAL, "shape");
+  *bytes = bwd_stats_bytes(batch, q_tokens, heads);
+  return OGX_OK;
+}
+
+int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                      const float* lse, int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
+                      int64_t kv_heads, int64_t head_dim, int64_t dout_stride_b, int64_t dout_stride_t,
+                      int64_t q_stride_b, int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t,
+                      int64_t out_stride_b, int64_t out_stride_t, float softmax_scale, int64_t causal_block,
+                      const int* q_lengths, const int* kv_lengths, void* workspace, int64_t workspace_bytes, void* dq,
+                      int64_t dq_stride_b, int64_t dq_stride_t, void* dk, void* dv, int64_t dkv_stride_b,
+                      int64_t dkv_stride_t, void* stream) {
+  int rc = masked_attention_guard(q, k, v, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, q_stride_b,
+                                  q_stride_t, kv_stride_b, kv_stride_t, softmax_scale, causal_block);
+  if (rc) return rc;
+  const int64_t width = heads * 128, kv_width = kv_heads * 128;
+  if (dout == nullptr || out == nullptr || !aligned16(dout) || !aligned16(out) ||
+      !row_strides_ok(width, q_tokens, batch, dout_stride_t, dout_stride_b) ||
+      !row_strides_ok(width, q_tokens, batch, out_stride_t, out_stride_b))
+    return fail(OGX_EINVAL, "dout_or_out");
+  if (lse == nullptr || !aligned4(lse)) return fail(OGX_EINVAL, "lse");
+  if (!aligned4(q_lengths) || !aligned4(kv_lengths)) return fail(OGX_EINVAL, "lengths");
+  if (dq == nullptr || dk == nullptr || dv == nullptr || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
+      !row_strides_ok(width, q_tokens, batch, dq_stride_t, dq_stride_b) ||
+      !row_strides_ok(kv_width, kv_tokens, batch, dkv_stride_t, dkv_stride_b))
+    return fail(OGX_EINVAL, "gradients");
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < bwd_stats_bytes(batch, q_tokens, heads))
+    return fail(OGX_EINVAL, "workspace");
+  const int64_t q_tiles = bwd_tiles(q_tokens), kv_tiles = bwd_tiles(kv_tokens);
+  const int64_t dkdv_ctas = kv_tiles * kv_heads * batch, dq_ctas = q_tiles * heads * batch;
+  if (dkdv_ctas + dq_ctas > INT32_MAX) return fail(OGX_EINVAL, "shape");
+  CUtensorMap mq, mk, mv, mdo;
+  if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BT))) return rc;
+  if ((rc = token_map(&mdo, dout, heads, q_tokens, batch, dout_stride_t, dout_stride_b, ogx::attn::BT))) return rc;
+  if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, kv_stride_t, kv_stride_b, ogx::attn::BT))) return rc;
+  if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, kv_stride_t, kv_stride_b, ogx::attn::BT))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+
+  ogx::attn::StatsParams sp{};
+  sp.dout = static_cast<const __nv_bfloat16*>(dout);
+  sp.out = static_cast<const __nv_bfloat16*>(out);
+  sp.dout_stride_b = dout_stride_b;
+  sp.dout_stride_t = dout_stride_t;
+  sp.out_stride_b = out_stride_b;
+  sp.out_stride_t = out_stride_t;
+  sp.lse = lse;
+  sp.q_lengths = q_lengths;
+  sp.stats = static_cast<float*>(workspace);
+  sp.L = static_cast<int>(q_tokens);
+  sp.heads = static_cast<int>(heads);
+  sp.q_tiles = static_cast<int>(q_tiles);
+  sp.rows = batch * q_tiles * ogx::attn::BT * heads;
+  launch(ogx::attn::attn_bwd_stats_kernel, dim3(static_cast<unsigned>(grid_for(sp.rows * 16))), 256, 0, s, sp);
+  if ((rc = check_launch("attn_bwd_stats_kernel"))) return rc;
+
+  ogx::attn::BwdParams p{};
+  p.L = static_cast<int>(q_tokens);
+  p.L_kv = static_cast<int>(kv_tokens);
+  p.heads = static_cast<int>(heads);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.heads_per_kv = static_cast<int>(heads / kv_heads);
+  p.q_tiles = static_cast<int>(q_tiles);
+  p.kv_tiles = static_cast<int>(kv_tiles);
+  p.dkdv_ctas = static_cast<unsigned>(dkdv_ctas);
+  p.causal_block = static_cast<int>(causal_block);
+  p.scale = softmax_scale;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.q_lengths = q_lengths;
+  p.kv_lengths = kv_lengths;
+  p.stats = sp.stats;
+  p.dq = static_cast<__nv_bfloat16*>(dq);
+  p.dk = static_cast<__nv_bfloat16*>(dk);
+  p.dv = static_cast<__nv_bfloat16*>(dv);
+  p.dq_stride_b = dq_stride_b;
+  p.dq_stride_t = dq_stride_t;
+  p.dkv_stride_b = dkv_stride_b;
+  p.dkv_stride_t = dkv_stride_t;
+  auto kern = ogx::attn::attn_bwd_kernel;
+  if ((rc = ensure_smem(kern, ogx::attn::BWD_SMEM))) return rc;
+  launch(kern, dim3(static_cast<unsigned>(dkdv_ctas + dq_ctas)), ogx::attn::kBwdThreads, ogx::attn::BWD_SMEM, s, mq, mk,
+         mv, mdo, p);
+  return check_launch("attn_bwd_kernel");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------- Q/K norm + rotation and its gradients
+namespace {
+
+using ogx::qkn::kHead;
+using ogx::qkn::kNone;
+using ogx::qkn::kRow;
+
+constexpr int kQkMaxHeads = 128;  // q's and k's together: 8 head slots of 16 groups
+
+int pow2_at_least(int64_t n) {
+  int p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+
+struct QkShape {
+  int groups, team, teams, steps;
+};
+
+// A token's team has as many groups as heads, up to the CTA's; the groups' head slots are a compile-time number.
+QkShape qk_shape(int64_t all_heads, int64_t head_dim) {
+  QkShape r{};
+  r.groups = ogx::qkn::kThreads / static_cast<int>(head_dim / 8);
+  r.team = pow2_at_least(all_heads);
+  if (r.team > r.groups) r.team = r.groups;
+  r.teams = r.groups / r.team;
+  r.steps = pow2_at_least((all_heads + r.team - 1) / r.team);
+  return r;
+}
+
+int64_t qk_grid(const QkShape& sh, int64_t rows) {
+  const int64_t want = (rows + sh.teams - 1) / sh.teams;
+  const int64_t cap = static_cast<int64_t>(sm_count()) * 4;
+  return want < cap ? want : cap;
+}
+
+int64_t qk_weight_columns(int norm, int64_t all_heads, int64_t head_dim) {
+  return norm == kNone ? 0 : (norm == kHead ? 2 * head_dim : all_heads * head_dim);
+}
+
+int64_t qk_partial_rows(const QkShape& sh, int norm, int64_t grid) { return norm == kRow ? grid * sh.teams : grid; }
+
+template <int HD, int STEPS, bool BACKWARD>
+void qk_dispatch_norm(const ogx::qkn::Params& p, int norm, int64_t grid, cudaStream_t s) {
+  const dim3 g(static_cast<unsigned>(grid)), b(ogx::qkn::kThreads);
+  if (norm == kNone) return launch(ogx::qkn::qk_norm_rope_kernel<HD, STEPS, kNone, BACKWARD>, g, b, 0, s, p);
+  if (norm == kHead) return launch(ogx::qkn::qk_norm_rope_kernel<HD, STEPS, kHead, BACKWARD>, g, b, 0, s, p);
+  return launch(ogx::qkn::qk_norm_rope_kernel<HD, STEPS, kRow, BACKWARD>, g, b, 0, s, p);
+}
+
+template <int HD, bool BACKWARD>
+void qk_dispatch_steps(const ogx::qkn::Params& p, int steps, int norm, int64_t grid, cudaStream_t s) {
+  switch (steps) {
+    case 1: return qk_dispatch_norm<HD, 1, BACKWARD>(p, norm, grid, s);
+    case 2: return qk_dispatch_norm<HD, 2, BACKWARD>(p, norm, grid, s);
+    case 4: return qk_dispatch_norm<HD, 4, BACKWARD>(p, norm, grid, s);
+    default: return qk_dispatch_norm<HD, 8, BACKWARD>(p, norm, grid, s);
+  }
+}
+
+template <bool BACKWARD>
+void qk_dispatch(const ogx::qkn::Params& p, int64_t head_dim, int steps, int norm, int64_t grid, cudaStream_t s) {
+  if (head_dim == 128) return qk_dispatch_steps<128, BACKWARD>(p, steps, norm, grid, s);
+  return qk_dispatch_steps<64, BACKWARD>(p, steps, norm, grid, s);
+}
+
+int qk_norm_guard(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                  int64_t head_dim, int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
+                  const void* q_weight, const void* k_weight, int weight_dtype, int norm, float eps, const void* cos,
+                  const void* sin, int cs_dtype, int64_t rotary, int64_t cs_stride_b, int64_t cs_stride_h,
+                  int64_t cs_stride_t) {
+  if (q == nullptr || k == nullptr) return fail(OGX_EINVAL, "null_pointer");
+  if (head_dim != 64 && head_dim != 128) return fail(OGX_EINVAL, "head_dim: 64 or 128");
+  if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || heads > kQkMaxHeads || kv_heads > kQkMaxHeads ||
+      heads + kv_heads > kQkMaxHeads)
+    return fail(OGX_EINVAL, "qk_shape");
+  if (tokens > INT32_MAX || batch > INT32_MAX) return fail(OGX_EINVAL, "qk_shape");
+  if (q_stride_b % 8 || q_stride_t % 8 || k_stride_b % 8 || k_stride_t % 8) return fail(OGX_EINVAL, "qk_noncontiguous");
+  if (norm != kNone && norm != kHead && norm != kRow) return fail(OGX_EINVAL, "norm");
+  if (norm != kNone && (q_weight == nullptr || k_weight == nullptr || !dtype_ok(weight_dtype)))
+    return fail(OGX_EINVAL, "qk_weight_shape");
+  if (!(eps >= 0.f)) return fail(OGX_EINVAL, "eps");
+  if (cos == nullptr || sin == nullptr || !dtype_ok(cs_dtype)) return fail(OGX_EINVAL, "rope_shape");
+  if (rotary < 16 || rotary % 16 || rotary > head_dim) return fail(OGX_EINVAL, "rope_shape: rotary columns");
+  if (cs_stride_b % 8 || cs_stride_h % 8 || cs_stride_t % 8) return fail(OGX_EINVAL, "rope_shape: stride");
+  if (cs_stride_h != 0 && heads != kv_heads) return fail(OGX_EINVAL, "rope_shape: tables for each head");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(q_weight) || !aligned16(k_weight) || !aligned16(cos) ||
+      !aligned16(sin))
+    return fail(OGX_EINVAL, "alignment");
+  return OGX_OK;
+}
+
+// The part of the parameters both directions share.
+ogx::qkn::Params qk_params(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                           int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
+                           const void* q_weight, const void* k_weight, int weight_dtype, float eps, const void* cos,
+                           const void* sin, int cs_dtype, int64_t rotary, int interleaved, int64_t cs_stride_b, int64_t cs_stride_h,
+                           int64_t cs_stride_t, const QkShape& sh) {
+  ogx::qkn::Params p{};
+  p.x[0] = static_cast<const __nv_bfloat16*>(q);
+  p.x[1] = static_cast<const __nv_bfloat16*>(k);
+  p.x_stride_b[0] = q_stride_b;
+  p.x_stride_t[0] = q_stride_t;
+  p.x_stride_b[1] = k_stride_b;
+  p.x_stride_t[1] = k_stride_t;
+  p.weight[0] = q_weight;
+  p.weight[1] = k_weight;
+  p.cos = cos;
+  p.sin = sin;
+  p.cs_stride_b = cs_stride_b;
+  p.cs_stride_h = cs_stride_h;
+  p.cs_stride_t = cs_stride_t;
+  p.heads[0] = static_cast<int>(heads);
+  p.heads[1] = static_cast<int>(kv_heads);
+  p.rotary = static_cast<int>(rotary);
+  p.interleaved = interleaved != 0;
+  p.w_fp32 = weight_dtype == OGX_DTYPE_F32;
+  p.cs_fp32 = cs_dtype == OGX_DTYPE_F32;
+  p.team = sh.team;
+  p.tokens = tokens;
+  p.rows = batch * tokens;
+  p.eps = eps;
+  return p;
+}
+
+int qk_outputs(ogx::qkn::Params& p, void* y_q, int64_t q_stride_b, int64_t q_stride_t, void* y_k, int64_t k_stride_b,
+               int64_t k_stride_t) {
+  if (y_q == nullptr || y_k == nullptr || !aligned16(y_q) || !aligned16(y_k) || q_stride_b % 8 || q_stride_t % 8 ||
+      k_stride_b % 8 || k_stride_t % 8)
+    return fail(OGX_EINVAL, "output");
+  p.y[0] = static_cast<__nv_bfloat16*>(y_q);
+  p.y[1] = static_cast<__nv_bfloat16*>(y_k);
+  p.y_stride_b[0] = q_stride_b;
+  p.y_stride_t[0] = q_stride_t;
+  p.y_stride_b[1] = k_stride_b;
+  p.y_stride_t[1] = k_stride_t;
+  return OGX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ogx_qk_norm_rope(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                     int64_t head_dim, int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
+                     const void* q_weight, const void* k_weight, int weight_dtype, int norm, float eps,
+                     const void* cos, const void* sin, int cs_dtype, int64_t rotary, int interleaved,
+                     int64_t cs_stride_b, int64_t cs_stride_h, int64_t cs_stride_t, void* q_out, int64_t q_out_stride_b,
+                     int64_t q_out_stride_t, void* k_out, int64_t k_out_stride_b, int64_t k_out_stride_t,
+                     void* stream) {
+  int rc = qk_norm_guard(q, k, batch, tokens, heads, kv_heads, head_dim, q_stride_b, q_stride_t, k_stride_b, k_stride_t,
+                         q_weight, k_weight, weight_dtype, norm, eps, cos, sin, cs_dtype, rotary, cs_stride_b,
+                         cs_stride_h, cs_stride_t);
+  if (rc) return rc;
+  const QkShape sh = qk_shape(heads + kv_heads, head_dim);
+  ogx::qkn::Params p = qk_params(q, k, batch, tokens, heads, kv_heads, q_stride_b, q_stride_t, k_stride_b, k_stride_t,
+                                 q_weight, k_weight, weight_dtype, eps, cos, sin, cs_dtype, rotary, interleaved,
+                                 cs_stride_b, cs_stride_h, cs_stride_t, sh);
+  if ((rc = qk_outputs(p, q_out, q_out_stride_b, q_out_stride_t, k_out, k_out_stride_b, k_out_stride_t))) return rc;
+  qk_dispatch<false>(p, head_dim, sh.steps, norm, qk_grid(sh, p.rows), static_cast<cudaStream_t>(stream));
+  return check_launch("qk_norm_rope_kernel");
+}
+
+int ogx_qk_norm_rope_bwd_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                   int norm, int64_t* bytes) {
+  if (bytes == nullptr) return fail(OGX_EINVAL, "null_pointer");
+  if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || heads > kQkMaxHeads || kv_heads > kQkMaxHeads ||
+      heads + kv_heads > kQkMaxHeads || (head_dim != 64 && head_dim != 128))
+    return fail(OGX_EINVAL, "qk_shape");
+  const QkShape sh = qk_shape(heads + kv_heads, head_dim);
+  *bytes = 4 * qk_partial_rows(sh, norm, qk_grid(sh, batch * tokens)) *
+           qk_weight_columns(norm, heads + kv_heads, head_dim);
+  return OGX_OK;
+}
+
+int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq_out_stride_t, const void* dk_out,
+                         int64_t dk_out_stride_b, int64_t dk_out_stride_t, const void* q, const void* k, int64_t batch,
+                         int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
+                         int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, const void* q_weight,
+                         const void* k_weight, int weight_dtype, int norm, float eps, const void* cos, const void* sin,
+                         int cs_dtype, int64_t rotary, int interleaved, int64_t cs_stride_b, int64_t cs_stride_h,
+                         int64_t cs_stride_t, void* dq, int64_t dq_stride_b, int64_t dq_stride_t, void* dk,
+                         int64_t dk_stride_b, int64_t dk_stride_t, float* dq_weight, float* dk_weight, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  int rc = qk_norm_guard(q, k, batch, tokens, heads, kv_heads, head_dim, q_stride_b, q_stride_t, k_stride_b, k_stride_t,
+                         q_weight, k_weight, weight_dtype, norm, eps, cos, sin, cs_dtype, rotary, cs_stride_b,
+                         cs_stride_h, cs_stride_t);
+  if (rc) return rc;
+  if (dq_out == nullptr || dk_out == nullptr || !aligned16(dq_out) || !aligned16(dk_out) || dq_out_stride_b % 8 ||
+      dq_out_stride_t % 8 || dk_out_stride_b % 8 || dk_out_stride_t % 8)
+    return fail(OGX_EINVAL, "output_gradients");
+  const QkShape sh = qk_shape(heads + kv_heads, head_dim);
+  ogx::qkn::Params p = qk_params(q, k, batch, tokens, heads, kv_heads, q_stride_b, q_stride_t, k_stride_b, k_stride_t,
+                                 q_weight, k_weight, weight_dtype, eps, cos, sin, cs_dtype, rotary, interleaved,
+                                 cs_stride_b, cs_stride_h, cs_stride_t, sh);
+  p.dy[0] = static_cast<const __nv_bfloat16*>(dq_out);
+  p.dy[1] = static_cast<const __nv_bfloat16*>(dk_out);
+  p.dy_stride_b[0] = dq_out_stride_b;
+  p.dy_stride_t[0] = dq_out_stride_t;
+  p.dy_stride_b[1] = dk_out_stride_b;
+  p.dy_stride_t[1] = dk_out_stride_t;
+  if ((rc = qk_outputs(p, dq, dq_stride_b, dq_stride_t, dk, dk_stride_b, dk_stride_t))) return rc;
+  const int64_t grid = qk_grid(sh, p.rows);
+  const int64_t columns = qk_weight_columns(norm, heads + kv_heads, head_dim);
+  const int64_t partial_rows = qk_partial_rows(sh, norm, grid);
+  if (norm != kNone) {
+    if (dq_weight == nullptr || dk_weight == nullptr || !aligned4(dq_weight) || !aligned4(dk_weight))
+      return fail(OGX_EINVAL, "weight_gradients");
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < 4 * partial_rows * columns)
+      return fail(OGX_EINVAL, "workspace");
+  }
+  p.partials = static_cast<float*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  qk_dispatch<true>(p, head_dim, sh.steps, norm, grid, s);
+  if ((rc = check_launch("qk_norm_rope_kernel"))) return rc;
+  if (norm == kNone) return OGX_OK;
+  launch(ogx::qkn::qk_norm_weight_sum_kernel, dim3(static_cast<unsigned>((columns + 31) / 32)), dim3(1024), 0, s,
+         static_cast<const float*>(p.partials), static_cast<int>(partial_rows), static_cast<int>(columns),
+         static_cast<int>(norm == kHead ? head_dim : heads * head_dim), dq_weight, dk_weight);
+  return check_launch("qk_norm_weight_sum_kernel");
 }
 
 }  // extern "C"

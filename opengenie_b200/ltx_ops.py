@@ -13,12 +13,15 @@ only read inputs and write outputs, on the current CUDA stream.
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import DTYPE_BF16, DTYPE_F16, DTYPE_F32, QUANT_SINGLE, QUANT_TORCH
+from ._lib import (
+    DTYPE_BF16, DTYPE_F16, DTYPE_F32, NORM_HEAD, NORM_NONE, NORM_ROW, QUANT_SINGLE, QUANT_TORCH,
+)
 
 # Call counters, as the reference keeps them (triton_ltx_ops.py:1902-1946).
 _VIDEO_ADA_VALUES_CALLS = 0
@@ -1046,6 +1049,325 @@ def attention(
     return out
 
 
+# ---------------------------------------------------------------- training pass: attention and its gradients
+def _row_strides(t: torch.Tensor) -> tuple[int, int]:
+    """(batch stride, token stride) of rows [B, L, C]; axes of one entry count as contiguous."""
+    B, L, C = t.shape
+    stride_t = t.stride(1) if L > 1 else C
+    return (t.stride(0) if B > 1 else L * stride_t), stride_t
+
+
+def _rows_ok(t: torch.Tensor, *, written: bool = False) -> bool:
+    """bf16 rows the kernels can address: unit column stride, 16-byte aligned rows that do not overlap."""
+    stride_b, stride_t = _row_strides(t)
+    ok = (t.stride(-1) == 1 and stride_t % 8 == 0 and stride_b % 8 == 0 and stride_t >= t.shape[2]
+          and t.data_ptr() % 16 == 0)
+    if written and t.shape[0] > 1:
+        # a batch behind the other, or batches interleaved within the token stride
+        ok = ok and (stride_b >= (t.shape[1] - 1) * stride_t + t.shape[2]
+                     or (stride_b >= t.shape[2] and stride_t >= (t.shape[0] - 1) * stride_b + t.shape[2]))
+    return ok
+
+
+def _masked_attention_reason(q, k, v, heads, kv_heads, causal_block, q_lengths, kv_lengths) -> str | None:
+    for t in (q, k, v):
+        if not t.is_cuda or t.device != q.device or t.dtype != torch.bfloat16:
+            return "qkv_device_or_dtype"
+    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0]:
+        return "qkv_shape"
+    if min(q.shape) < 1 or min(k.shape) < 1:
+        return "qkv_shape"
+    if heads < 1 or q.shape[2] != heads * 128:
+        return "head_dim"
+    if kv_heads < 1 or heads % kv_heads or k.shape[2] != kv_heads * 128:
+        return "kv_heads"
+    if not (_rows_ok(q) and _rows_ok(k) and _rows_ok(v)) or _row_strides(k) != _row_strides(v):
+        return "qkv_stride"
+    if causal_block < 0:
+        return "causal_block"
+    for lengths in (q_lengths, kv_lengths):
+        if lengths is not None and (lengths.shape != (q.shape[0],) or lengths.dtype != torch.int32
+                                    or lengths.device != q.device or not lengths.is_contiguous()):
+            return "lengths: int32 [B] on the device of q"
+    return None
+
+
+def _workspace(name: str, device: torch.device, *sizes: int) -> torch.Tensor:
+    n = ctypes.c_int64(0)
+    _lib.call(name, *sizes, ctypes.addressof(n))
+    return torch.empty((n.value,), device=device, dtype=torch.uint8)
+
+
+def attention_with_lse(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    heads: int,
+    *,
+    kv_heads: int | None = None,
+    softmax_scale: float | None = None,
+    causal_block: int = 0,
+    q_lengths: torch.Tensor | None = None,
+    kv_lengths: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``attention`` with masks and shared key/value heads, and the softmax statistics that
+    ``attention_backward`` needs: returns (out [B, L, heads*128] bf16, lse [B, heads, L] fp32).
+
+    q is [B, L, heads*128], k and v [B, L_kv, kv_heads*128] bf16 (token rows may be strided; k and v share
+    their strides); query head h reads key/value head ``h // (heads // kv_heads)``.  Query i sees key j if
+    ``i < q_lengths[b]``, ``j < kv_lengths[b]`` (int32 [B] on the GPU; default: all) and, with ``causal_block``
+    n > 0, ``j // n <= (i + L_kv - L) // n``: n = 1 is the token-causal mask with both sequences ending
+    together, the tokens of a latent frame make it frame-causal (a token sees its own and all earlier frames).
+    ``lse`` is the natural log of a row's sum of exponentials.  A row that sees no key gets out 0 and lse
+    -inf; keys and values past ``kv_lengths`` may hold anything.
+
+    No reference counterpart: the reference infers with dense bidirectional attention only.
+    """
+    kv_heads = heads if kv_heads is None else kv_heads
+    reason = _masked_attention_reason(q, k, v, heads, kv_heads, causal_block, q_lengths, kv_lengths)
+    if reason is not None:
+        raise ValueError(reason)
+    B, L, _ = q.shape
+    scale = float(softmax_scale) if softmax_scale is not None else 128 ** -0.5
+    if out is None:
+        out = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device or not _rows_ok(out, written=True):
+        raise ValueError("out_shape: out must be bf16 [B, L, heads*128] with unit column stride")
+    lse = torch.empty((B, heads, L), device=q.device, dtype=torch.float32)
+    with torch.cuda.device(q.device):
+        _lib.call(
+            "ogx_attention_fwd_lse",
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), B, L, k.shape[1], heads, kv_heads, 128,
+            *_row_strides(q), *_row_strides(k), scale, int(causal_block), _ptr(q_lengths), _ptr(kv_lengths),
+            out.data_ptr(), *_row_strides(out), lse.data_ptr(), _stream(q),
+        )
+    return out, lse
+
+
+def attention_backward(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    heads: int,
+    *,
+    kv_heads: int | None = None,
+    softmax_scale: float | None = None,
+    causal_block: int = 0,
+    q_lengths: torch.Tensor | None = None,
+    kv_lengths: torch.Tensor | None = None,
+    grads: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients (dq, dk, dv) of ``attention_with_lse``, bf16, from ``dout`` = the gradient of ``out`` and the
+    forward call's arguments and results (same scale, masks and heads).
+
+    The probabilities are recomputed from ``lse``.  Every gradient is summed in one order (dk and dv over the
+    query heads that share a key head), so equal inputs give equal bits.  Rows past ``q_lengths`` and rows that
+    see no key get dq 0 and give nothing to dk and dv; keys past ``kv_lengths`` get 0.  ``grads`` takes (dq, dk,
+    dv) to write into, for example the slices of one packed [B, L, (heads + 2*kv_heads)*128] buffer; dk and dv
+    share their strides.  No reference counterpart (the reference only infers).
+    """
+    kv_heads = heads if kv_heads is None else kv_heads
+    reason = _masked_attention_reason(q, k, v, heads, kv_heads, causal_block, q_lengths, kv_lengths)
+    if reason is not None:
+        raise ValueError(reason)
+    B, L, _ = q.shape
+    for t in (dout, out):
+        if t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != q.device or not _rows_ok(t):
+            raise ValueError("dout_or_out: bf16 of q's shape with unit column stride")
+    if lse.shape != (B, heads, L) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        raise ValueError("lse: fp32 [B, heads, L] as attention_with_lse returns it")
+    scale = float(softmax_scale) if softmax_scale is not None else 128 ** -0.5
+    if grads is None:
+        dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=torch.bfloat16) for t in (q, k, v))
+    else:
+        dq, dk, dv = grads
+        for t, like in ((dq, q), (dk, k), (dv, v)):
+            if (t.shape != like.shape or t.dtype != torch.bfloat16 or t.device != q.device
+                    or not _rows_ok(t, written=True)):
+                raise ValueError("grads: bf16 tensors of the shapes of q, k and v with unit column stride")
+        if _row_strides(dk) != _row_strides(dv):
+            raise ValueError("grads: dk and dv share their strides")
+    with torch.cuda.device(q.device):
+        workspace = _workspace("ogx_attention_bwd_workspace", q.device, B, L, k.shape[1], heads, kv_heads)
+        _lib.call(
+            "ogx_attention_bwd",
+            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            B, L, k.shape[1], heads, kv_heads, 128, *_row_strides(dout), *_row_strides(q), *_row_strides(k),
+            *_row_strides(out), scale, int(causal_block), _ptr(q_lengths), _ptr(kv_lengths),
+            workspace.data_ptr(), workspace.numel(), dq.data_ptr(), *_row_strides(dq), dk.data_ptr(), dv.data_ptr(),
+            *_row_strides(dk), _stream(q),
+        )
+    return dq, dk, dv
+
+
+# ---------------------------------------------------------------- training pass: Q/K norm + rotation
+_NORMS = {"none": NORM_NONE, "head": NORM_HEAD, "row": NORM_ROW}
+
+
+def _qk_norm_rope_args(q, k, q_weight, k_weight, cos, sin, heads, kv_heads, norm):
+    """Checks of ``fused_qk_norm_rope`` and the rotation's (rotary, batch, head, token strides)."""
+    if norm not in _NORMS:
+        raise ValueError("norm: 'head', 'row' or 'none'")
+    for t in (q, k):
+        if not t.is_cuda or t.device != q.device or t.dtype != torch.bfloat16:
+            raise ValueError("qk_device_or_dtype")
+    if q.ndim != 3 or k.ndim != 3 or q.shape[:2] != k.shape[:2]:
+        raise ValueError("qk_shape")
+    B, L, _ = q.shape
+    if L < 1 or B < 1:
+        raise ValueError("empty_tokens")
+    if heads < 1 or kv_heads < 1 or q.shape[2] % heads or q.shape[2] // heads not in (64, 128):
+        raise ValueError("head_dim")
+    hd = q.shape[2] // heads
+    if k.shape[2] != kv_heads * hd or heads + kv_heads > 128:
+        raise ValueError("qk_shape")
+    if not (_rows_ok(q) and _rows_ok(k)):
+        raise ValueError("qk_noncontiguous")
+    if norm == "none":
+        if q_weight is not None or k_weight is not None:
+            raise ValueError("qk_weight_shape")
+    else:
+        want = (hd, hd) if norm == "head" else (heads * hd, kv_heads * hd)
+        if q_weight is None or k_weight is None or q_weight.shape != want[:1] or k_weight.shape != want[1:]:
+            raise ValueError("qk_weight_shape")
+        for w in (q_weight, k_weight):
+            if w.device != q.device or w.dtype not in (torch.bfloat16, torch.float32) or w.dtype != q_weight.dtype:
+                raise ValueError("qk_weight_shape")
+    if cos.ndim not in (3, 4) or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.stride() != sin.stride():
+        raise ValueError("rope_shape")
+    if cos.dtype not in (torch.bfloat16, torch.float32) or cos.device != q.device or sin.device != q.device:
+        raise ValueError("rope_shape")
+    half = cos.shape[-1]
+    if cos.shape[0] not in (1, B) or cos.shape[-2] != L or half % 8 or not 8 <= half <= hd // 2:
+        raise ValueError("rope_shape")
+    if cos.ndim == 4 and (cos.shape[1] != heads or heads != kv_heads):
+        raise ValueError("rope_shape")
+    stride_b = cos.stride(0) if cos.shape[0] > 1 else 0
+    stride_h = cos.stride(1) if cos.ndim == 4 and heads > 1 else 0
+    stride_t = cos.stride(-2) if L > 1 else half
+    if (cos.stride(-1) != 1 or stride_b % 8 or stride_h % 8 or stride_t % 8 or cos.data_ptr() % 16
+            or sin.data_ptr() % 16):
+        raise ValueError("rope_shape")
+    return hd, 2 * half, stride_b, stride_h, stride_t
+
+
+def _contiguous16(w: torch.Tensor | None) -> torch.Tensor | None:
+    """The weight, copied only where its layout or alignment needs it."""
+    if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0):
+        return w
+    return w.clone(memory_format=torch.contiguous_format)
+
+
+def fused_qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    q_weight: torch.Tensor | None,
+    k_weight: torch.Tensor | None,
+    eps: float,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    heads: int,
+    *,
+    kv_heads: int | None = None,
+    norm: str = "head",
+    interleaved: bool = False,
+    out: tuple[torch.Tensor, torch.Tensor] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Q/K RMSNorm and rotation in one pass for any head counts and batch: q [B, L, heads*d] and k [B, L,
+    kv_heads*d] bf16, d 64 or 128; fp32 math, one bf16 rounding.
+
+    ``norm``: "head" normalises each head by itself (weights [d]), "row" all heads of a row together (weights
+    [heads*d] and [kv_heads*d], the video block's norm), "none" only rotates (weights None).  The first
+    R = 2 * cos.shape[-1] columns of each head turn by the token's angles: columns (j, j + R/2), or (2j, 2j + 1)
+    with ``interleaved``.  cos/sin (bf16 or fp32): [1|B, L, R/2] shared by the heads or [1|B, heads, L, R/2]
+    (then kv_heads == heads).  ``out`` may be (q, k) for an in-place update.
+
+    ``fused_video_qk_rmsnorm_rope`` (ltx_serve/triton_ltx_ops.py:320-378) is the case norm="row", 32 heads of
+    128, B = 1; ``fused_qk_norm_rope_backward`` gives the gradients of all of them.
+    """
+    kv_heads = heads if kv_heads is None else kv_heads
+    hd, rotary, cs_b, cs_h, cs_t = _qk_norm_rope_args(q, k, q_weight, k_weight, cos, sin, heads, kv_heads, norm)
+    if out is None:
+        q_out, k_out = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+    else:
+        q_out, k_out = out
+        for t, like in ((q_out, q), (k_out, k)):
+            if (t.shape != like.shape or t.dtype != torch.bfloat16 or t.device != q.device
+                    or not _rows_ok(t, written=True)):
+                raise ValueError("qk_out_shape")
+    q_weight, k_weight = _contiguous16(q_weight), _contiguous16(k_weight)
+    with torch.cuda.device(q.device):
+        _lib.call(
+            "ogx_qk_norm_rope",
+            q.data_ptr(), k.data_ptr(), q.shape[0], q.shape[1], heads, kv_heads, hd, *_row_strides(q),
+            *_row_strides(k), _ptr(q_weight), _ptr(k_weight), DTYPE_F32 if q_weight is None else _code(q_weight),
+            _NORMS[norm], float(eps), cos.data_ptr(), sin.data_ptr(), _code(cos), rotary, int(interleaved),
+            cs_b, cs_h, cs_t, q_out.data_ptr(), *_row_strides(q_out), k_out.data_ptr(), *_row_strides(k_out),
+            _stream(q),
+        )
+    return q_out, k_out
+
+
+def fused_qk_norm_rope_backward(
+    dq_out: torch.Tensor,
+    dk_out: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    q_weight: torch.Tensor | None,
+    k_weight: torch.Tensor | None,
+    eps: float,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    heads: int,
+    *,
+    kv_heads: int | None = None,
+    norm: str = "head",
+    interleaved: bool = False,
+    out: tuple[torch.Tensor, torch.Tensor] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of ``fused_qk_norm_rope`` (and of ``fused_video_qk_rmsnorm_rope``: norm="row"): from the
+    gradients of its outputs and its inputs, (dq, dk, dq_weight, dk_weight).
+
+    dq and dk are bf16 (``out`` may be (dq_out, dk_out) for an in-place update); the weights' gradients are fp32
+    sums over all rows (and, for norm="head", heads), whatever the weights' type, and None for norm="none".  The
+    sums run in a fixed order.  No reference counterpart (the reference only infers).
+    """
+    kv_heads = heads if kv_heads is None else kv_heads
+    hd, rotary, cs_b, cs_h, cs_t = _qk_norm_rope_args(q, k, q_weight, k_weight, cos, sin, heads, kv_heads, norm)
+    for t, like in ((dq_out, q), (dk_out, k)):
+        if t.shape != like.shape or t.dtype != torch.bfloat16 or t.device != q.device or not _rows_ok(t):
+            raise ValueError("output_gradients: bf16 of the shapes of q and k with unit column stride")
+    if out is None:
+        dq, dk = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+    else:
+        dq, dk = out
+        for t, like in ((dq, q), (dk, k)):
+            if (t.shape != like.shape or t.dtype != torch.bfloat16 or t.device != q.device
+                    or not _rows_ok(t, written=True)):
+                raise ValueError("qk_out_shape")
+    q_weight, k_weight = _contiguous16(q_weight), _contiguous16(k_weight)
+    dqw = dkw = workspace = None
+    with torch.cuda.device(q.device):
+        if norm != "none":
+            dqw, dkw = (torch.empty(w.shape, device=q.device, dtype=torch.float32) for w in (q_weight, k_weight))
+            workspace = _workspace("ogx_qk_norm_rope_bwd_workspace", q.device, q.shape[0], q.shape[1], heads, kv_heads,
+                                   hd, _NORMS[norm])
+        _lib.call(
+            "ogx_qk_norm_rope_bwd",
+            dq_out.data_ptr(), *_row_strides(dq_out), dk_out.data_ptr(), *_row_strides(dk_out), q.data_ptr(),
+            k.data_ptr(), q.shape[0], q.shape[1], heads, kv_heads, hd, *_row_strides(q), *_row_strides(k),
+            _ptr(q_weight), _ptr(k_weight), DTYPE_F32 if q_weight is None else _code(q_weight), _NORMS[norm],
+            float(eps), cos.data_ptr(), sin.data_ptr(), _code(cos), rotary, int(interleaved), cs_b, cs_h, cs_t,
+            dq.data_ptr(), *_row_strides(dq), dk.data_ptr(), *_row_strides(dk), _ptr(dqw), _ptr(dkw), _ptr(workspace),
+            0 if workspace is None else workspace.numel(), _stream(q),
+        )
+    return dq, dk, dqw, dkw
+
+
 def collect_video_ada_values_calls() -> int:
     return _VIDEO_ADA_VALUES_CALLS
 
@@ -1056,6 +1378,8 @@ __all__ = [
     "RopePositions",
     "ada_from_table_guard_reason",
     "attention",
+    "attention_backward",
+    "attention_with_lse",
     "collect_video_ada_values_calls",
     "fp8_linear_forward",
     "fp8_linear_from_quantized_e4m3",
@@ -1075,6 +1399,8 @@ __all__ = [
     "fused_gelu_tanh_fp8_quantize_e4m3",
     "fused_head_gate_mul_bf16",
     "fused_mul_from_ada",
+    "fused_qk_norm_rope",
+    "fused_qk_norm_rope_backward",
     "fused_qk_rmsnorm",
     "fused_residual_gate_bf16",
     "fused_residual_gate_bias_from_ada",
