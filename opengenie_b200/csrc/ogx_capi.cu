@@ -1615,63 +1615,65 @@ using ogx::qkn::kHead;
 using ogx::qkn::kNone;
 using ogx::qkn::kRow;
 
-constexpr int kQkMaxHeads = 128;  // q's and k's together: 8 head slots of 16 groups
-
-int pow2_at_least(int64_t n) {
-  int p = 1;
-  while (p < n) p *= 2;
-  return p;
-}
+constexpr int kQkMaxHeads = 128;  // q's and k's together
 
 struct QkShape {
-  int groups, team, teams, steps;
+  int team, teams, steps;
+  int64_t grid;
 };
 
-// A token's team has as many groups as heads, up to the CTA's; the groups' head slots are a compile-time number.
-QkShape qk_shape(int64_t all_heads, int64_t head_dim) {
+// Groups per token and CTAs.  A row norm's team has a group for every head of the wider tensor, up to the CTA's
+// groups, which then take `steps` heads of each tensor.  Heads by themselves take the team that leaves the fewest
+// of its head slots idle (32 + 8 heads: a team of 8 takes 4 + 1 steps, one of 16 would idle half of its third) if
+// the tokens fill the GPU's CTAs with it, else the widest useful one.
+QkShape qk_shape(int64_t heads, int64_t kv_heads, int64_t head_dim, int norm, int64_t rows) {
+  const int lanes = static_cast<int>(head_dim / 8);
+  const int groups = (norm == kRow ? ogx::qkn::kRowThreads : ogx::qkn::kThreads) / lanes;
+  const int64_t widest = heads > kv_heads ? heads : kv_heads;
   QkShape r{};
-  r.groups = ogx::qkn::kThreads / static_cast<int>(head_dim / 8);
-  r.team = pow2_at_least(all_heads);
-  if (r.team > r.groups) r.team = r.groups;
-  r.teams = r.groups / r.team;
-  r.steps = pow2_at_least((all_heads + r.team - 1) / r.team);
+  r.team = 1;
+  while (r.team < widest && r.team < groups) r.team *= 2;
+  const int64_t sms = sm_count();
+  if (norm == kRow) {
+    r.steps = static_cast<int>((widest + r.team - 1) / r.team);
+    r.steps = r.steps > 2 ? 4 : r.steps;
+  } else {
+    const auto slots = [&](int64_t team) { return team * ((heads + team - 1) / team + (kv_heads + team - 1) / team); };
+    for (int team = r.team / 2; team >= 1; team /= 2)
+      if (slots(team) < slots(r.team) && rows * team >= sms * 4 * groups) r.team = team;
+  }
+  r.teams = groups / r.team;
+  const int64_t want = (rows + r.teams - 1) / r.teams;
+  const int64_t cap = sms * (norm == kRow ? (r.steps == 1 ? 2 : 1) : 4);
+  r.grid = want < cap ? want : cap;
   return r;
-}
-
-int64_t qk_grid(const QkShape& sh, int64_t rows) {
-  const int64_t want = (rows + sh.teams - 1) / sh.teams;
-  const int64_t cap = static_cast<int64_t>(sm_count()) * 4;
-  return want < cap ? want : cap;
 }
 
 int64_t qk_weight_columns(int norm, int64_t all_heads, int64_t head_dim) {
   return norm == kNone ? 0 : (norm == kHead ? 2 * head_dim : all_heads * head_dim);
 }
 
-int64_t qk_partial_rows(const QkShape& sh, int norm, int64_t grid) { return norm == kRow ? grid * sh.teams : grid; }
+int64_t qk_partial_rows(const QkShape& sh, int norm) { return norm == kRow ? sh.grid * sh.teams : sh.grid; }
 
-template <int HD, int STEPS, bool BACKWARD>
-void qk_dispatch_norm(const ogx::qkn::Params& p, int norm, int64_t grid, cudaStream_t s) {
-  const dim3 g(static_cast<unsigned>(grid)), b(ogx::qkn::kThreads);
-  if (norm == kNone) return launch(ogx::qkn::qk_norm_rope_kernel<HD, STEPS, kNone, BACKWARD>, g, b, 0, s, p);
-  if (norm == kHead) return launch(ogx::qkn::qk_norm_rope_kernel<HD, STEPS, kHead, BACKWARD>, g, b, 0, s, p);
-  return launch(ogx::qkn::qk_norm_rope_kernel<HD, STEPS, kRow, BACKWARD>, g, b, 0, s, p);
-}
-
-template <int HD, bool BACKWARD>
-void qk_dispatch_steps(const ogx::qkn::Params& p, int steps, int norm, int64_t grid, cudaStream_t s) {
-  switch (steps) {
-    case 1: return qk_dispatch_norm<HD, 1, BACKWARD>(p, norm, grid, s);
-    case 2: return qk_dispatch_norm<HD, 2, BACKWARD>(p, norm, grid, s);
-    case 4: return qk_dispatch_norm<HD, 4, BACKWARD>(p, norm, grid, s);
-    default: return qk_dispatch_norm<HD, 8, BACKWARD>(p, norm, grid, s);
+template <int HD, bool INTER, bool BACKWARD>
+void qk_launch(const ogx::qkn::Params& p, const QkShape& sh, int norm, cudaStream_t s) {
+  const dim3 g(static_cast<unsigned>(sh.grid));
+  if (norm == kNone) return launch(ogx::qkn::qk_head_kernel<HD, kNone, INTER, BACKWARD>, g, ogx::qkn::kThreads, 0, s, p);
+  if (norm == kHead) return launch(ogx::qkn::qk_head_kernel<HD, kHead, INTER, BACKWARD>, g, ogx::qkn::kThreads, 0, s, p);
+  const dim3 b(ogx::qkn::kRowThreads);
+  if (sh.steps == 1) return launch(ogx::qkn::qk_row_kernel<HD, 1, INTER, BACKWARD>, g, b, 0, s, p);
+  if constexpr (HD == 128) {  // 64 groups of 64 columns take every head in two steps
+    if (sh.steps == 4) return launch(ogx::qkn::qk_row_kernel<HD, 4, INTER, BACKWARD>, g, b, 0, s, p);
   }
+  return launch(ogx::qkn::qk_row_kernel<HD, 2, INTER, BACKWARD>, g, b, 0, s, p);
 }
 
 template <bool BACKWARD>
-void qk_dispatch(const ogx::qkn::Params& p, int64_t head_dim, int steps, int norm, int64_t grid, cudaStream_t s) {
-  if (head_dim == 128) return qk_dispatch_steps<128, BACKWARD>(p, steps, norm, grid, s);
-  return qk_dispatch_steps<64, BACKWARD>(p, steps, norm, grid, s);
+void qk_dispatch(const ogx::qkn::Params& p, int64_t head_dim, int interleaved, const QkShape& sh, int norm,
+                 cudaStream_t s) {
+  if (head_dim == 128)
+    return interleaved ? qk_launch<128, true, BACKWARD>(p, sh, norm, s) : qk_launch<128, false, BACKWARD>(p, sh, norm, s);
+  return interleaved ? qk_launch<64, true, BACKWARD>(p, sh, norm, s) : qk_launch<64, false, BACKWARD>(p, sh, norm, s);
 }
 
 int qk_norm_guard(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
@@ -1704,7 +1706,7 @@ int qk_norm_guard(const void* q, const void* k, int64_t batch, int64_t tokens, i
 ogx::qkn::Params qk_params(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                            int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
                            const void* q_weight, const void* k_weight, int weight_dtype, float eps, const void* cos,
-                           const void* sin, int cs_dtype, int64_t rotary, int interleaved, int64_t cs_stride_b, int64_t cs_stride_h,
+                           const void* sin, int cs_dtype, int64_t rotary, int64_t cs_stride_b, int64_t cs_stride_h,
                            int64_t cs_stride_t, const QkShape& sh) {
   ogx::qkn::Params p{};
   p.x[0] = static_cast<const __nv_bfloat16*>(q);
@@ -1723,7 +1725,6 @@ ogx::qkn::Params qk_params(const void* q, const void* k, int64_t batch, int64_t 
   p.heads[0] = static_cast<int>(heads);
   p.heads[1] = static_cast<int>(kv_heads);
   p.rotary = static_cast<int>(rotary);
-  p.interleaved = interleaved != 0;
   p.w_fp32 = weight_dtype == OGX_DTYPE_F32;
   p.cs_fp32 = cs_dtype == OGX_DTYPE_F32;
   p.team = sh.team;
@@ -1762,12 +1763,12 @@ int ogx_qk_norm_rope(const void* q, const void* k, int64_t batch, int64_t tokens
                          q_weight, k_weight, weight_dtype, norm, eps, cos, sin, cs_dtype, rotary, cs_stride_b,
                          cs_stride_h, cs_stride_t);
   if (rc) return rc;
-  const QkShape sh = qk_shape(heads + kv_heads, head_dim);
+  const QkShape sh = qk_shape(heads, kv_heads, head_dim, norm, batch * tokens);
   ogx::qkn::Params p = qk_params(q, k, batch, tokens, heads, kv_heads, q_stride_b, q_stride_t, k_stride_b, k_stride_t,
-                                 q_weight, k_weight, weight_dtype, eps, cos, sin, cs_dtype, rotary, interleaved,
-                                 cs_stride_b, cs_stride_h, cs_stride_t, sh);
+                                 q_weight, k_weight, weight_dtype, eps, cos, sin, cs_dtype, rotary, cs_stride_b,
+                                 cs_stride_h, cs_stride_t, sh);
   if ((rc = qk_outputs(p, q_out, q_out_stride_b, q_out_stride_t, k_out, k_out_stride_b, k_out_stride_t))) return rc;
-  qk_dispatch<false>(p, head_dim, sh.steps, norm, qk_grid(sh, p.rows), static_cast<cudaStream_t>(stream));
+  qk_dispatch<false>(p, head_dim, interleaved, sh, norm, static_cast<cudaStream_t>(stream));
   return check_launch("qk_norm_rope_kernel");
 }
 
@@ -1777,9 +1778,9 @@ int ogx_qk_norm_rope_bwd_workspace(int64_t batch, int64_t tokens, int64_t heads,
   if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || heads > kQkMaxHeads || kv_heads > kQkMaxHeads ||
       heads + kv_heads > kQkMaxHeads || (head_dim != 64 && head_dim != 128))
     return fail(OGX_EINVAL, "qk_shape");
-  const QkShape sh = qk_shape(heads + kv_heads, head_dim);
-  *bytes = 4 * qk_partial_rows(sh, norm, qk_grid(sh, batch * tokens)) *
-           qk_weight_columns(norm, heads + kv_heads, head_dim);
+  if (norm != kNone && norm != kHead && norm != kRow) return fail(OGX_EINVAL, "norm");
+  const QkShape sh = qk_shape(heads, kv_heads, head_dim, norm, batch * tokens);
+  *bytes = 4 * qk_partial_rows(sh, norm) * qk_weight_columns(norm, heads + kv_heads, head_dim);
   return OGX_OK;
 }
 
@@ -1799,10 +1800,10 @@ int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq
   if (dq_out == nullptr || dk_out == nullptr || !aligned16(dq_out) || !aligned16(dk_out) || dq_out_stride_b % 8 ||
       dq_out_stride_t % 8 || dk_out_stride_b % 8 || dk_out_stride_t % 8)
     return fail(OGX_EINVAL, "output_gradients");
-  const QkShape sh = qk_shape(heads + kv_heads, head_dim);
+  const QkShape sh = qk_shape(heads, kv_heads, head_dim, norm, batch * tokens);
   ogx::qkn::Params p = qk_params(q, k, batch, tokens, heads, kv_heads, q_stride_b, q_stride_t, k_stride_b, k_stride_t,
-                                 q_weight, k_weight, weight_dtype, eps, cos, sin, cs_dtype, rotary, interleaved,
-                                 cs_stride_b, cs_stride_h, cs_stride_t, sh);
+                                 q_weight, k_weight, weight_dtype, eps, cos, sin, cs_dtype, rotary, cs_stride_b,
+                                 cs_stride_h, cs_stride_t, sh);
   p.dy[0] = static_cast<const __nv_bfloat16*>(dq_out);
   p.dy[1] = static_cast<const __nv_bfloat16*>(dk_out);
   p.dy_stride_b[0] = dq_out_stride_b;
@@ -1810,9 +1811,8 @@ int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq
   p.dy_stride_b[1] = dk_out_stride_b;
   p.dy_stride_t[1] = dk_out_stride_t;
   if ((rc = qk_outputs(p, dq, dq_stride_b, dq_stride_t, dk, dk_stride_b, dk_stride_t))) return rc;
-  const int64_t grid = qk_grid(sh, p.rows);
   const int64_t columns = qk_weight_columns(norm, heads + kv_heads, head_dim);
-  const int64_t partial_rows = qk_partial_rows(sh, norm, grid);
+  const int64_t partial_rows = qk_partial_rows(sh, norm);
   if (norm != kNone) {
     if (dq_weight == nullptr || dk_weight == nullptr || !aligned4(dq_weight) || !aligned4(dk_weight))
       return fail(OGX_EINVAL, "weight_gradients");
@@ -1821,7 +1821,7 @@ int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq
   }
   p.partials = static_cast<float*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  qk_dispatch<true>(p, head_dim, sh.steps, norm, grid, s);
+  qk_dispatch<true>(p, head_dim, interleaved, sh, norm, s);
   if ((rc = check_launch("qk_norm_rope_kernel"))) return rc;
   if (norm == kNone) return OGX_OK;
   launch(ogx::qkn::qk_norm_weight_sum_kernel, dim3(static_cast<unsigned>((columns + 31) / 32)), dim3(1024), 0, s,
