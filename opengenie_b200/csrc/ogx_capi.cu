@@ -1617,63 +1617,93 @@ using ogx::qkn::kRow;
 
 constexpr int kQkMaxHeads = 128;  // q's and k's together
 
+// A row norm's CTA: 256 threads where two heads per group are enough for the wider of q and k, else 512.
+int qk_threads(int64_t heads, int64_t kv_heads, int64_t head_dim, int norm) {
+  const int64_t groups = ogx::qkn::kThreads / (head_dim / 8);
+  return norm == kRow && (heads > kv_heads ? heads : kv_heads) > 2 * groups ? 2 * ogx::qkn::kThreads : ogx::qkn::kThreads;
+}
+
+// How one of q and k is shared out: groups per token, heads per group (row norm) and CTAs.
 struct QkShape {
   int team, teams, steps;
-  int64_t grid;
+  int64_t ctas;
 };
 
-// Groups per token and CTAs.  A row norm's team has a group for every head of the wider tensor, up to the CTA's
-// groups, which then take `steps` heads of each tensor.  Heads by themselves take the team that leaves the fewest
-// of its head slots idle (32 + 8 heads: a team of 8 takes 4 + 1 steps, one of 16 would idle half of its third) if
-// the tokens fill the GPU's CTAs with it, else the widest useful one.
-QkShape qk_shape(int64_t heads, int64_t kv_heads, int64_t head_dim, int norm, int64_t rows) {
-  const int lanes = static_cast<int>(head_dim / 8);
-  const int groups = (norm == kRow ? ogx::qkn::kRowThreads : ogx::qkn::kThreads) / lanes;
-  const int64_t widest = heads > kv_heads ? heads : kv_heads;
+// A row norm's team has a group for every head, up to the CTA's groups, which then take `steps` heads each.  Heads
+// by themselves go four to a group, so that a token's addresses and angles serve four heads, unless the tokens are
+// so few that CTAs would be idle.
+QkShape qk_shape(int64_t heads, int64_t other_heads, int64_t head_dim, int norm, bool backward, int64_t rows) {
+  const int threads = qk_threads(heads, other_heads, head_dim, norm);
+  const int groups = threads / static_cast<int>(head_dim / 8);
   QkShape r{};
-  r.team = 1;
-  while (r.team < widest && r.team < groups) r.team *= 2;
-  const int64_t sms = sm_count();
-  if (norm == kRow) {
-    r.steps = static_cast<int>((widest + r.team - 1) / r.team);
-    r.steps = r.steps > 2 ? 4 : r.steps;
-  } else {
-    const auto slots = [&](int64_t team) { return team * ((heads + team - 1) / team + (kv_heads + team - 1) / team); };
-    for (int team = r.team / 2; team >= 1; team /= 2)
-      if (slots(team) < slots(r.team) && rows * team >= sms * 4 * groups) r.team = team;
+  const auto team_for = [&](int64_t width) {
+    int team = 1;
+    while (team < width && team < groups) team *= 2;
+    return team;
+  };
+  r.team = team_for(heads);
+  if (norm != kRow) {
+    const int four = team_for((heads + 3) / 4);
+    if (rows * four >= static_cast<int64_t>(sm_count()) * groups) r.team = four;
   }
   r.teams = groups / r.team;
+  r.steps = static_cast<int>((heads + r.team - 1) / r.team);
+  r.steps = r.steps > 2 ? 4 : r.steps;
+  const int64_t widest = heads > other_heads ? heads : other_heads;
+  const int row_steps = widest > 2 * groups ? 4 : (widest > groups ? 2 : 1);
+  // one wave of resident CTAs, shared out between q and k by their heads
+  const int64_t wave = static_cast<int64_t>(sm_count()) *
+                       (norm == kRow ? ogx::qkn::row_ctas(threads, row_steps) : ogx::qkn::head_ctas(backward));
+  int64_t cap = wave * heads / (heads + other_heads);
+  cap = cap < 1 ? 1 : cap;
   const int64_t want = (rows + r.teams - 1) / r.teams;
-  const int64_t cap = sms * (norm == kRow ? (r.steps == 1 ? 2 : 1) : 4);
-  r.grid = want < cap ? want : cap;
+  r.ctas = want < cap ? want : cap;
   return r;
 }
 
-int64_t qk_weight_columns(int norm, int64_t all_heads, int64_t head_dim) {
-  return norm == kNone ? 0 : (norm == kHead ? 2 * head_dim : all_heads * head_dim);
+ogx::qkn::Stream qk_stream(const void* base, int64_t stride_b, int64_t stride_t, int64_t size, int64_t tokens,
+                           int64_t step) {
+  ogx::qkn::Stream r{};
+  r.base = const_cast<char*>(static_cast<const char*>(base));
+  r.stride_b = stride_b * size;
+  r.stride_t = stride_t * size;
+  r.step = step / tokens * r.stride_b + step % tokens * r.stride_t;
+  r.wrap = r.stride_b - tokens * r.stride_t;
+  return r;
 }
 
-int64_t qk_partial_rows(const QkShape& sh, int norm) { return norm == kRow ? sh.grid * sh.teams : sh.grid; }
+int64_t qk_partial_rows(const QkShape& sh, int norm) { return norm == kRow ? sh.ctas * sh.teams : sh.ctas; }
+int64_t qk_weight_columns(int norm, int64_t heads, int64_t head_dim) { return norm == kHead ? head_dim : heads * head_dim; }
+int64_t qk_partial_bytes(const QkShape& sh, int norm, int64_t heads, int64_t head_dim) {
+  return norm == kNone ? 0 : 4 * qk_partial_rows(sh, norm) * qk_weight_columns(norm, heads, head_dim);
+}
 
 template <int HD, bool INTER, bool BACKWARD>
-void qk_launch(const ogx::qkn::Params& p, const QkShape& sh, int norm, cudaStream_t s) {
-  const dim3 g(static_cast<unsigned>(sh.grid));
-  if (norm == kNone) return launch(ogx::qkn::qk_head_kernel<HD, kNone, INTER, BACKWARD>, g, ogx::qkn::kThreads, 0, s, p);
-  if (norm == kHead) return launch(ogx::qkn::qk_head_kernel<HD, kHead, INTER, BACKWARD>, g, ogx::qkn::kThreads, 0, s, p);
-  const dim3 b(ogx::qkn::kRowThreads);
-  if (sh.steps == 1) return launch(ogx::qkn::qk_row_kernel<HD, 1, INTER, BACKWARD>, g, b, 0, s, p);
+void qk_launch(const ogx::qkn::Params& p, int steps, int norm, cudaStream_t s) {
+  using namespace ogx::qkn;
+  const dim3 g(static_cast<unsigned>(p.t[0].ctas + p.t[1].ctas));
+  if (norm == kNone)
+    return p.cs_stride_h ? launch(qk_head_kernel<HD, kNone, INTER, true, BACKWARD>, g, kThreads, 0, s, p)
+                         : launch(qk_head_kernel<HD, kNone, INTER, false, BACKWARD>, g, kThreads, 0, s, p);
+  if (norm == kHead)
+    return p.cs_stride_h ? launch(qk_head_kernel<HD, kHead, INTER, true, BACKWARD>, g, kThreads, 0, s, p)
+                         : launch(qk_head_kernel<HD, kHead, INTER, false, BACKWARD>, g, kThreads, 0, s, p);
+  if (qk_threads(p.t[0].heads, p.t[1].heads, HD, norm) == 256)
+    return steps == 1 ? launch(qk_row_kernel<HD, 256, 1, INTER, BACKWARD>, g, 256, 0, s, p)
+                      : launch(qk_row_kernel<HD, 256, 2, INTER, BACKWARD>, g, 256, 0, s, p);
   if constexpr (HD == 128) {  // 64 groups of 64 columns take every head in two steps
-    if (sh.steps == 4) return launch(ogx::qkn::qk_row_kernel<HD, 4, INTER, BACKWARD>, g, b, 0, s, p);
+    if (steps == 4) return launch(qk_row_kernel<HD, 512, 4, INTER, BACKWARD>, g, 512, 0, s, p);
   }
-  return launch(ogx::qkn::qk_row_kernel<HD, 2, INTER, BACKWARD>, g, b, 0, s, p);
+  return launch(qk_row_kernel<HD, 512, 2, INTER, BACKWARD>, g, 512, 0, s, p);
 }
 
 template <bool BACKWARD>
-void qk_dispatch(const ogx::qkn::Params& p, int64_t head_dim, int interleaved, const QkShape& sh, int norm,
-                 cudaStream_t s) {
+void qk_dispatch(const ogx::qkn::Params& p, int64_t head_dim, int interleaved, int steps, int norm, cudaStream_t s) {
   if (head_dim == 128)
-    return interleaved ? qk_launch<128, true, BACKWARD>(p, sh, norm, s) : qk_launch<128, false, BACKWARD>(p, sh, norm, s);
-  return interleaved ? qk_launch<64, true, BACKWARD>(p, sh, norm, s) : qk_launch<64, false, BACKWARD>(p, sh, norm, s);
+    return interleaved ? qk_launch<128, true, BACKWARD>(p, steps, norm, s)
+                       : qk_launch<128, false, BACKWARD>(p, steps, norm, s);
+  return interleaved ? qk_launch<64, true, BACKWARD>(p, steps, norm, s)
+                     : qk_launch<64, false, BACKWARD>(p, steps, norm, s);
 }
 
 int qk_norm_guard(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
@@ -1686,7 +1716,8 @@ int qk_norm_guard(const void* q, const void* k, int64_t batch, int64_t tokens, i
   if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || heads > kQkMaxHeads || kv_heads > kQkMaxHeads ||
       heads + kv_heads > kQkMaxHeads)
     return fail(OGX_EINVAL, "qk_shape");
-  if (tokens > INT32_MAX || batch > INT32_MAX) return fail(OGX_EINVAL, "qk_shape");
+  // row numbers, and those a step past the last, stay below 2^31
+  if (tokens > (1 << 30) || batch > (1 << 30) || tokens * batch > (1 << 30)) return fail(OGX_EINVAL, "qk_shape");
   if (q_stride_b % 8 || q_stride_t % 8 || k_stride_b % 8 || k_stride_t % 8) return fail(OGX_EINVAL, "qk_noncontiguous");
   if (norm != kNone && norm != kHead && norm != kRow) return fail(OGX_EINVAL, "norm");
   if (norm != kNone && (q_weight == nullptr || k_weight == nullptr || !dtype_ok(weight_dtype)))
@@ -1702,49 +1733,47 @@ int qk_norm_guard(const void* q, const void* k, int64_t batch, int64_t tokens, i
   return OGX_OK;
 }
 
-// The part of the parameters both directions share.
+// The part of the parameters both directions share; *steps: heads per group of a row norm.
 ogx::qkn::Params qk_params(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
-                           int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
-                           const void* q_weight, const void* k_weight, int weight_dtype, float eps, const void* cos,
-                           const void* sin, int cs_dtype, int64_t rotary, int64_t cs_stride_b, int64_t cs_stride_h,
-                           int64_t cs_stride_t, const QkShape& sh) {
+                           int64_t head_dim, int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b,
+                           int64_t k_stride_t, const void* q_weight, const void* k_weight, int weight_dtype, int norm,
+                           float eps, const void* cos, const void* sin, int cs_dtype, int64_t rotary,
+                           int64_t cs_stride_b, int64_t cs_stride_h, int64_t cs_stride_t, bool backward,
+                           QkShape (&sh)[2], int* steps) {
   ogx::qkn::Params p{};
-  p.x[0] = static_cast<const __nv_bfloat16*>(q);
-  p.x[1] = static_cast<const __nv_bfloat16*>(k);
-  p.x_stride_b[0] = q_stride_b;
-  p.x_stride_t[0] = q_stride_t;
-  p.x_stride_b[1] = k_stride_b;
-  p.x_stride_t[1] = k_stride_t;
-  p.weight[0] = q_weight;
-  p.weight[1] = k_weight;
-  p.cos = cos;
-  p.sin = sin;
-  p.cs_stride_b = cs_stride_b;
-  p.cs_stride_h = cs_stride_h;
-  p.cs_stride_t = cs_stride_t;
-  p.heads[0] = static_cast<int>(heads);
-  p.heads[1] = static_cast<int>(kv_heads);
+  const int64_t n[2] = {heads, kv_heads};
+  for (int t = 0; t < 2; ++t) {
+    ogx::qkn::Tensor& a = p.t[t];
+    sh[t] = qk_shape(n[t], n[1 - t], head_dim, norm, backward, batch * tokens);
+    const int64_t step = sh[t].ctas * sh[t].teams;
+    a.x = qk_stream(t ? k : q, t ? k_stride_b : q_stride_b, t ? k_stride_t : q_stride_t, 2, tokens, step);
+    a.angles = qk_stream(nullptr, cs_stride_b, cs_stride_t, cs_dtype == OGX_DTYPE_F32 ? 4 : 2, tokens, step);
+    a.weight = t ? k_weight : q_weight;
+    a.heads = static_cast<int>(n[t]);
+    a.team = sh[t].team;
+    a.ctas = static_cast<int>(sh[t].ctas);
+    a.step_token = static_cast<int>(step % tokens);
+  }
+  *steps = sh[0].steps > sh[1].steps ? sh[0].steps : sh[1].steps;
+  p.cos = static_cast<const char*>(cos);
+  p.sin = static_cast<const char*>(sin);
+  p.cs_stride_h = cs_stride_h * (cs_dtype == OGX_DTYPE_F32 ? 4 : 2);
   p.rotary = static_cast<int>(rotary);
   p.w_fp32 = weight_dtype == OGX_DTYPE_F32;
   p.cs_fp32 = cs_dtype == OGX_DTYPE_F32;
-  p.team = sh.team;
-  p.tokens = tokens;
-  p.rows = batch * tokens;
+  p.tokens = static_cast<int>(tokens);
+  p.rows = static_cast<int>(batch * tokens);
   p.eps = eps;
   return p;
 }
 
-int qk_outputs(ogx::qkn::Params& p, void* y_q, int64_t q_stride_b, int64_t q_stride_t, void* y_k, int64_t k_stride_b,
-               int64_t k_stride_t) {
+int qk_outputs(ogx::qkn::Params& p, const QkShape (&sh)[2], void* y_q, int64_t q_stride_b, int64_t q_stride_t, void* y_k,
+               int64_t k_stride_b, int64_t k_stride_t) {
   if (y_q == nullptr || y_k == nullptr || !aligned16(y_q) || !aligned16(y_k) || q_stride_b % 8 || q_stride_t % 8 ||
       k_stride_b % 8 || k_stride_t % 8)
     return fail(OGX_EINVAL, "output");
-  p.y[0] = static_cast<__nv_bfloat16*>(y_q);
-  p.y[1] = static_cast<__nv_bfloat16*>(y_k);
-  p.y_stride_b[0] = q_stride_b;
-  p.y_stride_t[0] = q_stride_t;
-  p.y_stride_b[1] = k_stride_b;
-  p.y_stride_t[1] = k_stride_t;
+  p.t[0].y = qk_stream(y_q, q_stride_b, q_stride_t, 2, p.tokens, sh[0].ctas * sh[0].teams);
+  p.t[1].y = qk_stream(y_k, k_stride_b, k_stride_t, 2, p.tokens, sh[1].ctas * sh[1].teams);
   return OGX_OK;
 }
 
@@ -1763,12 +1792,13 @@ int ogx_qk_norm_rope(const void* q, const void* k, int64_t batch, int64_t tokens
                          q_weight, k_weight, weight_dtype, norm, eps, cos, sin, cs_dtype, rotary, cs_stride_b,
                          cs_stride_h, cs_stride_t);
   if (rc) return rc;
-  const QkShape sh = qk_shape(heads, kv_heads, head_dim, norm, batch * tokens);
-  ogx::qkn::Params p = qk_params(q, k, batch, tokens, heads, kv_heads, q_stride_b, q_stride_t, k_stride_b, k_stride_t,
-                                 q_weight, k_weight, weight_dtype, eps, cos, sin, cs_dtype, rotary, cs_stride_b,
-                                 cs_stride_h, cs_stride_t, sh);
-  if ((rc = qk_outputs(p, q_out, q_out_stride_b, q_out_stride_t, k_out, k_out_stride_b, k_out_stride_t))) return rc;
-  qk_dispatch<false>(p, head_dim, interleaved, sh, norm, static_cast<cudaStream_t>(stream));
+  QkShape sh[2];
+  int steps = 0;
+  ogx::qkn::Params p = qk_params(q, k, batch, tokens, heads, kv_heads, head_dim, q_stride_b, q_stride_t, k_stride_b,
+                                 k_stride_t, q_weight, k_weight, weight_dtype, norm, eps, cos, sin, cs_dtype, rotary,
+                                 cs_stride_b, cs_stride_h, cs_stride_t, false, sh, &steps);
+  if ((rc = qk_outputs(p, sh, q_out, q_out_stride_b, q_out_stride_t, k_out, k_out_stride_b, k_out_stride_t))) return rc;
+  qk_dispatch<false>(p, head_dim, interleaved, steps, norm, static_cast<cudaStream_t>(stream));
   return check_launch("qk_norm_rope_kernel");
 }
 
@@ -1779,8 +1809,8 @@ int ogx_qk_norm_rope_bwd_workspace(int64_t batch, int64_t tokens, int64_t heads,
       heads + kv_heads > kQkMaxHeads || (head_dim != 64 && head_dim != 128))
     return fail(OGX_EINVAL, "qk_shape");
   if (norm != kNone && norm != kHead && norm != kRow) return fail(OGX_EINVAL, "norm");
-  const QkShape sh = qk_shape(heads, kv_heads, head_dim, norm, batch * tokens);
-  *bytes = 4 * qk_partial_rows(sh, norm) * qk_weight_columns(norm, heads + kv_heads, head_dim);
+  *bytes = qk_partial_bytes(qk_shape(heads, kv_heads, head_dim, norm, true, batch * tokens), norm, heads, head_dim) +
+           qk_partial_bytes(qk_shape(kv_heads, heads, head_dim, norm, true, batch * tokens), norm, kv_heads, head_dim);
   return OGX_OK;
 }
 
@@ -1800,33 +1830,37 @@ int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq
   if (dq_out == nullptr || dk_out == nullptr || !aligned16(dq_out) || !aligned16(dk_out) || dq_out_stride_b % 8 ||
       dq_out_stride_t % 8 || dk_out_stride_b % 8 || dk_out_stride_t % 8)
     return fail(OGX_EINVAL, "output_gradients");
-  const QkShape sh = qk_shape(heads, kv_heads, head_dim, norm, batch * tokens);
-  ogx::qkn::Params p = qk_params(q, k, batch, tokens, heads, kv_heads, q_stride_b, q_stride_t, k_stride_b, k_stride_t,
-                                 q_weight, k_weight, weight_dtype, eps, cos, sin, cs_dtype, rotary, cs_stride_b,
-                                 cs_stride_h, cs_stride_t, sh);
-  p.dy[0] = static_cast<const __nv_bfloat16*>(dq_out);
-  p.dy[1] = static_cast<const __nv_bfloat16*>(dk_out);
-  p.dy_stride_b[0] = dq_out_stride_b;
-  p.dy_stride_t[0] = dq_out_stride_t;
-  p.dy_stride_b[1] = dk_out_stride_b;
-  p.dy_stride_t[1] = dk_out_stride_t;
-  if ((rc = qk_outputs(p, dq, dq_stride_b, dq_stride_t, dk, dk_stride_b, dk_stride_t))) return rc;
-  const int64_t columns = qk_weight_columns(norm, heads + kv_heads, head_dim);
-  const int64_t partial_rows = qk_partial_rows(sh, norm);
+  QkShape sh[2];
+  int steps = 0;
+  ogx::qkn::Params p = qk_params(q, k, batch, tokens, heads, kv_heads, head_dim, q_stride_b, q_stride_t, k_stride_b,
+                                 k_stride_t, q_weight, k_weight, weight_dtype, norm, eps, cos, sin, cs_dtype, rotary,
+                                 cs_stride_b, cs_stride_h, cs_stride_t, true, sh, &steps);
+  p.t[0].dy = qk_stream(dq_out, dq_out_stride_b, dq_out_stride_t, 2, tokens, sh[0].ctas * sh[0].teams);
+  p.t[1].dy = qk_stream(dk_out, dk_out_stride_b, dk_out_stride_t, 2, tokens, sh[1].ctas * sh[1].teams);
+  if ((rc = qk_outputs(p, sh, dq, dq_stride_b, dq_stride_t, dk, dk_stride_b, dk_stride_t))) return rc;
+  const int64_t q_bytes = qk_partial_bytes(sh[0], norm, heads, head_dim);
   if (norm != kNone) {
     if (dq_weight == nullptr || dk_weight == nullptr || !aligned4(dq_weight) || !aligned4(dk_weight))
       return fail(OGX_EINVAL, "weight_gradients");
-    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < 4 * partial_rows * columns)
+    if (workspace == nullptr || !aligned16(workspace) ||
+        workspace_bytes < q_bytes + qk_partial_bytes(sh[1], norm, kv_heads, head_dim))
       return fail(OGX_EINVAL, "workspace");
+    p.t[0].partials = static_cast<float*>(workspace);
+    p.t[1].partials = p.t[0].partials + q_bytes / 4;
   }
-  p.partials = static_cast<float*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  qk_dispatch<true>(p, head_dim, interleaved, sh, norm, s);
+  qk_dispatch<true>(p, head_dim, interleaved, steps, norm, s);
   if ((rc = check_launch("qk_norm_rope_kernel"))) return rc;
   if (norm == kNone) return OGX_OK;
-  launch(ogx::qkn::qk_norm_weight_sum_kernel, dim3(static_cast<unsigned>((columns + 31) / 32)), dim3(1024), 0, s,
-         static_cast<const float*>(p.partials), static_cast<int>(partial_rows), static_cast<int>(columns),
-         static_cast<int>(norm == kHead ? head_dim : heads * head_dim), dq_weight, dk_weight);
+  ogx::qkn::SumParams sp{};
+  for (int t = 0; t < 2; ++t) {
+    sp.partials[t] = p.t[t].partials;
+    sp.out[t] = t ? dk_weight : dq_weight;
+    sp.rows[t] = static_cast<int>(qk_partial_rows(sh[t], norm));
+    sp.cols[t] = static_cast<int>(qk_weight_columns(norm, p.t[t].heads, head_dim));
+  }
+  launch(ogx::qkn::qk_norm_weight_sum_kernel, dim3(static_cast<unsigned>((sp.cols[0] + 31) / 32 + (sp.cols[1] + 31) / 32)),
+         dim3(1024), 0, s, sp);
   return check_launch("qk_norm_weight_sum_kernel");
 }
 

@@ -9,8 +9,10 @@
 // (`hi`), so a rotation needs no other lane: two 8-byte loads at 4l and rotary/2 + 4l in the half layout; in the
 // interleaved one the low and the high halves of four packed words.  Past the rotated columns a lane holds 8
 // neighbours, with cos 1 and sin 0.  A head's sums travel by shuffles; a norm over the whole row adds the
-// groups' sums through shared memory.  CTAs are persistent, and while one works on its tokens the next ones are
-// on their way from HBM to L2 (bulk prefetches, which hold no registers).
+// groups' sums through shared memory.  A CTA works on q or on k (CTAs shared out by the heads), is persistent,
+// and while it works on its tokens the next ones are on their way from HBM to L2 (bulk prefetches by one warp,
+// which hold no registers).  Integer work per token would cost more issue slots than the norm: a thread keeps one
+// address per tensor and steps it by strides that the host has multiplied out.
 #pragma once
 
 #include "elementwise.cuh"
@@ -19,25 +21,40 @@ namespace ogx {
 namespace qkn {
 
 constexpr int kThreads = 256;
-constexpr int kRowThreads = 512;  // a row norm keeps all of a token's columns in registers
 enum Norm { kNone = 0, kHead = 1, kRow = 2 };
+// Resident CTAs per SM that the kernels are compiled for; a launch has at most one wave of them.
+__host__ __device__ constexpr int head_ctas(bool backward) { return backward ? 3 : 4; }
+__host__ __device__ constexpr int row_ctas(int threads, int steps) { return threads == 256 ? (steps == 1 ? 3 : 2) : 1; }
+
+// Rows of a tensor: the address of (batch, token) and the steps from a team's token to its next one (`wrap` more
+// when that crosses into another batch).  Bytes.
+struct Stream {
+  char* base;
+  int64_t stride_b, stride_t;
+  int64_t step, wrap;
+};
+
+// One of q and k.
+struct Tensor {
+  Stream x, dy, y;     // input rows; gradients of the output rows (backward); output rows or the input's gradients
+  Stream angles;       // offsets into cos and sin (base null)
+  const void* weight;  // [HD] (head), [heads * HD] (row)
+  float* partials;     // backward: [CTAs (head) or CTAs * teams (row)][weight columns]
+  int heads;
+  int team;            // groups per token, a power of two
+  int ctas;
+  int step_token;      // tokens (of a batch) from a team's token to its next one, batches left out
+};
 
 struct Params {
-  const __nv_bfloat16 *x[2];   // q, k (rows of heads * HD columns)
-  const __nv_bfloat16 *dy[2];  // gradients of the outputs (backward)
-  __nv_bfloat16* y[2];         // outputs, or the gradients of q and k
-  int64_t x_stride_b[2], x_stride_t[2], dy_stride_b[2], dy_stride_t[2], y_stride_b[2], y_stride_t[2];
-  const void* weight[2];       // [HD] (head), [heads * HD] (row)
-  const void *cos, *sin;       // [.., rotary / 2], element strides below
-  int64_t cs_stride_b, cs_stride_h, cs_stride_t;
-  int heads[2];
+  Tensor t[2];               // CTAs [0, t[0].ctas) take q, the rest k
+  const char *cos, *sin;     // [.., rotary / 2]
+  int64_t cs_stride_h;       // bytes; 0: shared by the heads
   int rotary;
-  int w_fp32, cs_fp32;         // else bf16
-  int team;                    // groups per token, a power of two
-  int64_t tokens;              // per batch
-  int64_t rows;                // batch * tokens
+  int w_fp32, cs_fp32;       // else bf16
+  int tokens;                // per batch
+  int rows;                  // batch * tokens
   float eps;
-  float* partials;             // backward: [gridDim.x, or row norm gridDim.x * teams][weight columns of q and k]
 };
 
 // The 8 columns of a lane as 2 + 2 packed pairs.
@@ -85,18 +102,19 @@ struct Columns {
       gap = p.rotary / 2;
     }
   }
-  __device__ __forceinline__ uint4 load(const __nv_bfloat16* head) const {
-    if constexpr (INTER) return __ldcs(reinterpret_cast<const uint4*>(head + lo));
-    const uint2 a = __ldcs(reinterpret_cast<const uint2*>(head + lo));
-    const uint2 b = __ldcs(reinterpret_cast<const uint2*>(head + lo + gap));
+  // `at`: the address of the lane's first column
+  __device__ __forceinline__ uint4 load(const char* at) const {
+    if constexpr (INTER) return __ldcs(reinterpret_cast<const uint4*>(at));
+    const uint2 a = __ldcs(reinterpret_cast<const uint2*>(at));
+    const uint2 b = __ldcs(reinterpret_cast<const uint2*>(at + gap * 2));
     return make_uint4(a.x, a.y, b.x, b.y);
   }
-  __device__ __forceinline__ void store(__nv_bfloat16* head, const uint4& v) const {
+  __device__ __forceinline__ void store(char* at, const uint4& v) const {
     if constexpr (INTER) {
-      __stcs(reinterpret_cast<uint4*>(head + lo), v);
+      __stcs(reinterpret_cast<uint4*>(at), v);
     } else {
-      __stcs(reinterpret_cast<uint2*>(head + lo), make_uint2(v.x, v.y));
-      __stcs(reinterpret_cast<uint2*>(head + lo + gap), make_uint2(v.z, v.w));
+      __stcs(reinterpret_cast<uint2*>(at), make_uint2(v.x, v.y));
+      __stcs(reinterpret_cast<uint2*>(at + gap * 2), make_uint2(v.z, v.w));
     }
   }
   // column of element e of (lo, hi) in the order of `Lane`: lo[0].x, lo[0].y, lo[1].x, .., hi[1].y
@@ -105,57 +123,86 @@ struct Columns {
   }
 };
 
-__device__ __forceinline__ void load4_of(const void* table, int64_t at, int fp32, f2 (&f)[2]) {
+// Four entries, from entry `entry` on, of the fp32 or bf16 values at `at`.
+__device__ __forceinline__ void load4_of(const char* at, int entry, int fp32, f2 (&f)[2]) {
   if (fp32) {
-    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(table) + at);
+    const float4 v = *reinterpret_cast<const float4*>(at + entry * 4);
     f[0] = f2{v.x, v.y};
     f[1] = f2{v.z, v.w};
   } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(table) + at);
+    const uint2 v = *reinterpret_cast<const uint2*>(at + entry * 2);
     f[0] = f2{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u)};
     f[1] = f2{__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u)};
   }
 }
 
-// cos and sin of a lane's four pairs; lanes past the rotated columns turn by nothing.  `sign` -1 turns back.
-struct Angles {
-  f2 c[2], s[2];
+// cos and sin of a lane's four pairs; lanes past the rotated columns turn by nothing; `sign` -1 turns back.
+struct Turn {
+  f2 c[2], s[2], ns[2];
+  // `at`: byte offset of the token's (and head's) first entry
   __device__ __forceinline__ void load(const Params& p, int64_t at, int sub, float sign) {
     if (sub * 8 < p.rotary) {
-      load4_of(p.cos, at + sub * 4, p.cs_fp32, c);
-      load4_of(p.sin, at + sub * 4, p.cs_fp32, s);
+      load4_of(p.cos + at, sub * 4, p.cs_fp32, c);
+      load4_of(p.sin + at, sub * 4, p.cs_fp32, s);
     } else {
       c[0] = c[1] = f2{1.f, 1.f};
       s[0] = s[1] = f2{0.f, 0.f};
     }
-    s[0] = mul2(s[0], f2{sign, sign});
-    s[1] = mul2(s[1], f2{sign, sign});
-  }
-  __device__ __forceinline__ void turn(Lane& v) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const f2 a = v.lo[i], b = v.hi[i];
-      const f2 t = mul2(b, s[i]);
-      v.lo[i] = fma2(a, c[i], f2{-t.x, -t.y});
-      v.hi[i] = fma2(b, c[i], mul2(a, s[i]));
+      ns[i] = mul2(s[i], f2{-sign, -sign});
+      s[i] = mul2(s[i], f2{sign, sign});
     }
+  }
+  __device__ __forceinline__ Lane operator()(const Lane& v) const {
+    Lane r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r.lo[i] = fma2(v.hi[i], ns[i], mul2(v.lo[i], c[i]));
+      r.hi[i] = fma2(v.lo[i], s[i], mul2(v.hi[i], c[i]));
+    }
+    return r;
+  }
+};
+
+// The weight and the rotation as one step: R(w o x).
+struct WeightedTurn {
+  f2 ll[2], lh[2], hl[2], hh[2];
+  __device__ __forceinline__ WeightedTurn(const Turn& t, const Lane& w) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      ll[i] = mul2(t.c[i], w.lo[i]);
+      lh[i] = mul2(t.ns[i], w.hi[i]);
+      hl[i] = mul2(t.s[i], w.lo[i]);
+      hh[i] = mul2(t.c[i], w.hi[i]);
+    }
+  }
+  __device__ __forceinline__ Lane operator()(const Lane& v) const {
+    Lane r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r.lo[i] = fma2(v.hi[i], lh[i], mul2(v.lo[i], ll[i]));
+      r.hi[i] = fma2(v.lo[i], hl[i], mul2(v.hi[i], hh[i]));
+    }
+    return r;
   }
 };
 
 template <bool INTER>
-__device__ __forceinline__ Lane load_weights(const Params& p, int t, int64_t at, const Columns<INTER>& col) {
+__device__ __forceinline__ Lane load_weights(const void* weights, int fp32, int at, const Columns<INTER>& col) {
+  const char* weight = static_cast<const char*>(weights);
   Lane w;
   if constexpr (INTER) {
     f2 a[2], b[2];
-    load4_of(p.weight[t], at + col.lo, p.w_fp32, a);
-    load4_of(p.weight[t], at + col.lo + 4, p.w_fp32, b);
+    load4_of(weight, at + col.lo, fp32, a);
+    load4_of(weight, at + col.lo + 4, fp32, b);
     w.lo[0] = f2{a[0].x, a[1].x};
     w.lo[1] = f2{b[0].x, b[1].x};
     w.hi[0] = f2{a[0].y, a[1].y};
     w.hi[1] = f2{b[0].y, b[1].y};
   } else {
-    load4_of(p.weight[t], at + col.lo, p.w_fp32, w.lo);
-    load4_of(p.weight[t], at + col.lo + col.gap, p.w_fp32, w.hi);
+    load4_of(weight, at + col.lo, fp32, w.lo);
+    load4_of(weight, at + col.lo + col.gap, fp32, w.hi);
   }
   return w;
 }
@@ -192,263 +239,316 @@ __device__ __forceinline__ void prefetch_row(const void* p, int bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
-// Prefetches row `row` of q, k and (backward) of their output gradients, one tensor per calling thread 0..3.
+// A CTA's place: its tensor and which of the tensor's CTAs it is.
+struct Place {
+  int tensor, cta;
+  __device__ __forceinline__ explicit Place(const Params& p) {
+    tensor = static_cast<int>(blockIdx.x) >= p.t[0].ctas;
+    cta = static_cast<int>(blockIdx.x) - (tensor ? p.t[0].ctas : 0);
+  }
+};
+
+__device__ __forceinline__ char* row_address(const Stream& s, int batch, int token) {
+  return s.base + batch * s.stride_b + token * s.stride_t;
+}
+
+// A team's token, stepping through the rows with additions.
+struct Cursor {
+  int row, token;
+  bool wrapped;  // the last step crossed into another batch
+  __device__ __forceinline__ void step(const Params& p, const Tensor& a, int rows) {
+    row += rows;
+    token += a.step_token;
+    wrapped = token >= p.tokens;
+    if (wrapped) token -= p.tokens;
+  }
+};
+__device__ __forceinline__ int64_t step_of(const Stream& s, bool wrapped) { return wrapped ? s.step + s.wrap : s.step; }
+
+// The rows of the CTA's tokens [row0, row0 + teams) to L2, by its first warp.
 template <int HD, bool X, bool DY>
-__device__ __forceinline__ void prefetch_token(const Params& p, int64_t row, int which) {
-  const int t = which & 1;
-  if (row >= p.rows) return;
-  const int64_t batch = row / p.tokens, token = row - batch * p.tokens;
-  if (which < 2 ? X : false) prefetch_row(p.x[t] + batch * p.x_stride_b[t] + token * p.x_stride_t[t], p.heads[t] * HD * 2);
-  if (which >= 2 ? DY : false)
-    prefetch_row(p.dy[t] + batch * p.dy_stride_b[t] + token * p.dy_stride_t[t], p.heads[t] * HD * 2);
+__device__ __forceinline__ void prefetch_rows(const Params& p, const Tensor& a, int row0, int teams) {
+  if (threadIdx.x >= 32) return;
+  for (int i = threadIdx.x; i < 2 * teams; i += 32) {
+    const int row = row0 + (i >> 1);
+    if (row >= p.rows) break;
+    const int batch = row / p.tokens, token = row - batch * p.tokens;
+    if (X && (i & 1) == 0) prefetch_row(row_address(a.x, batch, token), a.heads * HD * 2);
+    if (DY && (i & 1) == 1) prefetch_row(row_address(a.dy, batch, token), a.heads * HD * 2);
+  }
+}
+
+// Its part of a head's angles to L2, by each lane (bulk prefetches of so small pieces, one lane after the other,
+// took longer than the rows themselves).
+__device__ __forceinline__ void prefetch_angles(const Params& p, int64_t at, int sub) {
+  if (sub * 8 >= p.rotary) return;
+  const int64_t own = at + sub * (p.cs_fp32 ? 16 : 8);
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p.cos + own));
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p.sin + own));
+}
+
+__device__ __forceinline__ void elements(const Lane& v, float (&e)[8]) {
+  e[0] = v.lo[0].x; e[1] = v.lo[0].y; e[2] = v.lo[1].x; e[3] = v.lo[1].y;
+  e[4] = v.hi[0].x; e[5] = v.hi[0].y; e[6] = v.hi[1].x; e[7] = v.hi[1].y;
 }
 
 // ------------------------------------------------------------------------- norm of each head, or no norm
 // A group's heads are independent; UNROLL of them are loaded before the first is used.
-template <int HD, int NORM, bool INTER, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads, BACKWARD ? 3 : 4) qk_head_kernel(Params p) {
+template <int HD, int NORM, bool INTER, bool PER_HEAD, bool BACKWARD>
+__global__ void __launch_bounds__(kThreads, head_ctas(BACKWARD)) qk_head_kernel(const __grid_constant__ Params p) {
   constexpr int LANES = HD / 8;
   constexpr int GROUPS = kThreads / LANES;
   constexpr int UNROLL = BACKWARD ? 2 : 4;
   constexpr bool X = NORM != kNone || !BACKWARD;
-  __shared__ __align__(16) float weights[NORM == kHead ? 2 : 1][NORM == kHead ? HD : 4];  // lane by lane
+  constexpr float sign = BACKWARD ? -1.f : 1.f;
   pdl_trigger();
   pdl_wait();
+  const Place place(p);
+  const Tensor& a = p.t[place.tensor];
   const int sub = threadIdx.x % LANES;
   const int group = threadIdx.x / LANES;
-  const int member = group % p.team;
-  const int team = group / p.team;
-  const int teams = GROUPS / p.team;
+  const int heads = a.heads, stride = a.team;
+  const int member = group & (stride - 1);
+  const int team = group / stride;
+  const int teams = GROUPS / stride;
   const Columns<INTER> col(p, sub);
-  if constexpr (NORM == kHead) {
-    if (group < 2) {
-      const Lane w = load_weights<INTER>(p, group, 0, col);
-      *reinterpret_cast<Lane*>(&weights[group][sub * 8]) = w;
-    }
-    __syncthreads();
-  }
-  Lane dw[BACKWARD && NORM == kHead ? 2 : 1] = {};
+  Lane w;
+  if constexpr (NORM == kHead) w = load_weights<INTER>(a.weight, p.w_fp32, 0, col);
+  Lane dw{};
 
-  const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
+  const int rows_per_step = a.ctas * teams;
+  Cursor at{place.cta * teams + team, 0, false};
+  const int batch0 = at.row / p.tokens;
+  at.token = at.row - batch0 * p.tokens;
+  const int offset = (member * HD + col.lo) * 2;
+  const char* xp = row_address(a.x, batch0, at.token) + offset;
+  const char* dp = BACKWARD ? row_address(a.dy, batch0, at.token) + offset : nullptr;
+  char* yp = row_address(a.y, batch0, at.token) + offset;
+  int64_t angles = batch0 * a.angles.stride_b + at.token * a.angles.stride_t;
+  uint4 xr[UNROLL] = {}, dr[UNROLL] = {};  // idle slots keep what was there before, and write nothing
   // whole warps run every iteration: the shuffles name all lanes
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * teams; row0 < p.rows; row0 += step) {
-    if (threadIdx.x < 4 * teams) prefetch_token<HD, X, BACKWARD>(p, row0 + step + threadIdx.x / 4, threadIdx.x & 3);
-    const int64_t row = row0 + team;
-    const bool row_ok = row < p.rows;
-    const int64_t batch = row_ok ? row / p.tokens : 0;
-    const int64_t token = row_ok ? row - batch * p.tokens : 0;
-    const int64_t angles = batch * p.cs_stride_b + token * p.cs_stride_t;
-    Angles a;
-    if (p.cs_stride_h == 0) a.load(p, angles, sub, BACKWARD ? -1.f : 1.f);
+  for (int row0 = place.cta * teams; row0 < p.rows; row0 += rows_per_step) {
+    prefetch_rows<HD, X, BACKWARD>(p, a, row0 + rows_per_step, teams);
+    const bool row_ok = at.row < p.rows;
+    Turn turn{};
+    if constexpr (!PER_HEAD) {
+      if (row_ok) turn.load(p, angles, sub, sign);
+    }
+    const WeightedTurn step1(turn, w);  // used by the forward pass of a norm with shared tables
+    for (int i0 = 0; i0 < heads; i0 += UNROLL * stride) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const __nv_bfloat16* xrow = p.x[t] + batch * p.x_stride_b[t] + token * p.x_stride_t[t];
-      const __nv_bfloat16* drow = BACKWARD ? p.dy[t] + batch * p.dy_stride_b[t] + token * p.dy_stride_t[t] : nullptr;
-      __nv_bfloat16* yrow = p.y[t] + batch * p.y_stride_b[t] + token * p.y_stride_t[t];
-      for (int i0 = 0; i0 < p.heads[t]; i0 += UNROLL * p.team) {
-        uint4 xr[UNROLL], dr[BACKWARD ? UNROLL : 1];
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-          const int h = i0 + u * p.team + member;
-          const bool ok = row_ok && h < p.heads[t];
-          if (X) xr[u] = ok ? col.load(xrow + h * HD) : make_uint4(0, 0, 0, 0);
-          if constexpr (BACKWARD) dr[u] = ok ? col.load(drow + h * HD) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-          if (i0 + u * p.team >= p.heads[t]) break;  // the same for the whole CTA
-          const int h = i0 + u * p.team + member;
-          const bool ok = row_ok && h < p.heads[t];
-          if (p.cs_stride_h != 0) a.load(p, angles + (ok ? h : 0) * p.cs_stride_h, sub, BACKWARD ? -1.f : 1.f);
-          Lane v;
-          if constexpr (!BACKWARD) {
-            v = unpack_lane<INTER>(xr[u]);
-            if constexpr (NORM == kHead) {
-              const float r = rsqrtf(group_sum<LANES>(dot(v, v)) * (1.f / HD) + p.eps);
-              v = mul(mul(v, r), *reinterpret_cast<const Lane*>(&weights[t][sub * 8]));
-            }
-            a.turn(v);
-          } else {
-            v = unpack_lane<INTER>(dr[u]);
-            a.turn(v);
-            if constexpr (NORM == kHead) {
-              const Lane x = unpack_lane<INTER>(xr[u]);
-              const Lane gw = mul(v, *reinterpret_cast<const Lane*>(&weights[t][sub * 8]));
-              const float sq = group_sum<LANES>(dot(x, x)), gwx = group_sum<LANES>(dot(gw, x));
-              const float r = rsqrtf(sq * (1.f / HD) + p.eps);
-              const float along = gwx * (1.f / HD) * r * r * r;
-              dw[t] = fma(mul(v, x), ok ? r : 0.f, dw[t]);  // idle slots hold zeros, whose r may be infinite
-              v = fma(x, -along, mul(gw, r));
-            }
-          }
-          if (ok) col.store(yrow + h * HD, pack_lane<INTER>(v));
+      for (int u = 0; u < UNROLL; ++u) {
+        const int h = i0 + u * stride;
+        if (row_ok && h + member < heads) {
+          if constexpr (X) xr[u] = col.load(xp + h * (HD * 2));
+          if constexpr (BACKWARD) dr[u] = col.load(dp + h * (HD * 2));
         }
       }
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int h = i0 + u * stride;
+        if (h >= heads) break;  // the same for the whole CTA
+        const bool ok = row_ok && h + member < heads;
+        if constexpr (PER_HEAD) {
+          if (ok) turn.load(p, angles + (h + member) * p.cs_stride_h, sub, sign);
+        }
+        Lane v;
+        if constexpr (NORM == kNone) {
+          v = turn(unpack_lane<INTER>(BACKWARD ? dr[u] : xr[u]));
+        } else if constexpr (!BACKWARD) {
+          const Lane x = unpack_lane<INTER>(xr[u]);
+          const float inv = rsqrtf(group_sum<LANES>(dot(x, x)) * (1.f / HD) + p.eps);
+          v = mul(PER_HEAD ? turn(mul(x, w)) : step1(x), inv);
+        } else {
+          const Lane x = unpack_lane<INTER>(xr[u]);
+          const Lane g = turn(unpack_lane<INTER>(dr[u]));
+          const Lane gx = mul(g, x);
+          const float sq = group_sum<LANES>(dot(x, x)), gwx = group_sum<LANES>(dot(gx, w));
+          const float inv = rsqrtf(sq * (1.f / HD) + p.eps);
+          if (ok) dw = fma(gx, inv, dw);
+          v = fma(x, -gwx * (1.f / HD) * inv * inv * inv, mul(mul(g, w), inv));
+        }
+        if (ok) col.store(yp + h * (HD * 2), pack_lane<INTER>(v));
+      }
     }
+    at.step(p, a, rows_per_step);
+    if constexpr (X) xp += step_of(a.x, at.wrapped);
+    if constexpr (BACKWARD) dp += step_of(a.dy, at.wrapped);
+    yp += step_of(a.y, at.wrapped);
+    angles += step_of(a.angles, at.wrapped);
   }
 
   if constexpr (BACKWARD && NORM == kHead) {
-    // this CTA's share of the weight gradients, summed over the rows it took
-    __shared__ float part[GROUPS][2 * HD];
+    // this CTA's share of the weight gradient, summed over the rows it took
+    __shared__ float part[GROUPS][HD];
+    float e[8];
+    elements(dw, e);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const float e[8] = {dw[t].lo[0].x, dw[t].lo[0].y, dw[t].lo[1].x, dw[t].lo[1].y,
-                          dw[t].hi[0].x, dw[t].hi[0].y, dw[t].hi[1].x, dw[t].hi[1].y};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) part[group][t * HD + col.column(i)] = e[i];
-    }
+    for (int i = 0; i < 8; ++i) part[group][col.column(i)] = e[i];
     __syncthreads();
-    for (int c = threadIdx.x; c < 2 * HD; c += kThreads) {
+    if (threadIdx.x < HD) {
       float v = 0.f;
 #pragma unroll
-      for (int m = 0; m < GROUPS; ++m) v += part[m][c];
-      p.partials[static_cast<int64_t>(blockIdx.x) * (2 * HD) + c] = v;
+      for (int m = 0; m < GROUPS; ++m) v += part[m][threadIdx.x];
+      a.partials[static_cast<int64_t>(place.cta) * HD + threadIdx.x] = v;
     }
   }
 }
 
 // ------------------------------------------------------------------------- norm over all heads of a row
-// A team holds its token's columns (STEPS heads of q and of k per group) until the row's sums are known.
-template <int HD, int STEPS, bool INTER, bool BACKWARD>
-__global__ void __launch_bounds__(kRowThreads, STEPS == 1 ? 2 : 1) qk_row_kernel(Params p) {
+// A team holds its token's columns (STEPS heads per group) until the row's sums are known.
+template <int HD, int THREADS, int STEPS, bool INTER, bool BACKWARD>
+__global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kernel(const __grid_constant__ Params p) {
   constexpr int LANES = HD / 8;
-  constexpr int GROUPS = kRowThreads / LANES;
-  __shared__ __align__(16) float sums[2][GROUPS][4];  // alternating rows: each group's q (x^2, g w x), k (x^2, g w x)
+  constexpr int GROUPS = THREADS / LANES;
+  constexpr float sign = BACKWARD ? -1.f : 1.f;
+  __shared__ __align__(8) float sums[2][GROUPS][2];  // alternating rows: each group's sums of x^2 and g w x
   pdl_trigger();
   pdl_wait();
+  const Place place(p);
+  const Tensor& a = p.t[place.tensor];
   const int sub = threadIdx.x % LANES;
   const int group = threadIdx.x / LANES;
-  const int member = group % p.team;
-  const int team = group / p.team;
-  const int teams = GROUPS / p.team;
+  const int heads = a.heads, stride = a.team;
+  const int member = group & (stride - 1);
+  const int team = group / stride;
+  const int teams = GROUPS / stride;
   const Columns<INTER> col(p, sub);
-  Lane dw[BACKWARD ? 2 : 1][BACKWARD ? STEPS : 1] = {};
+  const float n = 1.f / static_cast<float>(heads * HD);
+  Lane dw[STEPS] = {};
+  // the weights of the group's heads stay in registers (four heads would not fit: they are read again)
+  constexpr bool KEEP = STEPS <= 2;
+  Lane w[STEPS];
+  const auto weights_of = [&](int i) {
+    const int h = i * stride + member;
+    return load_weights<INTER>(a.weight, p.w_fp32, (h < heads ? h : 0) * HD, col);
+  };
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) w[i] = weights_of(i);
+  }
 
-  const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
+  const int rows_per_step = a.ctas * teams;
+  Cursor at{place.cta * teams + team, 0, false};
+  const int batch0 = at.row / p.tokens;
+  at.token = at.row - batch0 * p.tokens;
+  const int offset = (member * HD + col.lo) * 2;
+  const char* xp = row_address(a.x, batch0, at.token) + offset;
+  const char* dp = BACKWARD ? row_address(a.dy, batch0, at.token) + offset : nullptr;
+  char* yp = row_address(a.y, batch0, at.token) + offset;
+  int64_t angles = batch0 * a.angles.stride_b + at.token * a.angles.stride_t;
+  const bool per_head = p.cs_stride_h != 0;
   int flip = 0;
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * teams; row0 < p.rows; row0 += step, flip ^= 1) {
-    if (threadIdx.x < 4 * teams) prefetch_token<HD, true, BACKWARD>(p, row0 + step + threadIdx.x / 4, threadIdx.x & 3);
-    const int64_t row = row0 + team;
-    const bool row_ok = row < p.rows;
-    const int64_t batch = row_ok ? row / p.tokens : 0;
-    const int64_t token = row_ok ? row - batch * p.tokens : 0;
-    const int64_t angles = batch * p.cs_stride_b + token * p.cs_stride_t;
-    uint4 xr[2][STEPS], dr[BACKWARD ? 2 : 1][BACKWARD ? STEPS : 1];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int h = i * p.team + member;
-        const bool ok = row_ok && h < p.heads[t];
-        xr[t][i] = ok ? col.load(p.x[t] + batch * p.x_stride_b[t] + token * p.x_stride_t[t] + h * HD)
-                      : make_uint4(0, 0, 0, 0);
-        if constexpr (BACKWARD)
-          dr[t][i] = ok ? col.load(p.dy[t] + batch * p.dy_stride_b[t] + token * p.dy_stride_t[t] + h * HD)
-                        : make_uint4(0, 0, 0, 0);
-      }
-    }
-    Angles a;
-    if (p.cs_stride_h == 0) a.load(p, angles, sub, BACKWARD ? -1.f : 1.f);
-    // the heads of q and k that a lane holds share their angles
-    float part[2][2] = {};
+  for (int row0 = place.cta * teams; row0 < p.rows; row0 += rows_per_step, flip ^= 1) {
+    prefetch_rows<HD, true, BACKWARD>(p, a, row0 + rows_per_step, teams);
+    const bool row_ok = at.row < p.rows;
+    uint4 xr[STEPS], dr[STEPS];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      const int h = i * p.team + member;
-      if (BACKWARD && p.cs_stride_h != 0) a.load(p, angles + (h < p.heads[0] ? h : 0) * p.cs_stride_h, sub, -1.f);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const Lane x = unpack_lane<INTER>(xr[t][i]);
-        part[t][0] += dot(x, x);
-        if constexpr (BACKWARD) {
-          Lane g = unpack_lane<INTER>(dr[t][i]);
-          a.turn(g);
-          const Lane w = load_weights<INTER>(p, t, static_cast<int64_t>(h < p.heads[t] ? h : 0) * HD, col);
-          part[t][1] += dot(mul(g, w), x);
-        }
+      xr[i] = dr[i] = make_uint4(0, 0, 0, 0);
+      if (row_ok && i * stride + member < heads) {
+        xr[i] = col.load(xp + i * stride * (HD * 2));
+        if constexpr (BACKWARD) dr[i] = col.load(dp + i * stride * (HD * 2));
       }
     }
+    at.step(p, a, rows_per_step);
+    const int64_t angles_next = angles + step_of(a.angles, at.wrapped);
+    if (per_head && at.row < p.rows) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      part[t][0] = group_sum<LANES>(part[t][0]);
-      if (BACKWARD) part[t][1] = group_sum<LANES>(part[t][1]);
+      for (int i = 0; i < STEPS; ++i)
+        if (i * stride + member < heads) prefetch_angles(p, angles_next + (i * stride + member) * p.cs_stride_h, sub);
     }
-    if (sub == 0)
-      *reinterpret_cast<float4*>(sums[flip][group]) = make_float4(part[0][0], part[0][1], part[1][0], part[1][1]);
+    Turn turn{};
+    if (!per_head && row_ok) turn.load(p, angles, sub, sign);
+    Lane x[STEPS], g[STEPS];
+    float sq = 0.f, gwx = 0.f;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int h = i * stride + member;
+      x[i] = unpack_lane<INTER>(xr[i]);
+      sq += dot(x[i], x[i]);
+      if ((BACKWARD || STEPS == 1) && per_head && row_ok && h < heads)
+        turn.load(p, angles + h * p.cs_stride_h, sub, sign);
+      if constexpr (BACKWARD) {
+        if constexpr (!KEEP) w[i] = weights_of(i);
+        g[i] = turn(unpack_lane<INTER>(dr[i]));
+        gwx += dot(mul(g[i], w[i]), x[i]);
+      }
+    }
+    sq = group_sum<LANES>(sq);
+    if constexpr (BACKWARD) gwx = group_sum<LANES>(gwx);
+    if (sub == 0) *reinterpret_cast<float2*>(sums[flip][group]) = make_float2(sq, gwx);
     __syncthreads();  // the other half of `sums` is written only after every thread has passed here again
-    float4 total = make_float4(0.f, 0.f, 0.f, 0.f);
-    // lanes of a group take the team's sums in turn
-    for (int m = sub; m < p.team; m += LANES) {
-      const float4 v = *reinterpret_cast<const float4*>(sums[flip][team * p.team + m]);
-      total.x += v.x;
-      total.y += v.y;
-      total.z += v.z;
-      total.w += v.w;
+    sq = gwx = 0.f;
+    for (int m = sub; m < stride; m += LANES) {
+      const float2 v = *reinterpret_cast<const float2*>(sums[flip][team * stride + m]);
+      sq += v.x;
+      gwx += v.y;
     }
-    const float sq[2] = {group_sum<LANES>(total.x), group_sum<LANES>(total.z)};
-    float gwx[2] = {0.f, 0.f};
-    if constexpr (BACKWARD) {
-      gwx[0] = group_sum<LANES>(total.y);
-      gwx[1] = group_sum<LANES>(total.w);
-    }
+    sq = group_sum<LANES>(sq);
+    const float inv = rsqrtf(sq * n + p.eps);
+    float along = 0.f;
+    if constexpr (BACKWARD) along = -group_sum<LANES>(gwx) * n * inv * inv * inv;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      const int h = i * p.team + member;
-      if (p.cs_stride_h != 0)
-        a.load(p, angles + (h < p.heads[0] ? h : 0) * p.cs_stride_h, sub, BACKWARD ? -1.f : 1.f);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const float n = 1.f / static_cast<float>(p.heads[t] * HD);
-        const float r = rsqrtf(sq[t] * n + p.eps);
-        const bool ok = row_ok && h < p.heads[t];
-        const Lane w = load_weights<INTER>(p, t, static_cast<int64_t>(h < p.heads[t] ? h : 0) * HD, col);
-        Lane v;
-        if constexpr (!BACKWARD) {
-          v = mul(mul(unpack_lane<INTER>(xr[t][i]), r), w);
-          a.turn(v);
-        } else {
-          const Lane x = unpack_lane<INTER>(xr[t][i]);
-          Lane g = unpack_lane<INTER>(dr[t][i]);
-          a.turn(g);
-          dw[t][i] = fma(mul(g, x), ok ? r : 0.f, dw[t][i]);
-          v = fma(x, -(gwx[t] * n * r * r * r), mul(mul(g, w), r));
-        }
-        if (ok)
-          col.store(p.y[t] + batch * p.y_stride_b[t] + token * p.y_stride_t[t] + h * HD, pack_lane<INTER>(v));
+      const int h = i * stride + member;
+      const bool ok = row_ok && h < heads;
+      Lane v;
+      if constexpr (!BACKWARD) {
+        // with one head per group its angles are still there
+        if (STEPS > 1 && per_head && ok) turn.load(p, angles + h * p.cs_stride_h, sub, sign);
+        if constexpr (!KEEP) w[i] = weights_of(i);
+        v = turn(mul(mul(x[i], inv), w[i]));
+      } else {
+        if constexpr (!KEEP) w[i] = weights_of(i);
+        if (ok) dw[i] = fma(mul(g[i], x[i]), inv, dw[i]);
+        v = fma(x[i], along, mul(mul(g[i], w[i]), inv));
       }
+      if (ok) col.store(yp + i * stride * (HD * 2), pack_lane<INTER>(v));
     }
+    xp += step_of(a.x, at.wrapped);
+    if constexpr (BACKWARD) dp += step_of(a.dy, at.wrapped);
+    yp += step_of(a.y, at.wrapped);
+    angles = angles_next;
   }
 
   if constexpr (BACKWARD) {
-    const int columns = (p.heads[0] + p.heads[1]) * HD;
-    float* dst = p.partials + (static_cast<int64_t>(blockIdx.x) * teams + team) * columns;
+    float* dst = a.partials + (static_cast<int64_t>(place.cta) * teams + team) * (heads * HD);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int i = 0; i < STEPS; ++i) {
+      const int h = i * stride + member;
+      if (h < heads) {
+        float e[8];
+        elements(dw[i], e);
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int h = i * p.team + member;
-        if (h < p.heads[t]) {
-          const float e[8] = {dw[t][i].lo[0].x, dw[t][i].lo[0].y, dw[t][i].lo[1].x, dw[t][i].lo[1].y,
-                              dw[t][i].hi[0].x, dw[t][i].hi[0].y, dw[t][i].hi[1].x, dw[t][i].hi[1].y};
-#pragma unroll
-          for (int k = 0; k < 8; ++k) dst[(t * p.heads[0] + h) * HD + col.column(k)] = e[k];
-        }
+        for (int k = 0; k < 8; ++k) dst[h * HD + col.column(k)] = e[k];
       }
     }
   }
 }
 
-// Sums the partial weight gradients over their rows in a fixed order: 32 columns per CTA, 32 slices of rows.
-__global__ void __launch_bounds__(1024) qk_norm_weight_sum_kernel(const float* __restrict__ partials, int rows, int cols,
-                                                                  int q_cols, float* dq_weight, float* dk_weight) {
+// Sums the partial weight gradients of q (and behind them of k) over their rows in a fixed order: 32 columns per
+// CTA, 32 slices of rows.
+struct SumParams {
+  const float* partials[2];
+  float* out[2];
+  int rows[2], cols[2];
+};
+
+__global__ void __launch_bounds__(1024) qk_norm_weight_sum_kernel(const __grid_constant__ SumParams p) {
   __shared__ float part[32][33];
   pdl_trigger();
   pdl_wait();
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+  const int q_ctas = (p.cols[0] + 31) / 32;
+  const int t = static_cast<int>(blockIdx.x) >= q_ctas;
+  const int cols = p.cols[t], rows = p.rows[t];
+  const int col = (static_cast<int>(blockIdx.x) - (t ? q_ctas : 0)) * 32 + (threadIdx.x & 31);
   const int slice = threadIdx.x >> 5;
   float v = 0.f;
   if (col < cols) {
-#pragma unroll 8
-    for (int r = slice; r < rows; r += 32) v += partials[static_cast<int64_t>(r) * cols + col];
+    const float* src = p.partials[t] + col;
+#pragma unroll 16
+    for (int r = slice; r < rows; r += 32) v += src[static_cast<int64_t>(r) * cols];
   }
   part[slice][threadIdx.x & 31] = v;
   __syncthreads();
@@ -456,10 +556,7 @@ __global__ void __launch_bounds__(1024) qk_norm_weight_sum_kernel(const float* _
     v = 0.f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) v += part[i][threadIdx.x];
-    if (col < q_cols)
-      dq_weight[col] = v;
-    else
-      dk_weight[col - q_cols] = v;
+    p.out[t][col] = v;
   }
 }
 
