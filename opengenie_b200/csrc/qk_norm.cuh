@@ -438,19 +438,23 @@ __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kern
   char* yp = row_address(a.y, batch0, at.token) + offset;
   int64_t angles = batch0 * a.angles.stride_b + at.token * a.angles.stride_t;
   const bool per_head = p.cs_stride_h != 0;
-  int flip = 0;
-  for (int row0 = place.cta * teams; row0 < p.rows; row0 += rows_per_step, flip ^= 1) {
-    prefetch_rows<HD, true, BACKWARD>(p, a, row0 + rows_per_step, teams);
-    const bool row_ok = at.row < p.rows;
-    uint4 xr[STEPS], dr[STEPS];
+  uint4 xr[STEPS] = {}, dr[STEPS] = {};
+  const auto load_row = [&](bool ok) {
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      xr[i] = dr[i] = make_uint4(0, 0, 0, 0);
-      if (row_ok && i * stride + member < heads) {
+      if (ok && i * stride + member < heads) {
         xr[i] = col.load(xp + i * stride * (HD * 2));
         if constexpr (BACKWARD) dr[i] = col.load(dp + i * stride * (HD * 2));
+      } else {
+        xr[i] = dr[i] = make_uint4(0, 0, 0, 0);
       }
     }
+  };
+  load_row(at.row < p.rows);
+  int flip = 0;
+  for (int row0 = place.cta * teams; row0 < p.rows; row0 += rows_per_step, flip ^= 1) {
+    prefetch_rows<HD, true, BACKWARD>(p, a, row0 + 2 * rows_per_step, teams);
+    const bool row_ok = at.row < p.rows;
     at.step(p, a, rows_per_step);
     const int64_t angles_next = angles + step_of(a.angles, at.wrapped);
     if (per_head && at.row < p.rows) {
@@ -475,6 +479,10 @@ __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kern
         gwx += dot(mul(g[i], w[i]), x[i]);
       }
     }
+    // the next row's loads run behind this row's sums and outputs
+    xp += step_of(a.x, at.wrapped);
+    if constexpr (BACKWARD) dp += step_of(a.dy, at.wrapped);
+    load_row(at.row < p.rows);
     sq = group_sum<LANES>(sq);
     if constexpr (BACKWARD) gwx = group_sum<LANES>(gwx);
     if (sub == 0) *reinterpret_cast<float2*>(sums[flip][group]) = make_float2(sq, gwx);
@@ -506,8 +514,6 @@ __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kern
       }
       if (ok) col.store(yp + i * stride * (HD * 2), pack_lane<INTER>(v));
     }
-    xp += step_of(a.x, at.wrapped);
-    if constexpr (BACKWARD) dp += step_of(a.dy, at.wrapped);
     yp += step_of(a.y, at.wrapped);
     angles = angles_next;
   }
