@@ -94,9 +94,16 @@ void launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaSt
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int sm_count() {
+  static std::atomic<int> known[64];  // per device ordinal
   int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return n;
+  if (dev < 64) {
+    const int k = known[dev].load(std::memory_order_relaxed);
+    if (k > 0) return k;
+  }
+  const bool ok = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0;
+  if (ok && dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return ok ? n : 148;
 }
 
 // ------------------------------------------------------------- tensor maps
@@ -907,12 +914,17 @@ int attention_common(const void* q, const void* k, const void* v, int64_t batch,
 // The softmax warpgroups raise their register limit with setmaxnreg, drawing on the registers the
 // launch reserved; only launch a build whose per-thread count is the one the split was sized for.
 int attn_register_split_ok(const void* kern) {
+  static std::mutex mu;
+  static std::unordered_map<const void*, bool> checked;  // a kernel's register count does not change
+  std::lock_guard<std::mutex> lock(mu);
+  if (checked.count(kern)) return OGX_OK;
   cudaFuncAttributes attr;
   int rc = check_cuda(cudaFuncGetAttributes(&attr, kern), "cudaFuncGetAttributes");
   if (rc) return rc;
   if (attr.numRegs != ogx::attn::kLaunchRegs)
     return fail(OGX_ECUDA, "attention kernel built with %d registers per thread, the register split needs %d", attr.numRegs,
                 ogx::attn::kLaunchRegs);
+  checked[kern] = true;
   return OGX_OK;
 }
 

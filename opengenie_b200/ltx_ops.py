@@ -14,6 +14,7 @@ only read inputs and write outputs, on the current CUDA stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -39,6 +40,16 @@ def _code(t: torch.Tensor) -> int:
 
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """Calls an entry point with ``device`` current, on its current stream (the entry's last argument)."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -1050,52 +1061,73 @@ def attention(
 
 
 # ---------------------------------------------------------------- training pass: attention and its gradients
-def _row_strides(t: torch.Tensor) -> tuple[int, int]:
-    """(batch stride, token stride) of rows [B, L, C]; axes of one entry count as contiguous."""
+def _rows(t: torch.Tensor, *, written: bool = False) -> tuple[int, int] | None:
+    """(batch stride, token stride) of bf16 rows [B, L, C] that the kernels can address: unit column stride and
+    16-byte aligned rows that do not overlap (nor, where they are written, do batches).  None if they cannot.
+    Axes of one entry count as contiguous."""
     B, L, C = t.shape
-    stride_t = t.stride(1) if L > 1 else C
-    return (t.stride(0) if B > 1 else L * stride_t), stride_t
+    stride_b, stride_t, stride_c = t.stride()
+    if L == 1:
+        stride_t = C
+    if B == 1:
+        stride_b = L * stride_t
+    if stride_c != 1 or stride_t % 8 or stride_b % 8 or stride_t < C or t.data_ptr() % 16:
+        return None
+    # a batch behind the other, or batches interleaved within the token stride
+    if written and B > 1 and not (stride_b >= (L - 1) * stride_t + C
+                                  or (stride_b >= C and stride_t >= (B - 1) * stride_b + C)):
+        return None
+    return stride_b, stride_t
 
 
-def _rows_ok(t: torch.Tensor, *, written: bool = False) -> bool:
-    """bf16 rows the kernels can address: unit column stride, 16-byte aligned rows that do not overlap."""
-    stride_b, stride_t = _row_strides(t)
-    ok = (t.stride(-1) == 1 and stride_t % 8 == 0 and stride_b % 8 == 0 and stride_t >= t.shape[2]
-          and t.data_ptr() % 16 == 0)
-    if written and t.shape[0] > 1:
-        # a batch behind the other, or batches interleaved within the token stride
-        ok = ok and (stride_b >= (t.shape[1] - 1) * stride_t + t.shape[2]
-                     or (stride_b >= t.shape[2] and stride_t >= (t.shape[0] - 1) * stride_b + t.shape[2]))
-    return ok
+def _given_rows(t: torch.Tensor, like: torch.Tensor, reason: str, *, written: bool = True) -> tuple[int, int]:
+    """The strides of a tensor the caller gave beside ``like``: bf16 rows of its shape on its device."""
+    if t.shape != like.shape or t.dtype != torch.bfloat16 or t.device != like.device:
+        raise ValueError(reason)
+    rows = _rows(t, written=written)
+    if rows is None:
+        raise ValueError(reason)
+    return rows
 
 
-def _masked_attention_reason(q, k, v, heads, kv_heads, causal_block, q_lengths, kv_lengths) -> str | None:
-    for t in (q, k, v):
-        if not t.is_cuda or t.device != q.device or t.dtype != torch.bfloat16:
-            return "qkv_device_or_dtype"
-    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0]:
-        return "qkv_shape"
-    if min(q.shape) < 1 or min(k.shape) < 1:
-        return "qkv_shape"
-    if heads < 1 or q.shape[2] != heads * 128:
-        return "head_dim"
-    if kv_heads < 1 or heads % kv_heads or k.shape[2] != kv_heads * 128:
-        return "kv_heads"
-    if not (_rows_ok(q) and _rows_ok(k) and _rows_ok(v)) or _row_strides(k) != _row_strides(v):
-        return "qkv_stride"
+def _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block, q_lengths, kv_lengths):
+    """Checks of the masked attention's common arguments; (q's strides, k's and v's strides, scale)."""
+    device = q.device
+    if device.type != "cuda" or k.device != device or v.device != device:
+        raise ValueError("qkv_device_or_dtype")
+    if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError("qkv_device_or_dtype")
+    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape:
+        raise ValueError("qkv_shape")
+    B, L, C = q.shape
+    Bk, M, Ck = k.shape
+    if Bk != B or B < 1 or L < 1 or M < 1:
+        raise ValueError("qkv_shape")
+    if heads < 1 or C != heads * 128:
+        raise ValueError("head_dim")
+    if kv_heads < 1 or heads % kv_heads or Ck != kv_heads * 128:
+        raise ValueError("kv_heads")
+    q_rows, k_rows, v_rows = _rows(q), _rows(k), _rows(v)
+    if q_rows is None or k_rows is None or k_rows != v_rows:
+        raise ValueError("qkv_stride")
     if causal_block < 0:
-        return "causal_block"
+        raise ValueError("causal_block")
     for lengths in (q_lengths, kv_lengths):
-        if lengths is not None and (lengths.shape != (q.shape[0],) or lengths.dtype != torch.int32
-                                    or lengths.device != q.device or not lengths.is_contiguous()):
-            return "lengths: int32 [B] on the device of q"
-    return None
+        if lengths is not None and (lengths.shape != (B,) or lengths.dtype != torch.int32
+                                    or lengths.device != device or not lengths.is_contiguous()):
+            raise ValueError("lengths: int32 [B] on the device of q")
+    scale = 128 ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError("softmax_scale")
+    return q_rows, k_rows, scale
 
 
-def _workspace(name: str, device: torch.device, *sizes: int) -> torch.Tensor:
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(name: str, device_index: int, *sizes: int) -> int:
     n = ctypes.c_int64(0)
-    _lib.call(name, *sizes, ctypes.addressof(n))
-    return torch.empty((n.value,), device=device, dtype=torch.uint8)
+    with torch.cuda.device(device_index):
+        _lib.call(name, *sizes, ctypes.addressof(n))
+    return n.value
 
 
 def attention_with_lse(
@@ -1125,23 +1157,20 @@ def attention_with_lse(
     No reference counterpart: the reference infers with dense bidirectional attention only.
     """
     kv_heads = heads if kv_heads is None else kv_heads
-    reason = _masked_attention_reason(q, k, v, heads, kv_heads, causal_block, q_lengths, kv_lengths)
-    if reason is not None:
-        raise ValueError(reason)
-    B, L, _ = q.shape
-    scale = float(softmax_scale) if softmax_scale is not None else 128 ** -0.5
+    q_rows, k_rows, scale = _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block, q_lengths,
+                                                   kv_lengths)
+    B, L, C = q.shape
     if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
-    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device or not _rows_ok(out, written=True):
-        raise ValueError("out_shape: out must be bf16 [B, L, heads*128] with unit column stride")
-    lse = torch.empty((B, heads, L), device=q.device, dtype=torch.float32)
-    with torch.cuda.device(q.device):
-        _lib.call(
-            "ogx_attention_fwd_lse",
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), B, L, k.shape[1], heads, kv_heads, 128,
-            *_row_strides(q), *_row_strides(k), scale, int(causal_block), _ptr(q_lengths), _ptr(kv_lengths),
-            out.data_ptr(), *_row_strides(out), lse.data_ptr(), _stream(q),
-        )
+        out = q.new_empty((B, L, C))
+        out_rows = (L * C, C)
+    else:
+        out_rows = _given_rows(out, q, "out_shape: out must be bf16 [B, L, heads*128] with unit column stride")
+    lse = q.new_empty((B, heads, L), dtype=torch.float32)
+    _call_on(
+        q.device, "ogx_attention_fwd_lse", q.data_ptr(), k.data_ptr(), v.data_ptr(), B, L, k.shape[1], heads, kv_heads,
+        128, *q_rows, *k_rows, scale, causal_block, _ptr(q_lengths), _ptr(kv_lengths), out.data_ptr(), *out_rows,
+        lse.data_ptr(),
+    )
     return out, lse
 
 
@@ -1171,36 +1200,32 @@ def attention_backward(
     share their strides.  No reference counterpart (the reference only infers).
     """
     kv_heads = heads if kv_heads is None else kv_heads
-    reason = _masked_attention_reason(q, k, v, heads, kv_heads, causal_block, q_lengths, kv_lengths)
-    if reason is not None:
-        raise ValueError(reason)
-    B, L, _ = q.shape
-    for t in (dout, out):
-        if t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != q.device or not _rows_ok(t):
-            raise ValueError("dout_or_out: bf16 of q's shape with unit column stride")
-    if lse.shape != (B, heads, L) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+    q_rows, k_rows, scale = _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block, q_lengths,
+                                                   kv_lengths)
+    device = q.device
+    B, L, C = q.shape
+    _, M, Ck = k.shape
+    reason = "dout_or_out: bf16 of q's shape with unit column stride"
+    dout_rows, out_rows = (_given_rows(t, q, reason, written=False) for t in (dout, out))
+    if lse.shape != (B, heads, L) or lse.dtype != torch.float32 or lse.device != device or not lse.is_contiguous():
         raise ValueError("lse: fp32 [B, heads, L] as attention_with_lse returns it")
-    scale = float(softmax_scale) if softmax_scale is not None else 128 ** -0.5
     if grads is None:
-        dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=torch.bfloat16) for t in (q, k, v))
+        dq, dk, dv = q.new_empty((B, L, C)), q.new_empty((B, M, Ck)), q.new_empty((B, M, Ck))
+        dq_rows, dk_rows = (L * C, C), (M * Ck, Ck)
     else:
         dq, dk, dv = grads
-        for t, like in ((dq, q), (dk, k), (dv, v)):
-            if (t.shape != like.shape or t.dtype != torch.bfloat16 or t.device != q.device
-                    or not _rows_ok(t, written=True)):
-                raise ValueError("grads: bf16 tensors of the shapes of q, k and v with unit column stride")
-        if _row_strides(dk) != _row_strides(dv):
-            raise ValueError("grads: dk and dv share their strides")
-    with torch.cuda.device(q.device):
-        workspace = _workspace("ogx_attention_bwd_workspace", q.device, B, L, k.shape[1], heads, kv_heads)
-        _lib.call(
-            "ogx_attention_bwd",
-            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-            B, L, k.shape[1], heads, kv_heads, 128, *_row_strides(dout), *_row_strides(q), *_row_strides(k),
-            *_row_strides(out), scale, int(causal_block), _ptr(q_lengths), _ptr(kv_lengths),
-            workspace.data_ptr(), workspace.numel(), dq.data_ptr(), *_row_strides(dq), dk.data_ptr(), dv.data_ptr(),
-            *_row_strides(dk), _stream(q),
-        )
+        reason = "grads: bf16 tensors of the shapes of q, k and v with unit column stride, dk and dv sharing theirs"
+        dq_rows, dk_rows = _given_rows(dq, q, reason), _given_rows(dk, k, reason)
+        if _given_rows(dv, v, reason) != dk_rows:
+            raise ValueError(reason)
+    workspace = q.new_empty(
+        (_workspace_bytes("ogx_attention_bwd_workspace", device.index, B, L, M, heads, kv_heads),), dtype=torch.uint8)
+    _call_on(
+        device, "ogx_attention_bwd", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+        lse.data_ptr(), B, L, M, heads, kv_heads, 128, *dout_rows, *q_rows, *k_rows, *out_rows, scale, causal_block,
+        _ptr(q_lengths), _ptr(kv_lengths), workspace.data_ptr(), workspace.numel(), dq.data_ptr(), *dq_rows,
+        dk.data_ptr(), dv.data_ptr(), *dk_rows,
+    )
     return dq, dk, dv
 
 
@@ -1209,50 +1234,57 @@ _NORMS = {"none": NORM_NONE, "head": NORM_HEAD, "row": NORM_ROW}
 
 
 def _qk_norm_rope_args(q, k, q_weight, k_weight, cos, sin, heads, kv_heads, norm):
-    """Checks of ``fused_qk_norm_rope`` and the rotation's (rotary, batch, head, token strides)."""
+    """Checks of ``fused_qk_norm_rope``; (head dim, rotary columns, q's strides, k's strides, the tables' batch, head
+    and token strides)."""
     if norm not in _NORMS:
         raise ValueError("norm: 'head', 'row' or 'none'")
-    for t in (q, k):
-        if not t.is_cuda or t.device != q.device or t.dtype != torch.bfloat16:
-            raise ValueError("qk_device_or_dtype")
-    if q.ndim != 3 or k.ndim != 3 or q.shape[:2] != k.shape[:2]:
+    device = q.device
+    if device.type != "cuda" or k.device != device or q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16:
+        raise ValueError("qk_device_or_dtype")
+    if q.ndim != 3 or k.ndim != 3:
         raise ValueError("qk_shape")
-    B, L, _ = q.shape
+    B, L, C = q.shape
+    Bk, M, Ck = k.shape
+    if Bk != B or M != L:
+        raise ValueError("qk_shape")
     if L < 1 or B < 1:
         raise ValueError("empty_tokens")
-    if heads < 1 or kv_heads < 1 or q.shape[2] % heads or q.shape[2] // heads not in (64, 128):
+    if heads < 1 or kv_heads < 1 or C not in (heads * 64, heads * 128):
         raise ValueError("head_dim")
-    hd = q.shape[2] // heads
-    if k.shape[2] != kv_heads * hd or heads + kv_heads > 128:
+    hd = C // heads
+    if Ck != kv_heads * hd or heads + kv_heads > 128:
         raise ValueError("qk_shape")
-    if not (_rows_ok(q) and _rows_ok(k)):
+    q_rows, k_rows = _rows(q), _rows(k)
+    if q_rows is None or k_rows is None:
         raise ValueError("qk_noncontiguous")
     if norm == "none":
         if q_weight is not None or k_weight is not None:
             raise ValueError("qk_weight_shape")
     else:
-        want = (hd, hd) if norm == "head" else (heads * hd, kv_heads * hd)
+        want = (hd, hd) if norm == "head" else (C, Ck)
         if q_weight is None or k_weight is None or q_weight.shape != want[:1] or k_weight.shape != want[1:]:
             raise ValueError("qk_weight_shape")
-        for w in (q_weight, k_weight):
-            if w.device != q.device or w.dtype not in (torch.bfloat16, torch.float32) or w.dtype != q_weight.dtype:
-                raise ValueError("qk_weight_shape")
-    if cos.ndim not in (3, 4) or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.stride() != sin.stride():
+        dtype = q_weight.dtype
+        if (q_weight.device != device or k_weight.device != device or k_weight.dtype != dtype
+                or dtype not in (torch.bfloat16, torch.float32)):
+            raise ValueError("qk_weight_shape")
+    shape, strides = cos.shape, cos.stride()
+    if cos.ndim not in (3, 4) or sin.shape != shape or sin.dtype != cos.dtype or sin.stride() != strides:
         raise ValueError("rope_shape")
-    if cos.dtype not in (torch.bfloat16, torch.float32) or cos.device != q.device or sin.device != q.device:
+    if cos.dtype not in (torch.bfloat16, torch.float32) or cos.device != device or sin.device != device:
         raise ValueError("rope_shape")
-    half = cos.shape[-1]
-    if cos.shape[0] not in (1, B) or cos.shape[-2] != L or half % 8 or not 8 <= half <= hd // 2:
+    half = shape[-1]
+    if shape[0] not in (1, B) or shape[-2] != L or half % 8 or not 8 <= half <= hd // 2:
         raise ValueError("rope_shape")
-    if cos.ndim == 4 and (cos.shape[1] != heads or heads != kv_heads):
+    if cos.ndim == 4 and (shape[1] != heads or heads != kv_heads):
         raise ValueError("rope_shape")
-    stride_b = cos.stride(0) if cos.shape[0] > 1 else 0
-    stride_h = cos.stride(1) if cos.ndim == 4 and heads > 1 else 0
-    stride_t = cos.stride(-2) if L > 1 else half
-    if (cos.stride(-1) != 1 or stride_b % 8 or stride_h % 8 or stride_t % 8 or cos.data_ptr() % 16
+    stride_b = strides[0] if shape[0] > 1 else 0
+    stride_h = strides[1] if cos.ndim == 4 and heads > 1 else 0
+    stride_t = strides[-2] if L > 1 else half
+    if (strides[-1] != 1 or stride_b % 8 or stride_h % 8 or stride_t % 8 or cos.data_ptr() % 16
             or sin.data_ptr() % 16):
         raise ValueError("rope_shape")
-    return hd, 2 * half, stride_b, stride_h, stride_t
+    return hd, 2 * half, q_rows, k_rows, (stride_b, stride_h, stride_t)
 
 
 def _contiguous16(w: torch.Tensor | None) -> torch.Tensor | None:
@@ -1290,25 +1322,21 @@ def fused_qk_norm_rope(
     128, B = 1; ``fused_qk_norm_rope_backward`` gives the gradients of all of them.
     """
     kv_heads = heads if kv_heads is None else kv_heads
-    hd, rotary, cs_b, cs_h, cs_t = _qk_norm_rope_args(q, k, q_weight, k_weight, cos, sin, heads, kv_heads, norm)
+    hd, rotary, q_rows, k_rows, cs_strides = _qk_norm_rope_args(q, k, q_weight, k_weight, cos, sin, heads, kv_heads, norm)
+    B, L, C = q.shape
     if out is None:
-        q_out, k_out = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+        q_out, k_out = q.new_empty((B, L, C)), k.new_empty(k.shape)
+        q_out_rows, k_out_rows = (L * C, C), (L * kv_heads * hd, kv_heads * hd)
     else:
         q_out, k_out = out
-        for t, like in ((q_out, q), (k_out, k)):
-            if (t.shape != like.shape or t.dtype != torch.bfloat16 or t.device != q.device
-                    or not _rows_ok(t, written=True)):
-                raise ValueError("qk_out_shape")
+        q_out_rows, k_out_rows = _given_rows(q_out, q, "qk_out_shape"), _given_rows(k_out, k, "qk_out_shape")
     q_weight, k_weight = _contiguous16(q_weight), _contiguous16(k_weight)
-    with torch.cuda.device(q.device):
-        _lib.call(
-            "ogx_qk_norm_rope",
-            q.data_ptr(), k.data_ptr(), q.shape[0], q.shape[1], heads, kv_heads, hd, *_row_strides(q),
-            *_row_strides(k), _ptr(q_weight), _ptr(k_weight), DTYPE_F32 if q_weight is None else _code(q_weight),
-            _NORMS[norm], float(eps), cos.data_ptr(), sin.data_ptr(), _code(cos), rotary, int(interleaved),
-            cs_b, cs_h, cs_t, q_out.data_ptr(), *_row_strides(q_out), k_out.data_ptr(), *_row_strides(k_out),
-            _stream(q),
-        )
+    _call_on(
+        q.device, "ogx_qk_norm_rope", q.data_ptr(), k.data_ptr(), B, L, heads, kv_heads, hd, *q_rows, *k_rows,
+        _ptr(q_weight), _ptr(k_weight), DTYPE_F32 if q_weight is None else _code(q_weight), _NORMS[norm], eps,
+        cos.data_ptr(), sin.data_ptr(), _code(cos), rotary, interleaved, *cs_strides, q_out.data_ptr(), *q_out_rows,
+        k_out.data_ptr(), *k_out_rows,
+    )
     return q_out, k_out
 
 
@@ -1337,34 +1365,32 @@ def fused_qk_norm_rope_backward(
     sums run in a fixed order.  No reference counterpart (the reference only infers).
     """
     kv_heads = heads if kv_heads is None else kv_heads
-    hd, rotary, cs_b, cs_h, cs_t = _qk_norm_rope_args(q, k, q_weight, k_weight, cos, sin, heads, kv_heads, norm)
-    for t, like in ((dq_out, q), (dk_out, k)):
-        if t.shape != like.shape or t.dtype != torch.bfloat16 or t.device != q.device or not _rows_ok(t):
-            raise ValueError("output_gradients: bf16 of the shapes of q and k with unit column stride")
+    hd, rotary, q_rows, k_rows, cs_strides = _qk_norm_rope_args(q, k, q_weight, k_weight, cos, sin, heads, kv_heads, norm)
+    B, L, C = q.shape
+    Ck = kv_heads * hd
+    reason = "output_gradients: bf16 of the shapes of q and k with unit column stride"
+    dq_out_rows = _given_rows(dq_out, q, reason, written=False)
+    dk_out_rows = _given_rows(dk_out, k, reason, written=False)
     if out is None:
-        dq, dk = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+        dq, dk = q.new_empty((B, L, C)), k.new_empty((B, L, Ck))
+        dq_rows, dk_rows = (L * C, C), (L * Ck, Ck)
     else:
         dq, dk = out
-        for t, like in ((dq, q), (dk, k)):
-            if (t.shape != like.shape or t.dtype != torch.bfloat16 or t.device != q.device
-                    or not _rows_ok(t, written=True)):
-                raise ValueError("qk_out_shape")
+        dq_rows, dk_rows = _given_rows(dq, q, "qk_out_shape"), _given_rows(dk, k, "qk_out_shape")
     q_weight, k_weight = _contiguous16(q_weight), _contiguous16(k_weight)
     dqw = dkw = workspace = None
-    with torch.cuda.device(q.device):
-        if norm != "none":
-            dqw, dkw = (torch.empty(w.shape, device=q.device, dtype=torch.float32) for w in (q_weight, k_weight))
-            workspace = _workspace("ogx_qk_norm_rope_bwd_workspace", q.device, q.shape[0], q.shape[1], heads, kv_heads,
-                                   hd, _NORMS[norm])
-        _lib.call(
-            "ogx_qk_norm_rope_bwd",
-            dq_out.data_ptr(), *_row_strides(dq_out), dk_out.data_ptr(), *_row_strides(dk_out), q.data_ptr(),
-            k.data_ptr(), q.shape[0], q.shape[1], heads, kv_heads, hd, *_row_strides(q), *_row_strides(k),
-            _ptr(q_weight), _ptr(k_weight), DTYPE_F32 if q_weight is None else _code(q_weight), _NORMS[norm],
-            float(eps), cos.data_ptr(), sin.data_ptr(), _code(cos), rotary, int(interleaved), cs_b, cs_h, cs_t,
-            dq.data_ptr(), *_row_strides(dq), dk.data_ptr(), *_row_strides(dk), _ptr(dqw), _ptr(dkw), _ptr(workspace),
-            0 if workspace is None else workspace.numel(), _stream(q),
-        )
+    size = 0
+    if norm != "none":
+        dqw, dkw = (w.new_empty(w.shape, dtype=torch.float32) for w in (q_weight, k_weight))
+        size = _workspace_bytes("ogx_qk_norm_rope_bwd_workspace", q.device.index, B, L, heads, kv_heads, hd, _NORMS[norm])
+        workspace = q.new_empty((size,), dtype=torch.uint8)
+    _call_on(
+        q.device, "ogx_qk_norm_rope_bwd", dq_out.data_ptr(), *dq_out_rows, dk_out.data_ptr(), *dk_out_rows,
+        q.data_ptr(), k.data_ptr(), B, L, heads, kv_heads, hd, *q_rows, *k_rows, _ptr(q_weight), _ptr(k_weight),
+        DTYPE_F32 if q_weight is None else _code(q_weight), _NORMS[norm], eps, cos.data_ptr(), sin.data_ptr(),
+        _code(cos), rotary, interleaved, *cs_strides, dq.data_ptr(), *dq_rows, dk.data_ptr(), *dk_rows, _ptr(dqw),
+        _ptr(dkw), _ptr(workspace), size,
+    )
     return dq, dk, dqw, dkw
 
 
