@@ -29,6 +29,7 @@ constexpr int BWD_SMEM_DKDV = (2 + 2 * B_STAGES) * T_BYTES + B_STAGES * STAT_BYT
 constexpr int BWD_SMEM_DQ = (2 + B_STAGES + DQ_K_STAGES) * T_BYTES;
 constexpr int BWD_SMEM = (BWD_SMEM_DKDV > BWD_SMEM_DQ ? BWD_SMEM_DKDV : BWD_SMEM_DQ) + 1024;
 constexpr int kBwdThreads = 384;               // TMA, MMA, row-zeroing and one idle warp; two softmax groups
+constexpr int kSoftmaxWarps = 8;
 
 struct BwdParams {
   int L, L_kv;
@@ -82,38 +83,84 @@ __device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a, uint32_t b, 
                (accumulate || kk > 0) ? 1u : 0u);
 }
 
-// A row's 128 fp32 columns in tensor memory, or `columns` of them, times `scale`, as bf16 to global memory.
-__device__ __forceinline__ void store_row(uint32_t taddr, int columns, float scale, __nv_bfloat16* dst, bool valid) {
+// Exchanges the pieces of four lanes: lane q of each group of four gets piece q of all four, in the lanes' order.
+__device__ __forceinline__ void transpose4(uint4 (&v)[4], uint32_t lane) {
+#pragma unroll
+  for (uint32_t bit = 1; bit <= 2; bit *= 2) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      if (i & bit) continue;
+      uint4& lo = v[i];
+      uint4& hi = v[i + bit];
+      uint4 t = up ? lo : hi;
+      t.x = __shfl_xor_sync(0xffffffffu, t.x, bit);
+      t.y = __shfl_xor_sync(0xffffffffu, t.y, bit);
+      t.z = __shfl_xor_sync(0xffffffffu, t.z, bit);
+      t.w = __shfl_xor_sync(0xffffffffu, t.w, bit);
+      if (up)
+        lo = t;
+      else
+        hi = t;
+    }
+  }
+}
+
+// `columns` fp32 columns in tensor memory of a warp's 32 rows, times `scale`, as bf16 to rows `stride` elements
+// apart, the first `rows` of them.  A lane holds a row; storing it so would send 32 rows' 16-byte pieces with every
+// instruction (one cycle of the L1 for each: 3.3 us for dK and dV of a tile), so four lanes trade pieces and store
+// 64 bytes of a row together.
+__device__ __forceinline__ void store_rows(uint32_t taddr, int columns, float scale, __nv_bfloat16* dst, int64_t stride,
+                                           int rows, uint32_t lane) {
+  __nv_bfloat16* mine = dst + static_cast<int64_t>(lane & ~3u) * stride + (lane & 3u) * 8;
+  const int left = rows - static_cast<int>(lane & ~3u);  // of this lane's four rows
 #pragma unroll 1
   for (int oc = 0; oc < columns / 32; ++oc) {
     uint32_t r[32];
     tmem_ld32(taddr + oc * 32, r);
     tmem_ld_wait();
-    if (valid) {
+    uint4 piece[4];
 #pragma unroll
-      for (int v8 = 0; v8 < 4; ++v8) {
-        float f[8];
+    for (int v8 = 0; v8 < 4; ++v8) {
+      float f[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[v8 * 8 + i]) * scale;
-        *reinterpret_cast<uint4*>(dst + oc * 32 + v8 * 8) = pack8(f);
-      }
+      for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[v8 * 8 + i]) * scale;
+      piece[v8] = pack8(f);
     }
+    transpose4(piece, lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) *reinterpret_cast<uint4*>(mine + i * stride + oc * 32) = piece[i];
   }
+}
+
+// One arrival for the warp's tensor-memory accesses so far (32 would queue at the barrier).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, uint32_t lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
 }
 
 __device__ __forceinline__ void zero_row(__nv_bfloat16* dst, int columns) {
   for (int i = 0; i < columns / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
 }
 
-// 64 scores of a row to probabilities: exp2(score * c + offset), three quarters on the MUFU and one on the FMA pipe.
+// 64 scores of a row to probabilities: exp2(score * c + offset), three quarters on the MUFU and one on the FMA
+// pipe.  offset(i): the offsets of columns i .. i + 3.
 template <typename Offset>
 __device__ __forceinline__ void probabilities(float (&s)[64], float c, Offset offset) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const f2 a = fma2(f2{s[2 * i], s[2 * i + 1]}, f2{c, c}, offset(2 * i));
-    const f2 pr = ((kPolyChunkMask >> (i / 8)) & 1u) ? ex2_poly2(a) : f2{ex2(a.x), ex2(a.y)};
-    s[2 * i] = pr.x;
-    s[2 * i + 1] = pr.y;
+  for (int i = 0; i < 64; i += 4) {
+    const float4 o = offset(i);
+    const bool poly = (kPolyChunkMask >> (i / 16)) & 1u;
+    const f2 a = fma2(f2{s[i], s[i + 1]}, f2{c, c}, f2{o.x, o.y});
+    const f2 b = fma2(f2{s[i + 2], s[i + 3]}, f2{c, c}, f2{o.z, o.w});
+    const f2 pa = poly ? ex2_poly2(a) : f2{ex2(a.x), ex2(a.y)};
+    const f2 pb = poly ? ex2_poly2(b) : f2{ex2(b.x), ex2(b.y)};
+    s[i] = pa.x;
+    s[i + 1] = pa.y;
+    s[i + 2] = pb.x;
+    s[i + 3] = pb.y;
   }
 }
 
@@ -356,7 +403,7 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
       tmem_ld32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(&pr[0]));
       tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&pr[32]));
       tmem_ld_wait();
-      probabilities(pr, p.scale_log2, [&](int i) { return *reinterpret_cast<const f2*>(stat + i); });
+      probabilities(pr, p.scale_log2, [&](int i) { return *reinterpret_cast<const float4*>(stat + i); });
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 64; ++i)
@@ -370,8 +417,7 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
         tmem_st8(s_tmem + cc * 8, pk);
       }
       tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&st.p_full);
+      warp_arrive(&st.p_full, lane);
 
       if (!mbar_wait(&st.dp_full, j & 1, abort)) {
         ok = false;
@@ -405,15 +451,15 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
         }
       }
       tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&st.ds_full[0]);
+      warp_arrive(&st.ds_full[0], lane);
     }
     if (ok && mbar_wait(&st.done, 0, abort)) {
       tc_fence_after();
       __nv_bfloat16* base = g == 0 ? p.dv : p.dk;
-      store_row(tmem + lane_off + (g == 0 ? 256 : 384), HD, g == 0 ? 1.f : p.scale,
-                base + batch * p.dkv_stride_b + key * p.dkv_stride_t + static_cast<int64_t>(kv_head) * HD,
-                key < p.L_kv);
+      const int key0 = k0 + static_cast<int>(quarter * 32);
+      store_rows(tmem + lane_off + (g == 0 ? 256 : 384), HD, g == 0 ? 1.f : p.scale,
+                 base + batch * p.dkv_stride_b + key0 * p.dkv_stride_t + static_cast<int64_t>(kv_head) * HD,
+                 p.dkv_stride_t, p.L_kv - key0, lane);
     }
   }
 }
@@ -561,7 +607,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
       tmem_ld32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(&pr[0]));
       tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&pr[32]));
       tmem_ld_wait();
-      probabilities(pr, p.scale_log2, [&](int) { return f2{nl, nl}; });
+      probabilities(pr, p.scale_log2, [&](int) { return make_float4(nl, nl, nl, nl); });
       if (!mbar_wait(&st.dp_full, j & 1, abort)) {
         ok = false;
         break;
@@ -573,8 +619,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
         tmem_ld32(dp_tmem + half * 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
         tmem_ld_wait();
         if (half == 1) {
-          tc_fence_before();
-          mbar_arrive(&st.dp_read);
+          warp_arrive(&st.dp_read, lane);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -597,14 +642,14 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
         }
       }
       tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&st.ds_full[b]);
+      warp_arrive(&st.ds_full[b], lane);
     }
     if (ok && mbar_wait(&st.done, 0, abort)) {
       tc_fence_after();
-      store_row(tmem + lane_off + 384 + g * 64, 64, p.scale,
-                p.dq + batch * p.dq_stride_b + token * p.dq_stride_t + static_cast<int64_t>(head) * HD + g * 64,
-                token < p.L);
+      const int token0 = q0 + static_cast<int>(quarter * 32);
+      store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale,
+                 p.dq + batch * p.dq_stride_b + token0 * p.dq_stride_t + static_cast<int64_t>(head) * HD + g * 64,
+                 p.dq_stride_t, p.L - token0, lane);
     }
   }
 }
@@ -630,11 +675,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&st.s_full[b], 1);
-      mbar_init(&st.ds_full[b], 256);
+      mbar_init(&st.ds_full[b], kSoftmaxWarps);
     }
-    mbar_init(&st.p_full, 256);
+    mbar_init(&st.p_full, kSoftmaxWarps);
     mbar_init(&st.dp_full, 1);
-    mbar_init(&st.dp_read, 256);
+    mbar_init(&st.dp_read, kSoftmaxWarps);
     mbar_init(&st.zero_request, 1);
     mbar_init(&st.zeroed, 1);
     mbar_init(&st.done, 1);
