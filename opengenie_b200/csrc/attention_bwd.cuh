@@ -46,21 +46,15 @@ struct BwdParams {
 };
 
 struct BwdShared {
-  uint64_t fixed_full;                             // the operands a CTA keeps: K and V, or Q and dO
+  uint64_t fixed_full[2];                          // the operands a CTA keeps, for S and for dP: K and V, or Q and dO
   uint64_t a_full[DQ_K_STAGES], a_empty[DQ_K_STAGES];  // Q and statistics (dK/dV), K (dQ)
   uint64_t b_full[B_STAGES], b_empty[B_STAGES];        // dO (dK/dV), V (dQ)
   uint64_t zero_request, zeroed;  // the MMA issuer asks warp 2 to zero rows past the sequence's length; its answer
-  uint64_t s_full[2], p_full, dp_full, dp_read, ds_full[2];
-  uint64_t done;
+  uint64_t s_full[2], p_full[2], dp_full, dp_read, ds_full[2];  // p_full: dK/dV, by halves of the queries
+  uint64_t dv_done, done;
   uint32_t tmem_base;
   int abort;
 };
-
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
 
 // D[128 x 128] (+)= A B^T, both tiles in shared memory with the 128 columns of d as the summed axis.
 __device__ __forceinline__ void mma_tile_ss(uint32_t d, uint32_t a, uint32_t b) {
@@ -72,14 +66,14 @@ __device__ __forceinline__ void mma_tile_ss(uint32_t d, uint32_t a, uint32_t b) 
   }
 }
 
-// D[128 x 128] (+)= A B with A (bf16, 128 x 128) in tensor memory: each softmax group writes its 64 columns over
-// the start of the fp32 columns it has read, so columns [0, 64) lie at a and columns [64, 128) at a + 64.  B's
-// rows are the summed axis.
+// D[128 x 128] (+)= A B, steps [FIRST, LAST) of 16 of the summed axis: A (bf16, 128 x 128) in tensor memory, each
+// run of RUN columns packed over the start of the RUN fp32 columns it came from; B's rows are the summed axis.
+template <int RUN, int FIRST, int LAST>
 __device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
   constexpr uint32_t idesc = make_idesc(1, 1, 0, 1, BT, HD);
 #pragma unroll
-  for (int kk = 0; kk < BT / 16; ++kk)
-    mma_f16_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, make_sdesc_sw128(b + kk * 2048, T_HALF_BYTES, 1024), idesc,
+  for (int kk = FIRST; kk < LAST; ++kk)
+    mma_f16_ts(d, a + kk * 16 / RUN * RUN + kk * 16 % RUN / 2, make_sdesc_sw128(b + kk * 2048, T_HALF_BYTES, 1024), idesc,
                (accumulate || kk > 0) ? 1u : 0u);
 }
 
@@ -145,14 +139,14 @@ __device__ __forceinline__ void zero_row(__nv_bfloat16* dst, int columns) {
   for (int i = 0; i < columns / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
 }
 
-// 64 scores of a row to probabilities: exp2(score * c + offset), three quarters on the MUFU and one on the FMA
-// pipe.  offset(i): the offsets of columns i .. i + 3.
+// 32 scores of a row to probabilities: exp2(score * c + offset), three quarters on the MUFU and one on the FMA pipe.
+// offset(i): the offsets of columns i .. i + 3.
 template <typename Offset>
-__device__ __forceinline__ void probabilities(float (&s)[64], float c, Offset offset) {
+__device__ __forceinline__ void probabilities(float* s, float c, Offset offset) {
 #pragma unroll
-  for (int i = 0; i < 64; i += 4) {
+  for (int i = 0; i < 32; i += 4) {
     const float4 o = offset(i);
-    const bool poly = (kPolyChunkMask >> (i / 16)) & 1u;
+    const bool poly = i >= 24;
     const f2 a = fma2(f2{s[i], s[i + 1]}, f2{c, c}, f2{o.x, o.y});
     const f2 b = fma2(f2{s[i + 2], s[i + 3]}, f2{c, c}, f2{o.z, o.w});
     const f2 pa = poly ? ex2_poly2(a) : f2{ex2(a.x), ex2(a.y)};
@@ -164,9 +158,19 @@ __device__ __forceinline__ void probabilities(float (&s)[64], float c, Offset of
   }
 }
 
+// 32 values as bf16 over the start of the tensor-memory columns at taddr.
+__device__ __forceinline__ void store_packed(uint32_t taddr, const float* v) {
+  uint32_t pk[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  tmem_st16(taddr, pk);
+}
+
 // ------------------------------------------------------------------------------------------- row statistics
-// 16 lanes per (token, head) row.  Rows past the sequence's length and rows that saw no key get -lse = -inf, so
-// their probabilities are 0; the tiles' padding rows too.
+// 16 lanes per (token, head) row; a team of such groups takes the heads of 8 tokens, so that a group's statistics of a
+// head leave as two whole 32-byte sectors (4-byte pieces of 16 sectors took 40 us at 9216 x 32 rows, this 27).
+// Rows past the sequence's length, rows that saw no key and the tiles' padding rows get -lse = -inf, so their
+// probabilities are 0.
 struct StatsParams {
   const __nv_bfloat16 *dout, *out;
   int64_t dout_stride_b, dout_stride_t, out_stride_b, out_stride_t;
@@ -174,46 +178,60 @@ struct StatsParams {
   const int* q_lengths;
   float* stats;
   int L, heads, q_tiles;
-  int64_t rows;  // batch * q_tiles * 128 * heads
+  int team;  // groups per 8 tokens, a power of two
 };
+constexpr int kStatsTokens = 8;
 
-__global__ void __launch_bounds__(256) attn_bwd_stats_kernel(StatsParams p) {
+__global__ void __launch_bounds__(256, 4) attn_bwd_stats_kernel(StatsParams p) {
   pdl_trigger();
   pdl_wait();
   const int sub = threadIdx.x & 15;
-  // whole warps stay together: the reduction below names all 32 lanes
-  const int64_t per_block = blockDim.x / 16;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per_block; r0 < p.rows; r0 += gridDim.x * per_block) {
-    const int64_t r = r0 + threadIdx.x / 16;
-    const bool in = r < p.rows;
-    const int64_t rr = in ? r : 0;
-    const int head = static_cast<int>(rr % p.heads);
-    const int64_t bt = rr / p.heads;
-    const int padded = p.q_tiles * BT;
-    const int token = static_cast<int>(bt % padded);
-    const int batch = static_cast<int>(bt / padded);
-    const bool live = in && token < clamp_length(p.q_lengths, batch, p.L);
-    float d = 0.f;
-    if (live) {
-      float a[8], b[8];
-      unpack8(*reinterpret_cast<const uint4*>(p.dout + batch * p.dout_stride_b + token * p.dout_stride_t +
-                                              static_cast<int64_t>(head) * HD + sub * 8),
-              a);
-      unpack8(*reinterpret_cast<const uint4*>(p.out + batch * p.out_stride_b + token * p.out_stride_t +
-                                              static_cast<int64_t>(head) * HD + sub * 8),
-              b);
+  const int group = threadIdx.x >> 4;
+  const int member = group & (p.team - 1);
+  const int batch = blockIdx.y;
+  const int token0 = (static_cast<int>(blockIdx.x) * (16 / p.team) + group / p.team) * kStatsTokens;
+  if (token0 - group / p.team * kStatsTokens >= p.q_tiles * BT) return;  // the whole CTA lies past the last tile
+  const int live = clamp_length(p.q_lengths, batch, p.L);
+  const int mine = token0 + (sub & 7);  // the token whose statistics this lane writes: -lse (lanes 0-7), -delta (8-15)
+  const __nv_bfloat16* dout = p.dout + batch * p.dout_stride_b + sub * 8;
+  const __nv_bfloat16* out = p.out + batch * p.out_stride_b + sub * 8;
+  // whole warps run every iteration: the reduction names all lanes
+  for (int h0 = 0; h0 < p.heads; h0 += p.team) {
+    const int head = h0 + member;
+    const bool ok = head < p.heads;
+    const float lse = ok && mine < live ? p.lse[(static_cast<int64_t>(batch) * p.heads + head) * p.L + mine] : -INFINITY;
+    float delta = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d = fmaf(a[i], b[i], d);
+    for (int half = 0; half < 2; ++half) {
+      uint4 a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int token = token0 + half * 4 + i;
+        a[i] = b[i] = make_uint4(0, 0, 0, 0);
+        if (ok && token < live) {
+          a[i] = __ldcs(reinterpret_cast<const uint4*>(dout + token * p.dout_stride_t + head * HD));
+          b[i] = __ldcs(reinterpret_cast<const uint4*>(out + token * p.out_stride_t + head * HD));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x[8], y[8], d = 0.f;
+        unpack8(a[i], x);
+        unpack8(b[i], y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e], d);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if ((sub & 7) == half * 4 + i) delta = d;
+      }
     }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (in && sub == 0) {
-      const int64_t bh = static_cast<int64_t>(batch) * p.heads + head;
-      const float lse = live ? p.lse[bh * p.L + token] : -INFINITY;
+    if (ok && mine < p.q_tiles * BT) {
       const bool empty = lse == -INFINITY;
-      float* dst = p.stats + (bh * p.q_tiles + token / BT) * STAT_FLOATS + token % BT;
-      dst[0] = empty ? -INFINITY : -lse * 1.4426950408889634f;
-      dst[BT] = empty ? 0.f : -d;
+      float* dst = p.stats + ((static_cast<int64_t>(batch) * p.heads + head) * p.q_tiles + mine / BT) * STAT_FLOATS + mine % BT;
+      if (sub < 8)
+        dst[0] = empty ? -INFINITY : -lse * 1.4426950408889634f;
+      else
+        dst[BT] = empty ? 0.f : -delta;
     }
   }
 }
@@ -224,7 +242,8 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(StatsParams p) {
 //   TMEM: S^T [0,128), dP^T [128,256), dV [256,384), dK [384,512); bf16 P^T over S^T, dS^T over dP^T.
 // Per query tile the MMA issuer runs dV += P dO, S(next), dK += dS Q, dP(next): while the softmax groups turn S
 // into P the tensor pipe does the previous tile's dK and this tile's dP, and while they turn dP into dS it does
-// dV and the next S.
+// dV and the next S.  A group of four warps takes 32 query columns of the first half and 32 of the second, and P goes
+// to the MMA issuer half by half: the first half's dV runs while the second half is still exponentials.
 __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv,
                                          const CUtensorMap* tdo, const BwdParams& p, BwdShared& st, uint8_t* smem,
                                          uint32_t tmem) {
@@ -265,9 +284,8 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
   if (warp == 0) {
     if (elect_one()) {
       // ---------------------------------------------------------- TMA producer
-      mbar_arrive_expect_tx(&st.fixed_full, 2 * T_BYTES);
-      load_rows(k_tile, tk, &st.fixed_full, T_HALF_BYTES, kv_head, k0, batch);
-      load_rows(v_tile, tv, &st.fixed_full, T_HALF_BYTES, kv_head, k0, batch);
+      mbar_arrive_expect_tx(&st.fixed_full[0], T_BYTES);
+      load_rows(k_tile, tk, &st.fixed_full[0], T_HALF_BYTES, kv_head, k0, batch);
       int a_issued = 0, b_issued = 0;
       int head = kv_head * p.heads_per_kv, tile = first_tile;
       for (int j = 0; j < n; ++j) {
@@ -280,6 +298,10 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
                         p.stats + ((static_cast<int64_t>(batch) * p.heads + head) * p.q_tiles + tile) * STAT_FLOATS,
                         STAT_BYTES, &st.a_full[s]);
         ++a_issued;
+        if (j == 0) {  // behind what the first scores need
+          mbar_arrive_expect_tx(&st.fixed_full[1], T_BYTES);
+          load_rows(v_tile, tv, &st.fixed_full[1], T_HALF_BYTES, kv_head, k0, batch);
+        }
         if (!mbar_wait(&st.b_empty[s], ph ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.b_full[s], T_BYTES);
         load_rows(do_tiles + s * T_BYTES, tdo, &st.b_full[s], T_HALF_BYTES, head, tile * BT, batch);
@@ -290,7 +312,8 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
         }
       }
       if (*abort) {  // let the copies in flight land before the CTA exits
-        mbar_wait(&st.fixed_full, 0, nullptr);
+        mbar_wait(&st.fixed_full[0], 0, nullptr);
+        if (a_issued > 0) mbar_wait(&st.fixed_full[1], 0, nullptr);
         for (int j = a_issued - 1; j >= 0 && j >= a_issued - B_STAGES; --j)
           mbar_wait(&st.a_full[j % B_STAGES], (j / B_STAGES) & 1, nullptr);
         for (int j = b_issued - 1; j >= 0 && j >= b_issued - B_STAGES; --j)
@@ -324,26 +347,30 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
         mma_tile_ss(t_dp, v_addr, do_addr + (j % B_STAGES) * T_BYTES);
         mma_commit(&st.dp_full);
       };
-      bool ok = mbar_wait(&st.fixed_full, 0, abort) && q_ready(0);
+      bool ok = mbar_wait(&st.fixed_full[0], 0, abort) && q_ready(0);
       if (ok) issue_s(0);
-      ok = ok && mbar_wait(&st.b_full[0], 0, abort);
+      ok = ok && mbar_wait(&st.fixed_full[1], 0, abort) && mbar_wait(&st.b_full[0], 0, abort);
       if (ok) {
         tc_fence_after();
         issue_dp(0);
       }
       for (int j = 0; j < n && ok; ++j) {
         const int s = j % B_STAGES;
-        if (!mbar_wait(&st.p_full, j & 1, abort)) break;
+        if (!mbar_wait(&st.p_full[0], j & 1, abort)) break;
         tc_fence_after();
-        mma_tile_ts(t_dv, t_s, do_addr + s * T_BYTES, j > 0);
+        mma_tile_ts<32, 0, 4>(t_dv, t_s, do_addr + s * T_BYTES, j > 0);
+        if (!mbar_wait(&st.p_full[1], j & 1, abort)) break;
+        tc_fence_after();
+        mma_tile_ts<32, 4, 8>(t_dv, t_s, do_addr + s * T_BYTES, true);
         mma_commit(&st.b_empty[s]);
+        if (j + 1 == n) mma_commit(&st.dv_done);
         if (j + 1 < n) {
           if (!q_ready(j + 1)) break;
           issue_s(j + 1);
         }
         if (!mbar_wait(&st.ds_full[0], j & 1, abort)) break;
         tc_fence_after();
-        mma_tile_ts(t_dk, t_dp, q_addr + s * T_BYTES, j > 0);
+        mma_tile_ts<32, 0, 8>(t_dk, t_dp, q_addr + s * T_BYTES, j > 0);
         mma_commit(&st.a_empty[s]);
         if (j + 1 < n) {
           const int s1 = (j + 1) % B_STAGES;
@@ -373,11 +400,11 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax groups
-    const int g = static_cast<int>(warp - 4) >> 2;  // query columns [64g, 64g + 64)
+    const int g = static_cast<int>(warp - 4) >> 2;  // query columns [32g, 32g + 32) and 64 on
     const uint32_t quarter = warp & 3;
     const int key = k0 + static_cast<int>(quarter * 32 + lane);
     const uint32_t lane_off = (quarter * 32u) << 16;
-    const uint32_t s_tmem = tmem + lane_off + g * 64;
+    const uint32_t s_tmem = tmem + lane_off + g * 32;
     const uint32_t dp_tmem = s_tmem + 128;
     const bool key_ok = key < vis.kv_len;
     const int first = vis.first(key);
@@ -391,9 +418,9 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
       const int q0 = tile * BT;
       if (++tile == end_tile) tile = first_tile;
       const bool masked = ragged_keys || q0 < all_from || q0 + BT > vis.q_len;
-      const int lo = key_ok ? first - q0 - g * 64 : 64;
-      const int hi = vis.q_len - q0 - g * 64;
-      const float* stat = reinterpret_cast<const float*>(stat_tiles + s * STAT_BYTES) + g * 64;
+      const int lo = key_ok ? first - q0 - g * 32 : BT;  // columns from this thread's first that its key is seen by
+      const int hi = vis.q_len - q0 - g * 32;
+      const float* stat = reinterpret_cast<const float*>(stat_tiles + s * STAT_BYTES) + g * 32;
       if (!mbar_wait(&st.a_full[s], (j / B_STAGES) & 1, abort) || !mbar_wait(&st.s_full[0], j & 1, abort)) {
         ok = false;
         break;
@@ -401,23 +428,21 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
       tc_fence_after();
       float pr[64];
       tmem_ld32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(&pr[0]));
-      tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&pr[32]));
+      tmem_ld32(s_tmem + 64, *reinterpret_cast<uint32_t(*)[32]>(&pr[32]));
       tmem_ld_wait();
-      probabilities(pr, p.scale_log2, [&](int i) { return *reinterpret_cast<const float4*>(stat + i); });
-      if (masked) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (i < lo || i >= hi) pr[i] = 0.f;
+      for (int half = 0; half < 2; ++half) {
+        probabilities(pr + half * 32, p.scale_log2,
+                      [&](int i) { return *reinterpret_cast<const float4*>(stat + half * 64 + i); });
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (half * 64 + i < lo || half * 64 + i >= hi) pr[half * 32 + i] = 0.f;
+        }
+        store_packed(s_tmem + half * 64, pr + half * 32);
+        tmem_st_wait();
+        warp_arrive(&st.p_full[half], lane);
       }
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc) {
-        uint32_t pk[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pk[i] = pack_bf16x2(pr[cc * 16 + 2 * i], pr[cc * 16 + 2 * i + 1]);
-        tmem_st8(s_tmem + cc * 8, pk);
-      }
-      tmem_st_wait();
-      warp_arrive(&st.p_full, lane);
 
       if (!mbar_wait(&st.dp_full, j & 1, abort)) {
         ok = false;
@@ -427,39 +452,39 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         float dp[32];
-        tmem_ld32(dp_tmem + half * 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
+        tmem_ld32(dp_tmem + half * 64, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int col = half * 32 + 2 * i;
-          const f2 nd = *reinterpret_cast<const f2*>(stat + BT + col);
-          const f2 ds = mul2(f2{pr[col], pr[col + 1]}, add2(f2{dp[2 * i], dp[2 * i + 1]}, nd));
-          dp[2 * i] = ds.x;
-          dp[2 * i + 1] = ds.y;
+        for (int i = 0; i < 32; i += 4) {
+          const int c = half * 32 + i;
+          const float4 nd = *reinterpret_cast<const float4*>(stat + BT + half * 64 + i);
+          const f2 x = mul2(f2{pr[c], pr[c + 1]}, add2(f2{dp[i], dp[i + 1]}, f2{nd.x, nd.y}));
+          const f2 y = mul2(f2{pr[c + 2], pr[c + 3]}, add2(f2{dp[i + 2], dp[i + 3]}, f2{nd.z, nd.w}));
+          dp[i] = x.x;
+          dp[i + 1] = x.y;
+          dp[i + 2] = y.x;
+          dp[i + 3] = y.y;
         }
         if (masked) {  // dP of a masked pair may be anything
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (half * 32 + i < lo || half * 32 + i >= hi) dp[i] = 0.f;
+            if (half * 64 + i < lo || half * 64 + i >= hi) dp[i] = 0.f;
         }
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          uint32_t pk[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pk[i] = pack_bf16x2(dp[cc * 16 + 2 * i], dp[cc * 16 + 2 * i + 1]);
-          tmem_st8(dp_tmem + half * 16 + cc * 8, pk);
-        }
+        store_packed(dp_tmem + half * 64, dp);
       }
       tmem_st_wait();
       warp_arrive(&st.ds_full[0], lane);
     }
+    // each group stores half of the columns of both: dV while the last dK product runs, then dK
+    const int key0 = k0 + static_cast<int>(quarter * 32);
+    const int64_t at = batch * p.dkv_stride_b + key0 * p.dkv_stride_t + static_cast<int64_t>(kv_head) * HD + g * 64;
+    if (ok && mbar_wait(&st.dv_done, 0, abort)) {
+      tc_fence_after();
+      store_rows(tmem + lane_off + 256 + g * 64, 64, 1.f, p.dv + at, p.dkv_stride_t, p.L_kv - key0, lane);
+    }
     if (ok && mbar_wait(&st.done, 0, abort)) {
       tc_fence_after();
-      __nv_bfloat16* base = g == 0 ? p.dv : p.dk;
-      const int key0 = k0 + static_cast<int>(quarter * 32);
-      store_rows(tmem + lane_off + (g == 0 ? 256 : 384), HD, g == 0 ? 1.f : p.scale,
-                 base + batch * p.dkv_stride_b + key0 * p.dkv_stride_t + static_cast<int64_t>(kv_head) * HD,
-                 p.dkv_stride_t, p.L_kv - key0, lane);
+      store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale, p.dk + at, p.dkv_stride_t, p.L_kv - key0, lane);
     }
   }
 }
@@ -507,9 +532,8 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
   if (warp == 0) {
     if (elect_one()) {
       // ---------------------------------------------------------- TMA producer
-      mbar_arrive_expect_tx(&st.fixed_full, 2 * T_BYTES);
-      load_rows(q_tile, tq, &st.fixed_full, T_HALF_BYTES, head, q0, batch);
-      load_rows(do_tile, tdo, &st.fixed_full, T_HALF_BYTES, head, q0, batch);
+      mbar_arrive_expect_tx(&st.fixed_full[0], T_BYTES);
+      load_rows(q_tile, tq, &st.fixed_full[0], T_HALF_BYTES, head, q0, batch);
       int a_issued = 0, b_issued = 0;
       for (int j = 0; j < n; ++j) {
         const int sk = j % DQ_K_STAGES, sv = j % B_STAGES;
@@ -517,13 +541,18 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
         mbar_arrive_expect_tx(&st.a_full[sk], T_BYTES);
         load_rows(k_tiles + sk * T_BYTES, tk, &st.a_full[sk], T_HALF_BYTES, kv_head, j * BT, batch);
         ++a_issued;
+        if (j == 0) {  // behind what the first scores need
+          mbar_arrive_expect_tx(&st.fixed_full[1], T_BYTES);
+          load_rows(do_tile, tdo, &st.fixed_full[1], T_HALF_BYTES, head, q0, batch);
+        }
         if (!mbar_wait(&st.b_empty[sv], ((j / B_STAGES) & 1) ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.b_full[sv], T_BYTES);
         load_rows(v_tiles + sv * T_BYTES, tv, &st.b_full[sv], T_HALF_BYTES, kv_head, j * BT, batch);
         ++b_issued;
       }
       if (*abort) {  // let the copies in flight land before the CTA exits
-        mbar_wait(&st.fixed_full, 0, nullptr);
+        mbar_wait(&st.fixed_full[0], 0, nullptr);
+        if (a_issued > 0) mbar_wait(&st.fixed_full[1], 0, nullptr);
         for (int j = a_issued - 1; j >= 0 && j >= a_issued - DQ_K_STAGES; --j)
           mbar_wait(&st.a_full[j % DQ_K_STAGES], (j / DQ_K_STAGES) & 1, nullptr);
         for (int j = b_issued - 1; j >= 0 && j >= b_issued - B_STAGES; --j)
@@ -555,7 +584,8 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
         mma_commit(&st.b_empty[j % B_STAGES]);
         return true;
       };
-      bool ok = mbar_wait(&st.fixed_full, 0, abort) && issue_s(0) && issue_dp(0) && (n < 2 || issue_s(1));
+      bool ok = mbar_wait(&st.fixed_full[0], 0, abort) && issue_s(0) && mbar_wait(&st.fixed_full[1], 0, abort) &&
+                issue_dp(0) && (n < 2 || issue_s(1));
       for (int j = 0; j < n && ok; ++j) {
         if (j + 1 < n) {
           if (!mbar_wait(&st.dp_read, j & 1, abort)) break;
@@ -563,7 +593,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
         }
         if (!mbar_wait(&st.ds_full[j & 1], (j >> 1) & 1, abort)) break;
         tc_fence_after();
-        mma_tile_ts(t_dq, tmem + (j & 1) * 128, k_addr + (j % DQ_K_STAGES) * T_BYTES, j > 0);
+        mma_tile_ts<64, 0, 8>(t_dq, tmem + (j & 1) * 128, k_addr + (j % DQ_K_STAGES) * T_BYTES, j > 0);
         mma_commit(&st.a_empty[j % DQ_K_STAGES]);
         if (j + 2 < n && !issue_s(j + 2)) break;
       }
@@ -608,6 +638,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
       tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&pr[32]));
       tmem_ld_wait();
       probabilities(pr, p.scale_log2, [&](int) { return make_float4(nl, nl, nl, nl); });
+      probabilities(pr + 32, p.scale_log2, [&](int) { return make_float4(nl, nl, nl, nl); });
       if (!mbar_wait(&st.dp_full, j & 1, abort)) {
         ok = false;
         break;
@@ -633,13 +664,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
           for (int i = 0; i < 32; ++i)
             if (half * 32 + i >= valid) dp[i] = 0.f;
         }
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          uint32_t pk[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pk[i] = pack_bf16x2(dp[cc * 16 + 2 * i], dp[cc * 16 + 2 * i + 1]);
-          tmem_st8(s_tmem + half * 16 + cc * 8, pk);
-        }
+        store_packed(s_tmem + half * 16, dp);
       }
       tmem_st_wait();
       warp_arrive(&st.ds_full[b], lane);
@@ -664,7 +689,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t warp = warp_idx();
   if (threadIdx.x == 0) {
-    mbar_init(&st.fixed_full, 1);
     for (int s = 0; s < DQ_K_STAGES; ++s) {
       mbar_init(&st.a_full[s], 1);
       mbar_init(&st.a_empty[s], 1);
@@ -674,14 +698,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&st.b_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
+      mbar_init(&st.fixed_full[b], 1);
       mbar_init(&st.s_full[b], 1);
+      mbar_init(&st.p_full[b], kSoftmaxWarps);
       mbar_init(&st.ds_full[b], kSoftmaxWarps);
     }
-    mbar_init(&st.p_full, kSoftmaxWarps);
     mbar_init(&st.dp_full, 1);
     mbar_init(&st.dp_read, kSoftmaxWarps);
     mbar_init(&st.zero_request, 1);
     mbar_init(&st.zeroed, 1);
+    mbar_init(&st.dv_done, 1);
     mbar_init(&st.done, 1);
     st.abort = 0;
     fence_mbar_init();

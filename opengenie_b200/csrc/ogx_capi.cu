@@ -1473,7 +1473,8 @@ int masked_attention_guard(const void* q, const void* k, const void* v, int64_t 
   if (q_tokens > kMost || kv_tokens > kMost || heads > 65535 || batch > 65535) return fail(OGX_EINVAL, "shape");
   if (heads % kv_heads) return fail(OGX_EINVAL, "kv_heads: heads must be a multiple of kv_heads");
   if (causal_block < 0 || causal_block > kMost) return fail(OGX_EINVAL, "causal_block");
-  if (!(softmax_scale > 0.f) || softmax_scale > 3.0e38f) return fail(OGX_EINVAL, "softmax_scale");
+  // both ends stay far inside fp32
+  if (!(softmax_scale >= 1e-30f) || softmax_scale > 1e30f) return fail(OGX_EINVAL, "softmax_scale");
   if (!row_strides_ok(heads * 128, q_tokens, batch, q_stride_t, q_stride_b) ||
       !row_strides_ok(kv_heads * 128, kv_tokens, batch, kv_stride_t, kv_stride_b))
     return fail(OGX_EINVAL, "stride");
@@ -1585,8 +1586,13 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   sp.L = static_cast<int>(q_tokens);
   sp.heads = static_cast<int>(heads);
   sp.q_tiles = static_cast<int>(q_tiles);
-  sp.rows = batch * q_tiles * ogx::attn::BT * heads;
-  launch(ogx::attn::attn_bwd_stats_kernel, dim3(static_cast<unsigned>(grid_for(sp.rows * 16))), 256, 0, s, sp);
+  sp.team = 1;
+  while (sp.team < heads && sp.team < 16) sp.team *= 2;
+  const int64_t stats_tokens = ogx::attn::kStatsTokens * (16 / sp.team);
+  launch(ogx::attn::attn_bwd_stats_kernel,
+         dim3(static_cast<unsigned>((q_tiles * ogx::attn::BT + stats_tokens - 1) / stats_tokens),
+              static_cast<unsigned>(batch)),
+         256, 0, s, sp);
   if ((rc = check_launch("attn_bwd_stats_kernel"))) return rc;
 
   ogx::attn::BwdParams p{};

@@ -1117,7 +1117,7 @@ def _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block
                                     or lengths.device != device or not lengths.is_contiguous()):
             raise ValueError("lengths: int32 [B] on the device of q")
     scale = 128 ** -0.5 if softmax_scale is None else float(softmax_scale)
-    if not 0.0 < scale < 3e38:
+    if not 1e-30 <= scale <= 1e30:
         raise ValueError("softmax_scale")
     return q_rows, k_rows, scale
 
