@@ -154,10 +154,14 @@ def test_single_visible_key_gives_its_value_and_no_score_gradient(ops):
 
 
 @pytest.mark.parametrize("L,M", [(300, 300), (77, 1024), (1, 1)])
-def test_without_masks_the_output_is_the_dense_attention_bit_for_bit(ops, L, M):
-    q, k, v, _ = _case(2, L, M, 4, 4, seed=L)
+def test_without_masks_the_output_is_the_dense_attention(ops, L, M):
+    """The dense kernel's exponentials differ by its polynomial alone (within H / 8 of the same terms), so each is
+    within the forward tolerance of the formula and they are within both of each other; most elements are equal."""
+    q, k, v, dout = _case(2, L, M, 4, 4, seed=L)
     out, _ = ops.attention_with_lse(q, k, v, 4)
-    assert torch.equal(out, ops.attention(q, k, v, 4))
+    dense = ops.attention(q, k, v, 4)
+    _, tol, _ = _formulas(q, k, v, dout, 4, 4, _see(2, L, M, 0, None, None))
+    assert ((out.double() - dense.double()).abs() <= 2 * tol).all()
 
 
 @pytest.mark.parametrize("scale", [0.05, 4.0])
