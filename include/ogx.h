@@ -371,8 +371,8 @@ int ogx_attention_fwd_e4m3_to_peers(const void* q, const void* k, const void* v,
  * -inf.  Keys and values past kv_lengths may hold anything (NaN included). */
 int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
                           int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
-                          int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t, float softmax_scale,
-                          int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
+                          int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b,
+                          int64_t v_stride_t, float softmax_scale, int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
                           int64_t out_stride_b, int64_t out_stride_t, float* lse, void* stream);
 
 /* Bytes of device workspace that ogx_attention_bwd needs for these sizes. */
@@ -380,19 +380,20 @@ int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_toke
                                 int64_t* bytes);
 
 /* Gradients of ogx_attention_fwd_lse: from dout (the gradient of out), the forward's inputs, out and lse, dq
- * [batch, q_tokens, heads*128] and dk, dv [batch, kv_tokens, kv_heads*128] (bf16, own strides, dk and dv
- * sharing theirs), every element written.  The probabilities are recomputed from lse.  Rows past q_lengths and
+ * [batch, q_tokens, heads*128] and dk, dv [batch, kv_tokens, kv_heads*128] (bf16, own strides), every element
+ * written.  The probabilities are recomputed from lse.  Rows past q_lengths and
  * rows that see no key get dq = 0 and give nothing to dk and dv (their q and dout may hold anything); keys past
  * kv_lengths get dk = dv = 0.  workspace: device memory, 16-byte aligned, overwritten; calls that may run at the
  * same time need one each. */
 int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
                       const float* lse, int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
                       int64_t kv_heads, int64_t head_dim, int64_t dout_stride_b, int64_t dout_stride_t,
-                      int64_t q_stride_b, int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t,
-                      int64_t out_stride_b, int64_t out_stride_t, float softmax_scale, int64_t causal_block,
-                      const int* q_lengths, const int* kv_lengths, void* workspace, int64_t workspace_bytes, void* dq,
-                      int64_t dq_stride_b, int64_t dq_stride_t, void* dk, void* dv, int64_t dkv_stride_b,
-                      int64_t dkv_stride_t, void* stream);
+                      int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
+                      int64_t v_stride_b, int64_t v_stride_t, int64_t out_stride_b, int64_t out_stride_t, float softmax_scale,
+                      int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* workspace,
+                      int64_t workspace_bytes, void* dq, int64_t dq_stride_b, int64_t dq_stride_t, void* dk,
+                      int64_t dk_stride_b, int64_t dk_stride_t, void* dv, int64_t dv_stride_b, int64_t dv_stride_t,
+                      void* stream);
 
 /* What the RMSNorm of ogx_qk_norm_rope runs over. */
 #define OGX_NORM_NONE 0 /* no norm: the rotation alone */

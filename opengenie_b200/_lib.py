@@ -136,16 +136,17 @@ _SIGNATURES: dict[str, list] = {
     ],
     "ogx_attention_fwd_lse": [
         c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
-        c_int64, c_int64, c_float, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+        c_int64, c_int64, c_int64, c_int64, c_float, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+        c_void_p, c_void_p,
     ],
     "ogx_attention_bwd_workspace": [
         c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
     ],
     "ogx_attention_bwd": [
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
-        c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
-        c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
-        c_int64, c_int64, c_void_p,
+        c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+        c_int64, c_float, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+        c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
     ],
     "ogx_qk_norm_rope": [
         c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,

@@ -21,7 +21,7 @@ from collections import Counter
 
 import torch
 
-from . import ltx_ops
+from . import ltx_ops, training
 
 # The reference's choices plus the B200-native backend.
 ATTENTION_CHOICES = (
@@ -60,6 +60,8 @@ class B200NativeAttention:
     def __call__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, mask=None) -> torch.Tensor:
         if mask is not None:
             raise ValueError("mask: the b200-native backend is dense bidirectional attention")
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return training.attention(q, k, v, heads)
         return ltx_ops.attention(q, k, v, heads)
 
 

@@ -42,7 +42,7 @@ struct BwdParams {
   const int* kv_lengths;
   const float* stats;  // [batch][heads][q_tiles][2][128]
   __nv_bfloat16 *dq, *dk, *dv;
-  int64_t dq_stride_b, dq_stride_t, dkv_stride_b, dkv_stride_t;
+  int64_t dq_stride_b, dq_stride_t, dk_stride_b, dk_stride_t, dv_stride_b, dv_stride_t;
 };
 
 struct BwdShared {
@@ -274,9 +274,11 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
   if (n == 0) {
     if (warp >= 4) {
       const int key = k0 + static_cast<int>((warp & 3) * 32 + lane);
-      __nv_bfloat16* base = warp < 8 ? p.dv : p.dk;
+      const int64_t column = static_cast<int64_t>(kv_head) * HD;
       if (key < p.L_kv)
-        zero_row(base + batch * p.dkv_stride_b + key * p.dkv_stride_t + static_cast<int64_t>(kv_head) * HD, HD);
+        zero_row(warp < 8 ? p.dv + batch * p.dv_stride_b + key * p.dv_stride_t + column
+                          : p.dk + batch * p.dk_stride_b + key * p.dk_stride_t + column,
+                 HD);
     }
     return;
   }
@@ -477,14 +479,16 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
     }
     // each group stores half of the columns of both: dV while the last dK product runs, then dK
     const int key0 = k0 + static_cast<int>(quarter * 32);
-    const int64_t at = batch * p.dkv_stride_b + key0 * p.dkv_stride_t + static_cast<int64_t>(kv_head) * HD + g * 64;
+    const int column = kv_head * HD + g * 64;
     if (ok && mbar_wait(&st.dv_done, 0, abort)) {
       tc_fence_after();
-      store_rows(tmem + lane_off + 256 + g * 64, 64, 1.f, p.dv + at, p.dkv_stride_t, p.L_kv - key0, lane);
+      store_rows(tmem + lane_off + 256 + g * 64, 64, 1.f, p.dv + batch * p.dv_stride_b + key0 * p.dv_stride_t + column,
+                 p.dv_stride_t, p.L_kv - key0, lane);
     }
     if (ok && mbar_wait(&st.done, 0, abort)) {
       tc_fence_after();
-      store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale, p.dk + at, p.dkv_stride_t, p.L_kv - key0, lane);
+      store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale,
+                 p.dk + batch * p.dk_stride_b + key0 * p.dk_stride_t + column, p.dk_stride_t, p.L_kv - key0, lane);
     }
   }
 }

@@ -1463,8 +1463,8 @@ bool row_strides_ok(int64_t width, int64_t tokens, int64_t batch, int64_t stride
 
 int masked_attention_guard(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
                            int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
-                           int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t, float softmax_scale,
-                           int64_t causal_block) {
+                           int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b, int64_t v_stride_t,
+                           float softmax_scale, int64_t causal_block) {
   if (q == nullptr || k == nullptr || v == nullptr) return fail(OGX_EINVAL, "null_pointer");
   if (head_dim != 128) return fail(OGX_EINVAL, "head_dim: only 128 is supported");
   if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1 || kv_heads < 1) return fail(OGX_EINVAL, "shape");
@@ -1476,7 +1476,8 @@ int masked_attention_guard(const void* q, const void* k, const void* v, int64_t 
   // both ends stay far inside fp32
   if (!(softmax_scale >= 1e-30f) || softmax_scale > 1e30f) return fail(OGX_EINVAL, "softmax_scale");
   if (!row_strides_ok(heads * 128, q_tokens, batch, q_stride_t, q_stride_b) ||
-      !row_strides_ok(kv_heads * 128, kv_tokens, batch, kv_stride_t, kv_stride_b))
+      !row_strides_ok(kv_heads * 128, kv_tokens, batch, k_stride_t, k_stride_b) ||
+      !row_strides_ok(kv_heads * 128, kv_tokens, batch, v_stride_t, v_stride_b))
     return fail(OGX_EINVAL, "stride");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return fail(OGX_EINVAL, "alignment");
   return OGX_OK;
@@ -1496,11 +1497,12 @@ extern "C" {
 
 int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
                           int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
-                          int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t, float softmax_scale,
-                          int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
+                          int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b,
+                          int64_t v_stride_t, float softmax_scale, int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
                           int64_t out_stride_b, int64_t out_stride_t, float* lse, void* stream) {
   int rc = masked_attention_guard(q, k, v, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, q_stride_b,
-                                  q_stride_t, kv_stride_b, kv_stride_t, softmax_scale, causal_block);
+                                  q_stride_t, k_stride_b, k_stride_t, v_stride_b, v_stride_t, softmax_scale,
+                                  causal_block);
   if (rc) return rc;
   if (out == nullptr || !aligned16(out) || !row_strides_ok(heads * 128, q_tokens, batch, out_stride_t, out_stride_b))
     return fail(OGX_EINVAL, "output");
@@ -1508,8 +1510,8 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
   if (!aligned4(q_lengths) || !aligned4(kv_lengths)) return fail(OGX_EINVAL, "lengths");
   CUtensorMap mq, mk, mv;
   if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BQ))) return rc;
-  if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, kv_stride_t, kv_stride_b, ogx::attn::BKV))) return rc;
-  if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, kv_stride_t, kv_stride_b, ogx::attn::BKV))) return rc;
+  if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, k_stride_t, k_stride_b, ogx::attn::BKV))) return rc;
+  if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, v_stride_t, v_stride_b, ogx::attn::BKV))) return rc;
   ogx::attn::Params p{};
   p.L = static_cast<int>(q_tokens);
   p.L_kv = static_cast<int>(kv_tokens);
@@ -1542,13 +1544,15 @@ int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_toke
 int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
                       const float* lse, int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
                       int64_t kv_heads, int64_t head_dim, int64_t dout_stride_b, int64_t dout_stride_t,
-                      int64_t q_stride_b, int64_t q_stride_t, int64_t kv_stride_b, int64_t kv_stride_t,
-                      int64_t out_stride_b, int64_t out_stride_t, float softmax_scale, int64_t causal_block,
-                      const int* q_lengths, const int* kv_lengths, void* workspace, int64_t workspace_bytes, void* dq,
-                      int64_t dq_stride_b, int64_t dq_stride_t, void* dk, void* dv, int64_t dkv_stride_b,
-                      int64_t dkv_stride_t, void* stream) {
+                      int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
+                      int64_t v_stride_b, int64_t v_stride_t, int64_t out_stride_b, int64_t out_stride_t, float softmax_scale,
+                      int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* workspace,
+                      int64_t workspace_bytes, void* dq, int64_t dq_stride_b, int64_t dq_stride_t, void* dk,
+                      int64_t dk_stride_b, int64_t dk_stride_t, void* dv, int64_t dv_stride_b, int64_t dv_stride_t,
+                      void* stream) {
   int rc = masked_attention_guard(q, k, v, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, q_stride_b,
-                                  q_stride_t, kv_stride_b, kv_stride_t, softmax_scale, causal_block);
+                                  q_stride_t, k_stride_b, k_stride_t, v_stride_b, v_stride_t, softmax_scale,
+                                  causal_block);
   if (rc) return rc;
   const int64_t width = heads * 128, kv_width = kv_heads * 128;
   if (dout == nullptr || out == nullptr || !aligned16(dout) || !aligned16(out) ||
@@ -1559,7 +1563,8 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   if (!aligned4(q_lengths) || !aligned4(kv_lengths)) return fail(OGX_EINVAL, "lengths");
   if (dq == nullptr || dk == nullptr || dv == nullptr || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
       !row_strides_ok(width, q_tokens, batch, dq_stride_t, dq_stride_b) ||
-      !row_strides_ok(kv_width, kv_tokens, batch, dkv_stride_t, dkv_stride_b))
+      !row_strides_ok(kv_width, kv_tokens, batch, dk_stride_t, dk_stride_b) ||
+      !row_strides_ok(kv_width, kv_tokens, batch, dv_stride_t, dv_stride_b))
     return fail(OGX_EINVAL, "gradients");
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < bwd_stats_bytes(batch, q_tokens, heads))
     return fail(OGX_EINVAL, "workspace");
@@ -1569,8 +1574,8 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   CUtensorMap mq, mk, mv, mdo;
   if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BT))) return rc;
   if ((rc = token_map(&mdo, dout, heads, q_tokens, batch, dout_stride_t, dout_stride_b, ogx::attn::BT))) return rc;
-  if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, kv_stride_t, kv_stride_b, ogx::attn::BT))) return rc;
-  if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, kv_stride_t, kv_stride_b, ogx::attn::BT))) return rc;
+  if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, k_stride_t, k_stride_b, ogx::attn::BT))) return rc;
+  if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, v_stride_t, v_stride_b, ogx::attn::BT))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 
   ogx::attn::StatsParams sp{};
@@ -1615,8 +1620,10 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   p.dv = static_cast<__nv_bfloat16*>(dv);
   p.dq_stride_b = dq_stride_b;
   p.dq_stride_t = dq_stride_t;
-  p.dkv_stride_b = dkv_stride_b;
-  p.dkv_stride_t = dkv_stride_t;
+  p.dk_stride_b = dk_stride_b;
+  p.dk_stride_t = dk_stride_t;
+  p.dv_stride_b = dv_stride_b;
+  p.dv_stride_t = dv_stride_t;
   auto kern = ogx::attn::attn_bwd_kernel;
   if ((rc = ensure_smem(kern, ogx::attn::BWD_SMEM))) return rc;
   launch(kern, dim3(static_cast<unsigned>(dkdv_ctas + dq_ctas)), ogx::attn::kBwdThreads, ogx::attn::BWD_SMEM, s, mq, mk,

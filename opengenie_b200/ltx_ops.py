@@ -1091,7 +1091,7 @@ def _given_rows(t: torch.Tensor, like: torch.Tensor, reason: str, *, written: bo
 
 
 def _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block, q_lengths, kv_lengths):
-    """Checks of the masked attention's common arguments; (q's strides, k's and v's strides, scale)."""
+    """Checks of the masked attention's common arguments; (strides of q, of k, of v, scale)."""
     device = q.device
     if device.type != "cuda" or k.device != device or v.device != device:
         raise ValueError("qkv_device_or_dtype")
@@ -1108,7 +1108,7 @@ def _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block
     if kv_heads < 1 or heads % kv_heads or Ck != kv_heads * 128:
         raise ValueError("kv_heads")
     q_rows, k_rows, v_rows = _rows(q), _rows(k), _rows(v)
-    if q_rows is None or k_rows is None or k_rows != v_rows:
+    if q_rows is None or k_rows is None or v_rows is None:
         raise ValueError("qkv_stride")
     if causal_block < 0:
         raise ValueError("causal_block")
@@ -1119,7 +1119,7 @@ def _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block
     scale = 128 ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not 1e-30 <= scale <= 1e30:
         raise ValueError("softmax_scale")
-    return q_rows, k_rows, scale
+    return q_rows, k_rows, v_rows, scale
 
 
 @functools.lru_cache(maxsize=256)
@@ -1146,8 +1146,8 @@ def attention_with_lse(
     """``attention`` with masks and shared key/value heads, and the softmax statistics that
     ``attention_backward`` needs: returns (out [B, L, heads*128] bf16, lse [B, heads, L] fp32).
 
-    q is [B, L, heads*128], k and v [B, L_kv, kv_heads*128] bf16 (token rows may be strided; k and v share
-    their strides); query head h reads key/value head ``h // (heads // kv_heads)``.  Query i sees key j if
+    q is [B, L, heads*128], k and v [B, L_kv, kv_heads*128] bf16 (token rows may be strided, each its own
+    way); query head h reads key/value head ``h // (heads // kv_heads)``.  Query i sees key j if
     ``i < q_lengths[b]``, ``j < kv_lengths[b]`` (int32 [B] on the GPU; default: all) and, with ``causal_block``
     n > 0, ``j // n <= (i + L_kv - L) // n``: n = 1 is the token-causal mask with both sequences ending
     together, the tokens of a latent frame make it frame-causal (a token sees its own and all earlier frames).
@@ -1157,8 +1157,8 @@ def attention_with_lse(
     No reference counterpart: the reference infers with dense bidirectional attention only.
     """
     kv_heads = heads if kv_heads is None else kv_heads
-    q_rows, k_rows, scale = _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block, q_lengths,
-                                                   kv_lengths)
+    q_rows, k_rows, v_rows, scale = _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block,
+                                                           q_lengths, kv_lengths)
     B, L, C = q.shape
     if out is None:
         out = q.new_empty((B, L, C))
@@ -1168,7 +1168,7 @@ def attention_with_lse(
     lse = q.new_empty((B, heads, L), dtype=torch.float32)
     _call_on(
         q.device, "ogx_attention_fwd_lse", q.data_ptr(), k.data_ptr(), v.data_ptr(), B, L, k.shape[1], heads, kv_heads,
-        128, *q_rows, *k_rows, scale, causal_block, _ptr(q_lengths), _ptr(kv_lengths), out.data_ptr(), *out_rows,
+        128, *q_rows, *k_rows, *v_rows, scale, causal_block, _ptr(q_lengths), _ptr(kv_lengths), out.data_ptr(), *out_rows,
         lse.data_ptr(),
     )
     return out, lse
@@ -1196,12 +1196,11 @@ def attention_backward(
     The probabilities are recomputed from ``lse``.  Every gradient is summed in one order (dk and dv over the
     query heads that share a key head), so equal inputs give equal bits.  Rows past ``q_lengths`` and rows that
     see no key get dq 0 and give nothing to dk and dv; keys past ``kv_lengths`` get 0.  ``grads`` takes (dq, dk,
-    dv) to write into, for example the slices of one packed [B, L, (heads + 2*kv_heads)*128] buffer; dk and dv
-    share their strides.  No reference counterpart (the reference only infers).
+    dv) to write into, for example the slices of one packed [B, L, (heads + 2*kv_heads)*128] buffer.  No reference counterpart (the reference only infers).
     """
     kv_heads = heads if kv_heads is None else kv_heads
-    q_rows, k_rows, scale = _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block, q_lengths,
-                                                   kv_lengths)
+    q_rows, k_rows, v_rows, scale = _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block,
+                                                           q_lengths, kv_lengths)
     device = q.device
     B, L, C = q.shape
     _, M, Ck = k.shape
@@ -1211,20 +1210,19 @@ def attention_backward(
         raise ValueError("lse: fp32 [B, heads, L] as attention_with_lse returns it")
     if grads is None:
         dq, dk, dv = q.new_empty((B, L, C)), q.new_empty((B, M, Ck)), q.new_empty((B, M, Ck))
-        dq_rows, dk_rows = (L * C, C), (M * Ck, Ck)
+        dq_rows, dk_rows, dv_rows = (L * C, C), (M * Ck, Ck), (M * Ck, Ck)
     else:
         dq, dk, dv = grads
-        reason = "grads: bf16 tensors of the shapes of q, k and v with unit column stride, dk and dv sharing theirs"
-        dq_rows, dk_rows = _given_rows(dq, q, reason), _given_rows(dk, k, reason)
-        if _given_rows(dv, v, reason) != dk_rows:
-            raise ValueError(reason)
+        reason = "grads: bf16 tensors of the shapes of q, k and v with unit column stride"
+        dq_rows, dk_rows, dv_rows = (_given_rows(t, like, reason) for t, like in ((dq, q), (dk, k), (dv, v)))
     workspace = q.new_empty(
         (_workspace_bytes("ogx_attention_bwd_workspace", device.index, B, L, M, heads, kv_heads),), dtype=torch.uint8)
     _call_on(
         device, "ogx_attention_bwd", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-        lse.data_ptr(), B, L, M, heads, kv_heads, 128, *dout_rows, *q_rows, *k_rows, *out_rows, scale, causal_block,
+        lse.data_ptr(), B, L, M, heads, kv_heads, 128, *dout_rows, *q_rows, *k_rows, *v_rows, *out_rows, scale,
+        causal_block,
         _ptr(q_lengths), _ptr(kv_lengths), workspace.data_ptr(), workspace.numel(), dq.data_ptr(), *dq_rows,
-        dk.data_ptr(), dv.data_ptr(), *dk_rows,
+        dk.data_ptr(), *dk_rows, dv.data_ptr(), *dv_rows,
     )
     return dq, dk, dv
 

@@ -32,7 +32,7 @@ def test_python_surface_refuses_cpu_tensors():
 
 # ogx_attention_fwd_lse arguments by name, a call that every guard accepts up to the tensor maps
 FWD = dict(q=16, k=16, v=16, batch=1, q_tokens=8, kv_tokens=8, heads=4, kv_heads=2, head_dim=128, q_stride_b=4096,
-           q_stride_t=512, kv_stride_b=2048, kv_stride_t=256, scale=0.1, causal_block=0, q_lengths=None, kv_lengths=None,
+           q_stride_t=512, k_stride_b=2048, k_stride_t=256, v_stride_b=2048, v_stride_t=256, scale=0.1, causal_block=0, q_lengths=None, kv_lengths=None,
            out=16, out_stride_b=4096, out_stride_t=512, lse=16, stream=None)
 
 
@@ -42,7 +42,7 @@ FWD = dict(q=16, k=16, v=16, batch=1, q_tokens=8, kv_tokens=8, heads=4, kv_heads
     (dict(kv_heads=3), "kv_heads"), (dict(causal_block=-1), "causal_block"), (dict(scale=0.0), "softmax_scale"),
     (dict(scale=-1.0), "softmax_scale"), (dict(scale=float("nan")), "softmax_scale"),
     (dict(scale=float("inf")), "softmax_scale"), (dict(q_stride_t=511), "stride"), (dict(q_stride_t=504), "stride"),
-    (dict(kv_stride_t=248), "stride"), (dict(q_stride_b=-8), "stride"), (dict(q_stride_t=1 << 38), "stride"),
+    (dict(k_stride_t=248), "stride"), (dict(v_stride_t=248), "stride"), (dict(q_stride_b=-8), "stride"), (dict(q_stride_t=1 << 38), "stride"),
     (dict(k=8), "alignment"), (dict(out=None), "output"), (dict(out=24), "output"), (dict(out_stride_t=256), "output"),
     (dict(lse=None), "lse"), (dict(lse=18), "lse"), (dict(kv_lengths=18), "lengths"),
 ], ids=str)
@@ -52,16 +52,16 @@ def test_attention_entry_refusals(ogx_lib, change, reason):
 
 
 BWD = dict(dout=16, q=16, k=16, v=16, out=16, lse=16, batch=1, q_tokens=8, kv_tokens=8, heads=4, kv_heads=2,
-           head_dim=128, dout_stride_b=4096, dout_stride_t=512, q_stride_b=4096, q_stride_t=512, kv_stride_b=2048,
-           kv_stride_t=256, out_stride_b=4096, out_stride_t=512, scale=0.1, causal_block=0, q_lengths=None,
+           head_dim=128, dout_stride_b=4096, dout_stride_t=512, q_stride_b=4096, q_stride_t=512, k_stride_b=2048,
+           k_stride_t=256, v_stride_b=2048, v_stride_t=256, out_stride_b=4096, out_stride_t=512, scale=0.1, causal_block=0, q_lengths=None,
            kv_lengths=None, workspace=16, workspace_bytes=1 << 40, dq=16, dq_stride_b=4096, dq_stride_t=512, dk=16,
-           dv=16, dkv_stride_b=2048, dkv_stride_t=256, stream=None)
+           dk_stride_b=2048, dk_stride_t=256, dv=16, dv_stride_b=2048, dv_stride_t=256, stream=None)
 
 
 @pytest.mark.parametrize("change,reason", [
     (dict(v=None), "null_pointer"), (dict(dout=None), "dout_or_out"), (dict(out=8), "dout_or_out"),
     (dict(dout_stride_t=256), "dout_or_out"), (dict(lse=None), "lse"), (dict(dq=None), "gradients"),
-    (dict(dk=8), "gradients"), (dict(dkv_stride_t=128), "gradients"), (dict(workspace=None), "workspace"),
+    (dict(dk=8), "gradients"), (dict(dk_stride_t=128), "gradients"), (dict(dv_stride_t=128), "gradients"), (dict(workspace=None), "workspace"),
     (dict(workspace_bytes=15), "workspace"), (dict(workspace=8), "workspace"), (dict(scale=0.0), "softmax_scale"),
     (dict(q_lengths=2), "lengths"),
 ], ids=str)
