@@ -1703,6 +1703,18 @@ int64_t qk_partial_bytes(const QkShape& sh, int norm, int64_t heads, int64_t hea
   return norm == kNone ? 0 : 4 * qk_partial_rows(sh, norm) * qk_weight_columns(norm, heads, head_dim);
 }
 
+template <int HD, bool INTER, bool PER_HEAD, bool BACKWARD>
+void qk_launch_row(const ogx::qkn::Params& p, int steps, dim3 g, cudaStream_t s) {
+  using namespace ogx::qkn;
+  if (qk_threads(p.t[0].heads, p.t[1].heads, HD, kRow) == 256)
+    return steps == 1 ? launch(qk_row_kernel<HD, 256, 1, INTER, PER_HEAD, BACKWARD>, g, 256, 0, s, p)
+                      : launch(qk_row_kernel<HD, 256, 2, INTER, PER_HEAD, BACKWARD>, g, 256, 0, s, p);
+  if constexpr (HD == 128) {  // 64 groups of 64 columns take every head in two steps
+    if (steps == 4) return launch(qk_row_kernel<HD, 512, 4, INTER, PER_HEAD, BACKWARD>, g, 512, 0, s, p);
+  }
+  return launch(qk_row_kernel<HD, 512, 2, INTER, PER_HEAD, BACKWARD>, g, 512, 0, s, p);
+}
+
 template <int HD, bool INTER, bool BACKWARD>
 void qk_launch(const ogx::qkn::Params& p, int steps, int norm, cudaStream_t s) {
   using namespace ogx::qkn;
@@ -1713,13 +1725,8 @@ void qk_launch(const ogx::qkn::Params& p, int steps, int norm, cudaStream_t s) {
   if (norm == kHead)
     return p.cs_stride_h ? launch(qk_head_kernel<HD, kHead, INTER, true, BACKWARD>, g, kThreads, 0, s, p)
                          : launch(qk_head_kernel<HD, kHead, INTER, false, BACKWARD>, g, kThreads, 0, s, p);
-  if (qk_threads(p.t[0].heads, p.t[1].heads, HD, norm) == 256)
-    return steps == 1 ? launch(qk_row_kernel<HD, 256, 1, INTER, BACKWARD>, g, 256, 0, s, p)
-                      : launch(qk_row_kernel<HD, 256, 2, INTER, BACKWARD>, g, 256, 0, s, p);
-  if constexpr (HD == 128) {  // 64 groups of 64 columns take every head in two steps
-    if (steps == 4) return launch(qk_row_kernel<HD, 512, 4, INTER, BACKWARD>, g, 512, 0, s, p);
-  }
-  return launch(qk_row_kernel<HD, 512, 2, INTER, BACKWARD>, g, 512, 0, s, p);
+  if (p.cs_stride_h) return qk_launch_row<HD, INTER, true, BACKWARD>(p, steps, g, s);
+  qk_launch_row<HD, INTER, false, BACKWARD>(p, steps, g, s);
 }
 
 template <bool BACKWARD>

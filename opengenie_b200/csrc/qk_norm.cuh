@@ -136,22 +136,34 @@ __device__ __forceinline__ void load4_of(const char* at, int entry, int fp32, f2
   }
 }
 
-// cos and sin of a lane's four pairs; lanes past the rotated columns turn by nothing; `sign` -1 turns back.
+// Where a lane finds its four pairs' angles: the address of its cos entries, and sin's distance from it.
+struct AngleRow {
+  const char* cos;
+  int64_t to_sin;
+  int fp32;
+  bool turned;  // false: the lane's columns lie past the rotated ones
+  __device__ __forceinline__ AngleRow(const Params& p, int64_t at, int sub)
+      : cos(p.cos + at + sub * (p.cs_fp32 ? 16 : 8)), to_sin(p.sin - p.cos), fp32(p.cs_fp32), turned(sub * 8 < p.rotary) {}
+};
+
+// cos and sin of a lane's four pairs, for the rotation or (BACK) for turning back; columns that do not turn have 1, 0.
 struct Turn {
   f2 c[2], s[2], ns[2];
-  // `at`: byte offset of the token's (and head's) first entry
-  __device__ __forceinline__ void load(const Params& p, int64_t at, int sub, float sign) {
-    if (sub * 8 < p.rotary) {
-      load4_of(p.cos + at, sub * 4, p.cs_fp32, c);
-      load4_of(p.sin + at, sub * 4, p.cs_fp32, s);
+  template <bool BACK>
+  __device__ __forceinline__ void load(const AngleRow& a, int64_t offset) {
+    f2 t[2];
+    if (a.turned) {
+      load4_of(a.cos + offset, 0, a.fp32, c);
+      load4_of(a.cos + offset + a.to_sin, 0, a.fp32, t);
     } else {
       c[0] = c[1] = f2{1.f, 1.f};
-      s[0] = s[1] = f2{0.f, 0.f};
+      t[0] = t[1] = f2{0.f, 0.f};
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      ns[i] = mul2(s[i], f2{-sign, -sign});
-      s[i] = mul2(s[i], f2{sign, sign});
+      const f2 n = mul2(t[i], f2{-1.f, -1.f});
+      s[i] = BACK ? n : t[i];
+      ns[i] = BACK ? t[i] : n;
     }
   }
   __device__ __forceinline__ Lane operator()(const Lane& v) const {
@@ -280,11 +292,10 @@ __device__ __forceinline__ void prefetch_rows(const Params& p, const Tensor& a, 
 
 // Its part of a head's angles to L2, by each lane (bulk prefetches of so small pieces, one lane after the other,
 // took longer than the rows themselves).
-__device__ __forceinline__ void prefetch_angles(const Params& p, int64_t at, int sub) {
-  if (sub * 8 >= p.rotary) return;
-  const int64_t own = at + sub * (p.cs_fp32 ? 16 : 8);
-  asm volatile("prefetch.global.L2 [%0];" ::"l"(p.cos + own));
-  asm volatile("prefetch.global.L2 [%0];" ::"l"(p.sin + own));
+__device__ __forceinline__ void prefetch_angles(const AngleRow& a, int64_t offset) {
+  if (!a.turned) return;
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(a.cos + offset));
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(a.cos + offset + a.to_sin));
 }
 
 __device__ __forceinline__ void elements(const Lane& v, float (&e)[8]) {
@@ -300,7 +311,6 @@ __global__ void __launch_bounds__(kThreads, head_ctas(BACKWARD)) qk_head_kernel(
   constexpr int GROUPS = kThreads / LANES;
   constexpr int UNROLL = BACKWARD ? 2 : 4;
   constexpr bool X = NORM != kNone || !BACKWARD;
-  constexpr float sign = BACKWARD ? -1.f : 1.f;
   pdl_trigger();
   pdl_wait();
   const Place place(p);
@@ -324,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, head_ctas(BACKWARD)) qk_head_kernel(
   const char* xp = row_address(a.x, batch0, at.token) + offset;
   const char* dp = BACKWARD ? row_address(a.dy, batch0, at.token) + offset : nullptr;
   char* yp = row_address(a.y, batch0, at.token) + offset;
-  int64_t angles = batch0 * a.angles.stride_b + at.token * a.angles.stride_t;
+  AngleRow angles(p, batch0 * a.angles.stride_b + at.token * a.angles.stride_t + (PER_HEAD ? member * p.cs_stride_h : 0), sub);
   uint4 xr[UNROLL] = {}, dr[UNROLL] = {};  // idle slots keep what was there before, and write nothing
   // whole warps run every iteration: the shuffles name all lanes
   for (int row0 = place.cta * teams; row0 < p.rows; row0 += rows_per_step) {
@@ -332,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, head_ctas(BACKWARD)) qk_head_kernel(
     const bool row_ok = at.row < p.rows;
     Turn turn{};
     if constexpr (!PER_HEAD) {
-      if (row_ok) turn.load(p, angles, sub, sign);
+      if (row_ok) turn.load<BACKWARD>(angles, 0);
     }
     const WeightedTurn step1(turn, w);  // used by the forward pass of a norm with shared tables
     for (int i0 = 0; i0 < heads; i0 += UNROLL * stride) {
@@ -350,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, head_ctas(BACKWARD)) qk_head_kernel(
         if (h >= heads) break;  // the same for the whole CTA
         const bool ok = row_ok && h + member < heads;
         if constexpr (PER_HEAD) {
-          if (ok) turn.load(p, angles + (h + member) * p.cs_stride_h, sub, sign);
+          if (ok) turn.load<BACKWARD>(angles, h * p.cs_stride_h);
         }
         Lane v;
         if constexpr (NORM == kNone) {
@@ -375,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, head_ctas(BACKWARD)) qk_head_kernel(
     if constexpr (X) xp += step_of(a.x, at.wrapped);
     if constexpr (BACKWARD) dp += step_of(a.dy, at.wrapped);
     yp += step_of(a.y, at.wrapped);
-    angles += step_of(a.angles, at.wrapped);
+    angles.cos += step_of(a.angles, at.wrapped);
   }
 
   if constexpr (BACKWARD && NORM == kHead) {
@@ -397,11 +407,10 @@ __global__ void __launch_bounds__(kThreads, head_ctas(BACKWARD)) qk_head_kernel(
 
 // ------------------------------------------------------------------------- norm over all heads of a row
 // A team holds its token's columns (STEPS heads per group) until the row's sums are known.
-template <int HD, int THREADS, int STEPS, bool INTER, bool BACKWARD>
+template <int HD, int THREADS, int STEPS, bool INTER, bool PER_HEAD, bool BACKWARD>
 __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kernel(const __grid_constant__ Params p) {
   constexpr int LANES = HD / 8;
   constexpr int GROUPS = THREADS / LANES;
-  constexpr float sign = BACKWARD ? -1.f : 1.f;
   __shared__ __align__(8) float sums[2][GROUPS][2];  // alternating rows: each group's sums of x^2 and g w x
   pdl_trigger();
   pdl_wait();
@@ -436,8 +445,9 @@ __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kern
   const char* xp = row_address(a.x, batch0, at.token) + offset;
   const char* dp = BACKWARD ? row_address(a.dy, batch0, at.token) + offset : nullptr;
   char* yp = row_address(a.y, batch0, at.token) + offset;
-  int64_t angles = batch0 * a.angles.stride_b + at.token * a.angles.stride_t;
-  const bool per_head = p.cs_stride_h != 0;
+  const int64_t head_step = stride * p.cs_stride_h;  // to the angles of the group's next head
+  AngleRow angles(p, batch0 * a.angles.stride_b + at.token * a.angles.stride_t + (PER_HEAD ? member * p.cs_stride_h : 0), sub);
+  // groups past the last head keep zeros; a team past the last row keeps its last one, and writes nothing
   uint4 xr[STEPS] = {}, dr[STEPS] = {};
   const auto load_row = [&](bool ok) {
 #pragma unroll
@@ -445,8 +455,6 @@ __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kern
       if (ok && i * stride + member < heads) {
         xr[i] = col.load(xp + i * stride * (HD * 2));
         if constexpr (BACKWARD) dr[i] = col.load(dp + i * stride * (HD * 2));
-      } else {
-        xr[i] = dr[i] = make_uint4(0, 0, 0, 0);
       }
     }
   };
@@ -456,14 +464,14 @@ __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kern
     prefetch_rows<HD, true, BACKWARD>(p, a, row0 + 2 * rows_per_step, teams);
     const bool row_ok = at.row < p.rows;
     at.step(p, a, rows_per_step);
-    const int64_t angles_next = angles + step_of(a.angles, at.wrapped);
-    if (per_head && at.row < p.rows) {
+    const int64_t to_next = step_of(a.angles, at.wrapped);
+    if (PER_HEAD && at.row < p.rows) {
 #pragma unroll
       for (int i = 0; i < STEPS; ++i)
-        if (i * stride + member < heads) prefetch_angles(p, angles_next + (i * stride + member) * p.cs_stride_h, sub);
+        if (i * stride + member < heads) prefetch_angles(angles, to_next + i * head_step);
     }
     Turn turn{};
-    if (!per_head && row_ok) turn.load(p, angles, sub, sign);
+    if (!PER_HEAD && row_ok) turn.load<BACKWARD>(angles, 0);
     Lane x[STEPS], g[STEPS];
     float sq = 0.f, gwx = 0.f;
 #pragma unroll
@@ -471,8 +479,7 @@ __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kern
       const int h = i * stride + member;
       x[i] = unpack_lane<INTER>(xr[i]);
       sq += dot(x[i], x[i]);
-      if ((BACKWARD || STEPS == 1) && per_head && row_ok && h < heads)
-        turn.load(p, angles + h * p.cs_stride_h, sub, sign);
+      if ((BACKWARD || STEPS == 1) && PER_HEAD && row_ok && h < heads) turn.load<BACKWARD>(angles, i * head_step);
       if constexpr (BACKWARD) {
         if constexpr (!KEEP) w[i] = weights_of(i);
         g[i] = turn(unpack_lane<INTER>(dr[i]));
@@ -504,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kern
       Lane v;
       if constexpr (!BACKWARD) {
         // with one head per group its angles are still there
-        if (STEPS > 1 && per_head && ok) turn.load(p, angles + h * p.cs_stride_h, sub, sign);
+        if (STEPS > 1 && PER_HEAD && ok) turn.load<BACKWARD>(angles, i * head_step);
         if constexpr (!KEEP) w[i] = weights_of(i);
         v = turn(mul(mul(x[i], inv), w[i]));
       } else {
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kern
       if (ok) col.store(yp + i * stride * (HD * 2), pack_lane<INTER>(v));
     }
     yp += step_of(a.y, at.wrapped);
-    angles = angles_next;
+    angles.cos += to_next;
   }
 
   if constexpr (BACKWARD) {
