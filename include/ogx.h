@@ -368,14 +368,21 @@ int ogx_attention_fwd_e4m3_to_peers(const void* q, const void* k, const void* v,
  * causal_block 1 is the token-causal mask with both sequences ending together, n a mask over blocks of n
  * positions (the tokens of a latent frame).  out: bf16 [batch, q_tokens, heads*128]; lse: f32 [batch, heads,
  * q_tokens], the natural log of each row's sum of exponentials.  A row that sees no key gets out = 0 and lse =
- * -inf.  Keys and values past kv_lengths may hold anything (NaN included). */
+ * -inf.  Keys and values past kv_lengths may hold anything (NaN included).  Few queries over many keys are shared out
+ * over the keys and joined in a second launch; workspace (device memory, 16-byte aligned, overwritten; calls that may
+ * run at the same time need one each) holds the parts: ogx_attention_fwd_lse_workspace says how much, often 0 (then
+ * it may be NULL). */
 int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
                           int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
                           int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b,
                           int64_t v_stride_t, float softmax_scale, int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
-                          int64_t out_stride_b, int64_t out_stride_t, float* lse, void* stream);
+                          int64_t out_stride_b, int64_t out_stride_t, float* lse, void* workspace,
+                          int64_t workspace_bytes, void* stream);
 
-/* Bytes of device workspace that ogx_attention_bwd needs for these sizes. */
+/* Bytes of device workspace that ogx_attention_fwd_lse needs for these sizes on the current device. */
+int ogx_attention_fwd_lse_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t* bytes);
+
+/* Bytes of device workspace that ogx_attention_bwd needs for these sizes on the current device. */
 int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads,
                                 int64_t* bytes);
 

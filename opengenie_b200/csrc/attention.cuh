@@ -80,6 +80,11 @@ struct Params {
   int causal_block;            // 0: every key is visible
   const int* q_lengths;        // [batch] or null
   const int* kv_lengths;       // [batch] or null
+  // few query blocks over many keys: `splits` CTAs share a block's key tiles (split_tiles each) and leave their
+  // unnormalised rows and row statistics, [batch][heads][splits][L] x (128 | max, sum), for attn_join_kernel
+  int splits, split_tiles;
+  float* part_o;
+  float2* part_ml;
 };
 
 // Which keys a query sees.  Queries from q_len on see none; keys from kv_len on are seen by none.  With
@@ -226,7 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t warp = warp_idx();
   const uint32_t lane = threadIdx.x & 31;
   const int head = blockIdx.y;
-  const int batch = blockIdx.z;
+  const int batch = MASKED ? blockIdx.z / p.splits : blockIdx.z;
+  const int split = MASKED ? blockIdx.z % p.splits : 0;
   // causal rows get longer with their index: the longest blocks start first
   const int q_block0 = (MASKED ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * (NQ * BQ);
   const int kv_head = MASKED ? head / p.heads_per_kv : head;
@@ -263,12 +269,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   int nkv = (p.L_kv + BKV - 1) / BKV;
   Visibility vis{};
   int fix_tile = -1;  // the V tile whose last rows lie past the keys' length
+  const int tile0 = MASKED ? split * p.split_tiles : 0;  // this CTA's first key tile
   if constexpr (MASKED) {
     vis = Visibility{clamp_length(p.q_lengths, batch, p.L), clamp_length(p.kv_lengths, batch, p.L_kv), p.causal_block,
                      p.L_kv - p.L};
     const int last = min(q_block0 + NQ * BQ, vis.q_len) - 1;  // limit() grows with the row
     nkv = last < q_block0 ? 0 : (vis.limit(last) + BKV - 1) / BKV;
-    if (vis.kv_len < p.L_kv && vis.kv_len % BKV != 0 && vis.kv_len / BKV < nkv) fix_tile = vis.kv_len / BKV;
+    nkv = min(max(nkv - tile0, 0), p.split_tiles);
+    const int border = vis.kv_len / BKV - tile0;
+    if (vis.kv_len < p.L_kv && vis.kv_len % BKV != 0 && border >= 0 && border < nkv) fix_tile = border;
   }
   tc_fence_before();
   __syncthreads();
@@ -302,11 +311,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t ph = (j / KV_STAGES) & 1;
         if (!mbar_wait(&st.k_empty[s], ph ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.k_full[s], KV_TILE_BYTES);
-        load_rows(k_tiles + s * KV_TILE_BYTES, &tk, &st.k_full[s], KV_HALF_BYTES, kv_head, j * BKV, batch);
+        load_rows(k_tiles + s * KV_TILE_BYTES, &tk, &st.k_full[s], KV_HALF_BYTES, kv_head, (tile0 + j) * BKV, batch);
         ++issued;
         if (!mbar_wait(&st.v_empty[s], ph ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.v_full[s], KV_TILE_BYTES);
-        load_rows(v_tiles + s * KV_TILE_BYTES, &tv, &st.v_full[s], KV_HALF_BYTES, kv_head, j * BKV, batch);
+        load_rows(v_tiles + s * KV_TILE_BYTES, &tv, &st.v_full[s], KV_HALF_BYTES, kv_head, (tile0 + j) * BKV, batch);
         ++issued;
       }
       if (*abort) {
@@ -403,7 +412,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m_run = -INFINITY;  // running max, already multiplied by c
     float l_run = 0.f;
     bool ok = true;
-    const int limit = MASKED ? vis.limit(q_block0 + q * BQ + row) : p.L_kv;
+    // visible keys from this CTA's first one on
+    const int limit = MASKED ? vis.limit(q_block0 + q * BQ + row) - tile0 * BKV : p.L_kv;
     for (int j = 0; j < nkv; ++j) {
       const int b = j & 1;
       const uint32_t s_tmem = tmem + lane_off + TMEM_S + q * 128 + b * 64;
@@ -436,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float alpha = 1.f;
       bool rescale = false;
       if (j == 0) {
-        m_use = (MASKED && limit <= 0) ? 0.f : m_tile;  // key 0 is visible to every row that sees any
+        m_use = (MASKED && limit <= 0) ? 0.f : m_tile;  // a row that sees any of these keys sees the first
       } else if (m_tile > m_run + kRescaleThreshold) {
         m_use = m_tile;
         alpha = ex2(m_run - m_tile);
@@ -485,7 +495,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (MASKED && nkv == 0) {
       const int token = q_block0 + q * BQ + row;
-      if (token < p.L) {
+      if (token < p.L && p.splits > 1) {
+        p.part_ml[((static_cast<int64_t>(batch) * gridDim.y + head) * p.splits + split) * p.L + token] =
+            make_float2(-INFINITY, 0.f);
+      } else if (token < p.L) {
         uint4* dst = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(batch) * p.out_stride_b +
                                               static_cast<int64_t>(token) * p.out_stride_t +
                                               static_cast<int64_t>(head) * HD);
@@ -498,7 +511,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int token = q_block0 + q * BQ + row;
       const float inv_l = 1.f / l_run;
       if constexpr (MASKED) {
-        if (token < p.L)
+        if (p.splits > 1) {
+          const int64_t at = ((static_cast<int64_t>(batch) * gridDim.y + head) * p.splits + split) * p.L + token;
+          if (token < p.L) p.part_ml[at] = limit <= 0 ? make_float2(-INFINITY, 0.f) : make_float2(m_run, l_run);
+#pragma unroll 1
+          for (int oc = 0; oc < 4; ++oc) {
+            uint32_t orr[32];
+            tmem_ld32(o_tmem + oc * 32, orr);
+            tmem_ld_wait();
+            if (token < p.L && limit > 0) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                reinterpret_cast<uint4*>(p.part_o + at * HD + oc * 32)[i] =
+                    make_uint4(orr[4 * i], orr[4 * i + 1], orr[4 * i + 2], orr[4 * i + 3]);
+            }
+          }
+        } else if (token < p.L)
           p.lse[(static_cast<int64_t>(batch) * gridDim.y + head) * p.L + token] =
               limit <= 0 ? -INFINITY : (m_run + log2f(l_run)) * 0.6931471805599453f;
       }
@@ -555,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(head) * HD + g * 16u) = v;
           }
         }
-      } else {
+      } else if (!MASKED || p.splits == 1) {
 #pragma unroll 1
         for (int oc = 0; oc < 4; ++oc) {
           uint32_t orr[32];
@@ -586,6 +614,51 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
+}
+
+// Joins the splits of the MASKED kernel, one warp per query row: with m_i, l_i, O_i of split i and M = max m_i,
+// O = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  Splits where a row saw no key have l = 0 and an O that was never
+// written.  The splits are added in their order.
+struct JoinParams {
+  const float* part_o;
+  const float2* part_ml;
+  __nv_bfloat16* out;
+  int64_t out_stride_b, out_stride_t;
+  float* lse;
+  int L, heads, splits;
+  int64_t rows;  // batch * heads * L
+};
+
+__global__ void __launch_bounds__(256) attn_join_kernel(JoinParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const int64_t bh = row / p.L;
+  const int token = static_cast<int>(row - bh * p.L);
+  const int64_t first = bh * p.splits * p.L + token;
+  float m = -INFINITY;
+  for (int i = 0; i < p.splits; ++i) m = fmaxf(m, p.part_ml[first + static_cast<int64_t>(i) * p.L].x);
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < p.splits; ++i) {
+    const int64_t at = first + static_cast<int64_t>(i) * p.L;
+    const float2 ml = p.part_ml[at];
+    if (ml.y == 0.f) continue;  // the same for the whole warp
+    const float w = exp2f(ml.x - m);
+    const float4 v = reinterpret_cast<const float4*>(p.part_o + at * HD)[lane];
+    l = fmaf(w, ml.y, l);
+    o.x = fmaf(w, v.x, o.x);
+    o.y = fmaf(w, v.y, o.y);
+    o.z = fmaf(w, v.z, o.z);
+    o.w = fmaf(w, v.w, o.w);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t batch = bh / p.heads, head = bh - batch * p.heads;
+  reinterpret_cast<uint2*>(p.out + batch * p.out_stride_b + token * p.out_stride_t + head * HD)[lane] =
+      make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  if (lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------------------------------

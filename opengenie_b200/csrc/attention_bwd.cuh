@@ -4,12 +4,19 @@
 //   dV = P^T dO,   dP = dO V^T,   dS = P o (dP - delta),   dQ = c dS K,   dK = c dS^T Q;
 // dK and dV of a shared key/value head sum over its query heads.
 //
-// Two launches.  attn_bwd_stats_kernel writes per query row -lse * log2(e) and -delta.  attn_bwd_kernel has a
-// CTA for every tile of 128 keys of a key/value head (dK and dV, over all query tiles of its query heads)
-// and a CTA for every tile of 128 queries of a head (dQ, over all key tiles).  S and dP are computed in both:
-// seven tile products instead of five.  In return every gradient is summed in one CTA's tensor memory in a
-// fixed order: no fp32 buffer for dQ, no atomics, and the same bits on every run.  The five-product form adds
-// its dQ tiles to HBM (a 64 KB reduction per tile pair, in whatever order the CTAs reach it).
+// attn_bwd_stats_kernel writes per query row -lse * log2(e) and -delta.  attn_bwd_kernel has a CTA for every tile
+// of 128 keys of a key/value head (dK and dV, over all query tiles of its query heads) and a CTA for every tile of
+// 128 queries of a head (dQ, over all key tiles).  S and dP are computed in both: seven tile products instead of
+// five.  In return every gradient is summed in one CTA's tensor memory in a fixed order: no fp32 buffer for dQ, no
+// atomics, and the same bits on every run.  (The five-product form adds its dQ tiles to HBM, a 64 KB reduction per
+// tile pair, in whatever order the CTAs reach it.)  Where one side has so few tiles that the GPU would idle behind
+// long sums, several CTAs share a sum and attn_bwd_join_kernel adds their parts, in their order.
+//
+// What bounds it, at 9216 x 9216 x 32 heads: 3.71 ms back to back, under the 1000 W cap (1.43 GHz) 1312 TFLOP/s of
+// its seven products, 96 % of what cuBLAS sustains there; 3.20 ms in a burst.  Per tile pair the two roles take 2700
+// and 1900 cycles for 2048 and 1536 of products: the S and dP products use the whole 128 bytes per clock of shared
+// memory, so that every TMA write (64 KB a pair) delays them, and a CTA spends about 9000 cycles on starting (TMA
+// latency, first scores) and storing.
 #pragma once
 
 #include "attention.cuh"
@@ -36,6 +43,8 @@ struct BwdParams {
   int heads, kv_heads, heads_per_kv;
   int q_tiles, kv_tiles;
   unsigned dkdv_ctas;  // CTAs [0, dkdv_ctas) make dK and dV, the rest dQ
+  int dkdv_splits, dq_splits;  // CTAs that share a tile's sum
+  float *dkdv_parts, *dq_parts;  // fp32 [tile][split][dV, dK][128][128], [tile][split][128][128] (splits > 1)
   int causal_block;
   float scale, scale_log2;
   const int* q_lengths;
@@ -125,6 +134,19 @@ __device__ __forceinline__ void store_rows(uint32_t taddr, int columns, float sc
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (i < left) *reinterpret_cast<uint4*>(mine + i * stride + oc * 32) = piece[i];
+  }
+}
+
+// `columns` fp32 columns of a warp's 32 rows to a CTA's part of a shared sum (rows of 128, a row per lane).
+__device__ __forceinline__ void store_part(uint32_t taddr, int columns, float* dst, uint32_t lane) {
+#pragma unroll 1
+  for (int oc = 0; oc < columns / 32; ++oc) {
+    uint32_t r[32];
+    tmem_ld32(taddr + oc * 32, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      reinterpret_cast<uint4*>(dst + lane * HD + oc * 32)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
   }
 }
 
@@ -256,7 +278,8 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
   const uint32_t lane = threadIdx.x & 31;
   volatile int* abort = &st.abort;
 
-  const unsigned idx = blockIdx.x;
+  const int split = static_cast<int>(blockIdx.x % p.dkdv_splits);
+  const unsigned idx = blockIdx.x / p.dkdv_splits;
   const int kt = static_cast<int>(idx % p.kv_tiles);
   const int bh = static_cast<int>(idx / p.kv_tiles);
   const int kv_head = bh % p.kv_heads;
@@ -267,12 +290,22 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
   const int first_tile = max(vis.first(k0), 0) / BT;
   const int end_tile = (vis.q_len + BT - 1) / BT;
   const int per_head = (k0 >= vis.kv_len || end_tile <= first_tile) ? 0 : end_tile - first_tile;
-  const int n = per_head * p.heads_per_kv;
+  // this CTA's tiles of all those of the group's heads: [begin, begin + n)
+  const int all = per_head * p.heads_per_kv;
+  const int share = (all + p.dkdv_splits - 1) / p.dkdv_splits;
+  const int begin = min(split * share, all);
+  const int n = min(share, all - begin);
+  const int head0 = kv_head * p.heads_per_kv + (per_head > 0 ? begin / per_head : 0);
+  const int tile0 = first_tile + (per_head > 0 ? begin % per_head : 0);
+  float* part = p.dkdv_parts + (static_cast<int64_t>(idx) * p.dkdv_splits + split) * (2 * BT * HD);
   // the last query tile of each head has rows past the sequence's length, holding the caller's memory
   const bool fix = vis.q_len < p.L && vis.q_len % BT != 0;
 
   if (n == 0) {
-    if (warp >= 4) {
+    if (warp >= 4 && p.dkdv_splits > 1) {
+      for (int i = threadIdx.x - 128; i < 2 * BT * HD / 4; i += 256)
+        reinterpret_cast<uint4*>(part)[i] = make_uint4(0, 0, 0, 0);
+    } else if (warp >= 4) {
       const int key = k0 + static_cast<int>((warp & 3) * 32 + lane);
       const int64_t column = static_cast<int64_t>(kv_head) * HD;
       if (key < p.L_kv)
@@ -289,7 +322,7 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
       mbar_arrive_expect_tx(&st.fixed_full[0], T_BYTES);
       load_rows(k_tile, tk, &st.fixed_full[0], T_HALF_BYTES, kv_head, k0, batch);
       int a_issued = 0, b_issued = 0;
-      int head = kv_head * p.heads_per_kv, tile = first_tile;
+      int head = head0, tile = tile0;
       for (int j = 0; j < n; ++j) {
         const int s = j % B_STAGES;
         const uint32_t ph = (j / B_STAGES) & 1;
@@ -333,7 +366,7 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
       auto q_ready = [&](int j) {
         const int s = j % B_STAGES;
         if (!mbar_wait(&st.a_full[s], (j / B_STAGES) & 1, abort)) return false;
-        if (fix && (j + 1) % per_head == 0) {
+        if (fix && (begin + j + 1) % per_head == 0) {
           if (!mbar_wait(&st.b_full[s], (j / B_STAGES) & 1, abort)) return false;
           mbar_arrive(&st.zero_request);
           if (!mbar_wait(&st.zeroed, requests++ & 1, abort)) return false;
@@ -388,7 +421,7 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
     if (fix) {
       // ---------------------------------------------------------- zeroes the rows past the queries' length
       uint32_t request = 0;
-      for (int j = per_head - 1; j < n; j += per_head) {
+      for (int j = per_head - 1 - begin % per_head; j < n; j += per_head) {
         const int s = j % B_STAGES;
         const uint32_t ph = (j / B_STAGES) & 1;
         if (!mbar_wait(&st.zero_request, request++ & 1, abort)) break;
@@ -414,7 +447,7 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
     const int all_from = vis.first(min(k0 + BT, vis.kv_len) - 1);
     const bool ragged_keys = k0 + BT > vis.kv_len;
     bool ok = true;
-    int tile = first_tile;
+    int tile = tile0;
     for (int j = 0; j < n; ++j) {
       const int s = j % B_STAGES;
       const int q0 = tile * BT;
@@ -482,13 +515,19 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
     const int column = kv_head * HD + g * 64;
     if (ok && mbar_wait(&st.dv_done, 0, abort)) {
       tc_fence_after();
-      store_rows(tmem + lane_off + 256 + g * 64, 64, 1.f, p.dv + batch * p.dv_stride_b + key0 * p.dv_stride_t + column,
-                 p.dv_stride_t, p.L_kv - key0, lane);
+      if (p.dkdv_splits > 1)
+        store_part(tmem + lane_off + 256 + g * 64, 64, part + quarter * 32 * HD + g * 64, lane);
+      else
+        store_rows(tmem + lane_off + 256 + g * 64, 64, 1.f,
+                   p.dv + batch * p.dv_stride_b + key0 * p.dv_stride_t + column, p.dv_stride_t, p.L_kv - key0, lane);
     }
     if (ok && mbar_wait(&st.done, 0, abort)) {
       tc_fence_after();
-      store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale,
-                 p.dk + batch * p.dk_stride_b + key0 * p.dk_stride_t + column, p.dk_stride_t, p.L_kv - key0, lane);
+      if (p.dkdv_splits > 1)
+        store_part(tmem + lane_off + 384 + g * 64, 64, part + BT * HD + quarter * 32 * HD + g * 64, lane);
+      else
+        store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale,
+                   p.dk + batch * p.dk_stride_b + key0 * p.dk_stride_t + column, p.dk_stride_t, p.L_kv - key0, lane);
     }
   }
 }
@@ -509,7 +548,8 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
   const uint32_t lane = threadIdx.x & 31;
   volatile int* abort = &st.abort;
 
-  const unsigned idx = blockIdx.x - p.dkdv_ctas;
+  const int split = static_cast<int>((blockIdx.x - p.dkdv_ctas) % p.dq_splits);
+  const unsigned idx = (blockIdx.x - p.dkdv_ctas) / p.dq_splits;
   const int qt = p.q_tiles - 1 - static_cast<int>(idx % p.q_tiles);  // causal rows get longer with their index
   const int bh = static_cast<int>(idx / p.q_tiles);
   const int head = bh % p.heads;
@@ -519,11 +559,19 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
   const Visibility vis{clamp_length(p.q_lengths, batch, p.L), clamp_length(p.kv_lengths, batch, p.L_kv),
                        p.causal_block, p.L_kv - p.L};
   const int last = min(q0 + BT, vis.q_len) - 1;
-  const int n = last < q0 ? 0 : (vis.limit(last) + BT - 1) / BT;
-  const int fix_tile = (vis.kv_len < p.L_kv && vis.kv_len % BT != 0 && vis.kv_len / BT < n) ? vis.kv_len / BT : -1;
+  // this CTA's tiles of those its queries see: [tile0, tile0 + n)
+  const int all = last < q0 ? 0 : (vis.limit(last) + BT - 1) / BT;
+  const int share = (all + p.dq_splits - 1) / p.dq_splits;
+  const int tile0 = min(split * share, all);
+  const int n = min(share, all - tile0);
+  const int border = vis.kv_len / BT - tile0;
+  const int fix_tile = (vis.kv_len < p.L_kv && vis.kv_len % BT != 0 && border >= 0 && border < n) ? border : -1;
+  float* part = p.dq_parts + (static_cast<int64_t>(idx) * p.dq_splits + split) * (BT * HD);
 
   if (n == 0) {
-    if (warp >= 4) {
+    if (warp >= 4 && p.dq_splits > 1) {
+      for (int i = threadIdx.x - 128; i < BT * HD / 4; i += 256) reinterpret_cast<uint4*>(part)[i] = make_uint4(0, 0, 0, 0);
+    } else if (warp >= 4) {
       const int token = q0 + static_cast<int>((warp & 3) * 32 + lane);
       if (token < p.L)
         zero_row(p.dq + batch * p.dq_stride_b + token * p.dq_stride_t + static_cast<int64_t>(head) * HD +
@@ -543,7 +591,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
         const int sk = j % DQ_K_STAGES, sv = j % B_STAGES;
         if (!mbar_wait(&st.a_empty[sk], ((j / DQ_K_STAGES) & 1) ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.a_full[sk], T_BYTES);
-        load_rows(k_tiles + sk * T_BYTES, tk, &st.a_full[sk], T_HALF_BYTES, kv_head, j * BT, batch);
+        load_rows(k_tiles + sk * T_BYTES, tk, &st.a_full[sk], T_HALF_BYTES, kv_head, (tile0 + j) * BT, batch);
         ++a_issued;
         if (j == 0) {  // behind what the first scores need
           mbar_arrive_expect_tx(&st.fixed_full[1], T_BYTES);
@@ -551,7 +599,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
         }
         if (!mbar_wait(&st.b_empty[sv], ((j / B_STAGES) & 1) ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.b_full[sv], T_BYTES);
-        load_rows(v_tiles + sv * T_BYTES, tv, &st.b_full[sv], T_HALF_BYTES, kv_head, j * BT, batch);
+        load_rows(v_tiles + sv * T_BYTES, tv, &st.b_full[sv], T_HALF_BYTES, kv_head, (tile0 + j) * BT, batch);
         ++b_issued;
       }
       if (*abort) {  // let the copies in flight land before the CTA exits
@@ -630,7 +678,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
     for (int j = 0; j < n; ++j) {
       const int b = j & 1;
       const uint32_t s_tmem = tmem + lane_off + b * 128 + g * 64;
-      const int valid = limit - j * BT - g * 64;  // columns of this thread's 64 that its query sees
+      const int valid = limit - (tile0 + j) * BT - g * 64;  // columns of this thread's 64 that its query sees
       const bool masked = __any_sync(0xffffffffu, valid < 64);
       if (!mbar_wait(&st.s_full[b], (j >> 1) & 1, abort)) {
         ok = false;
@@ -676,10 +724,70 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
     if (ok && mbar_wait(&st.done, 0, abort)) {
       tc_fence_after();
       const int token0 = q0 + static_cast<int>(quarter * 32);
-      store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale,
+      if (p.dq_splits > 1)
+        store_part(tmem + lane_off + 384 + g * 64, 64, part + quarter * 32 * HD + g * 64, lane);
+      else
+        store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale,
                  p.dq + batch * p.dq_stride_b + token0 * p.dq_stride_t + static_cast<int64_t>(head) * HD + g * 64,
                  p.dq_stride_t, p.L - token0, lane);
     }
+  }
+}
+
+// Adds the parts of shared sums: a CTA per 32 rows of a tile (dV and dK tiles, then dQ tiles).
+__global__ void __launch_bounds__(256) attn_bwd_join_kernel(const __grid_constant__ BwdParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int col = (threadIdx.x & 31) * 4;  // a thread takes 4 columns of every eighth row
+  const int row0 = (blockIdx.x & 3) * 32 + (threadIdx.x >> 5);
+  const unsigned tile = blockIdx.x >> 2;
+  const unsigned dkdv_tiles = p.dkdv_splits > 1 ? 2 * (p.dkdv_ctas / p.dkdv_splits) : 0;
+  const float* src;
+  __nv_bfloat16* dst;
+  int64_t part_stride, row_stride;
+  int splits, valid;
+  float scale = p.scale;
+  if (tile < dkdv_tiles) {
+    const unsigned idx = tile >> 1;
+    const bool is_dk = tile & 1;
+    const int k0 = static_cast<int>(idx % p.kv_tiles) * BT;
+    const int bh = static_cast<int>(idx / p.kv_tiles);
+    const int kv_head = bh % p.kv_heads, batch = bh / p.kv_heads;
+    splits = p.dkdv_splits;
+    part_stride = 2 * BT * HD;
+    src = p.dkdv_parts + static_cast<int64_t>(idx) * splits * part_stride + (is_dk ? BT * HD : 0);
+    row_stride = is_dk ? p.dk_stride_t : p.dv_stride_t;
+    dst = (is_dk ? p.dk + batch * p.dk_stride_b : p.dv + batch * p.dv_stride_b) + k0 * row_stride +
+          static_cast<int64_t>(kv_head) * HD;
+    valid = p.L_kv - k0;
+    if (!is_dk) scale = 1.f;
+  } else {
+    const unsigned idx = tile - dkdv_tiles;
+    const int q0 = (p.q_tiles - 1 - static_cast<int>(idx % p.q_tiles)) * BT;
+    const int bh = static_cast<int>(idx / p.q_tiles);
+    const int head = bh % p.heads, batch = bh / p.heads;
+    splits = p.dq_splits;
+    part_stride = BT * HD;
+    src = p.dq_parts + static_cast<int64_t>(idx) * splits * part_stride;
+    row_stride = p.dq_stride_t;
+    dst = p.dq + batch * p.dq_stride_b + q0 * row_stride + static_cast<int64_t>(head) * HD;
+    valid = p.L - q0;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = row0 + i * 8;
+    if (row >= valid) continue;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(src + k * part_stride + row * HD + col);
+      sum.x += v.x;
+      sum.y += v.y;
+      sum.z += v.z;
+      sum.w += v.w;
+    }
+    *reinterpret_cast<uint2*>(dst + row * row_stride + col) =
+        make_uint2(pack_bf16x2(sum.x * scale, sum.y * scale), pack_bf16x2(sum.z * scale, sum.w * scale));
   }
 }
 

@@ -1488,18 +1488,110 @@ bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0
 int64_t bwd_tiles(int64_t tokens) { return (tokens + ogx::attn::BT - 1) / ogx::attn::BT; }
 
 int64_t bwd_stats_bytes(int64_t batch, int64_t q_tokens, int64_t heads) {
-  return batch * heads * bwd_tiles(q_tokens) * ogx::attn::STAT_BYTES;
+  return batch * heads * bwd_tiles(q_tokens) * ogx::attn::STAT_FLOATS * 4;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int64_t kMaxSplits = 64;
+
+// CTAs per query block of the forward kernel.  In units of one 64-key tile, a CTA costs its tiles and about 8 more to
+// start and end; joining costs a launch, 6.  Few blocks over many keys are shared out until the waves of CTAs stop
+// getting shorter.  32 heads, us alone and shared: 1 query x 5000 keys 90 and 33, x 50000 832 and 201; 512 x 9216 136
+// and 86.
+int64_t fwd_splits(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads) {
+  const int64_t blocks = batch * heads * ceil_div(q_tokens, 256), tiles = ceil_div(kv_tokens, ogx::attn::BKV);
+  const int64_t sms = sm_count();
+  if (blocks >= 2 * sms) return 1;
+  int64_t best = 1, best_cost = ceil_div(blocks, sms) * (tiles + 8);
+  for (int64_t n = 2; n <= kMaxSplits && n * 4 <= tiles && batch * n <= 65535; ++n) {
+    const int64_t cost = ceil_div(blocks * n, sms) * (ceil_div(tiles, n) + 8) + 6;
+    if (cost < best_cost) {
+      best = n;
+      best_cost = cost;
+    }
+  }
+  return ceil_div(tiles, ceil_div(tiles, best));  // no split without a tile
+}
+
+int64_t fwd_part_rows(int64_t batch, int64_t q_tokens, int64_t heads, int64_t splits) {
+  return batch * heads * splits * q_tokens;
+}
+
+// CTAs per tile of the backward kernel's two roles.  Times are in units of one dQ tile pair (0.9 us): a CTA costs its
+// pairs and 6 more to start and store; a dK/dV pair costs 1.5, or 2.2 where its operands come from HBM, as for a CTA
+// whose tiles few others read.  The dK/dV CTAs start first, so the launch takes the longest of them, or an SM's share of
+// everything, or an SM's share of dK/dV and then the longest dQ sum; joining costs 10 and 2 per part.  Without causality,
+// us alone and as chosen here: 2304 x 2304 with 2 key/value heads of 16 queries each 417 and 226 (4 CTAs per dK/dV
+// tile), 28800 x 64, 16 heads 508 and 242 (4), 100 x 9216, 16 heads 133 and 89 (6 per dQ tile).
+void bwd_splits(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t* dkdv,
+                int64_t* dq) {
+  static const int64_t counts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kMaxSplits};
+  const double sms = static_cast<double>(sm_count());
+  const int64_t q_tiles = bwd_tiles(q_tokens), kv_tiles = bwd_tiles(kv_tokens);
+  const int64_t dkdv_len = q_tiles * (heads / kv_heads), dq_len = kv_tiles;  // tile pairs of an unshared sum
+  const double dkdv_sums = static_cast<double>(batch * kv_heads * kv_tiles);
+  const double dq_sums = static_cast<double>(batch * heads * q_tiles);
+  double best = 0;
+  *dkdv = *dq = 1;
+  for (int64_t a : counts) {
+    if (a > 1 && a * 2 > dkdv_len) break;
+    for (int64_t b : counts) {
+      if (b > 1 && b * 2 > dq_len) break;
+      const double dkdv_pairs = static_cast<double>(ceil_div(dkdv_len, a));
+      const double dq_pairs = static_cast<double>(ceil_div(dq_len, b));
+      const double first = dkdv_sums * a * (dkdv_pairs * 1.5 + 6) / sms;
+      const double all = first + dq_sums * b * (dq_pairs + 6) / sms;
+      double cost = std::max(std::max(dkdv_pairs * 2.2 + 6, all), first + dq_pairs + 6);
+      if (a == 1 && b == 1) {
+        best = cost;
+        if (cost == all) return;  // every SM has work to the end
+        continue;
+      }
+      cost += 10 + 2 * static_cast<double>((a > 1 ? a : 0) + (b > 1 ? b : 0));
+      if (cost < best) {
+        best = cost;
+        *dkdv = a;
+        *dq = b;
+      }
+    }
+  }
+}
+
+struct BwdWorkspace {
+  int64_t dkdv_splits, dq_splits;
+  int64_t dkdv_at, dq_at, bytes;  // the parts lie behind the statistics
+};
+
+BwdWorkspace bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads) {
+  BwdWorkspace w{};
+  bwd_splits(batch, q_tokens, kv_tokens, heads, kv_heads, &w.dkdv_splits, &w.dq_splits);
+  const int64_t tile = ogx::attn::BT * ogx::attn::HD * 4;
+  w.dkdv_at = bwd_stats_bytes(batch, q_tokens, heads);
+  w.dq_at = w.dkdv_at + (w.dkdv_splits > 1 ? batch * kv_heads * bwd_tiles(kv_tokens) * w.dkdv_splits * 2 * tile : 0);
+  w.bytes = w.dq_at + (w.dq_splits > 1 ? batch * heads * bwd_tiles(q_tokens) * w.dq_splits * tile : 0);
+  return w;
 }
 
 }  // namespace
 
 extern "C" {
 
+int ogx_attention_fwd_lse_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
+                                    int64_t* bytes) {
+  if (bytes == nullptr) return fail(OGX_EINVAL, "null_pointer");
+  if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1) return fail(OGX_EINVAL, "shape");
+  const int64_t splits = fwd_splits(batch, q_tokens, kv_tokens, heads);
+  *bytes = splits > 1 ? fwd_part_rows(batch, q_tokens, heads, splits) * (ogx::attn::HD + 2) * 4 : 0;
+  return OGX_OK;
+}
+
 int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
                           int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
                           int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b,
                           int64_t v_stride_t, float softmax_scale, int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
-                          int64_t out_stride_b, int64_t out_stride_t, float* lse, void* stream) {
+                          int64_t out_stride_b, int64_t out_stride_t, float* lse, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
   int rc = masked_attention_guard(q, k, v, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, q_stride_b,
                                   q_stride_t, k_stride_b, k_stride_t, v_stride_b, v_stride_t, softmax_scale,
                                   causal_block);
@@ -1508,6 +1600,10 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
     return fail(OGX_EINVAL, "output");
   if (lse == nullptr || !aligned4(lse)) return fail(OGX_EINVAL, "lse");
   if (!aligned4(q_lengths) || !aligned4(kv_lengths)) return fail(OGX_EINVAL, "lengths");
+  const int64_t splits = fwd_splits(batch, q_tokens, kv_tokens, heads);
+  const int64_t parts = fwd_part_rows(batch, q_tokens, heads, splits);
+  if (splits > 1 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < parts * (ogx::attn::HD + 2) * 4))
+    return fail(OGX_EINVAL, "workspace");
   CUtensorMap mq, mk, mv;
   if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BQ))) return rc;
   if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, k_stride_t, k_stride_b, ogx::attn::BKV))) return rc;
@@ -1527,17 +1623,37 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
   auto kern = ogx::attn::attn_fwd_kernel<false, true>;
   if ((rc = attn_register_split_ok(reinterpret_cast<const void*>(kern)))) return rc;
   if ((rc = ensure_smem(kern, ogx::attn::SMEM_BYTES))) return rc;
+  const int64_t tiles = ceil_div(kv_tokens, ogx::attn::BKV);
+  p.splits = static_cast<int>(splits);
+  p.split_tiles = static_cast<int>(ceil_div(tiles, splits));
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = splits > 1 ? reinterpret_cast<float2*>(p.part_o + parts * ogx::attn::HD) : nullptr;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>((q_tokens + 255) / 256), static_cast<unsigned>(heads),
-                  static_cast<unsigned>(batch));
-  launch(kern, grid, ogx::attn::kThreads, ogx::attn::SMEM_BYTES, static_cast<cudaStream_t>(stream), mq, mk, mv, p);
-  return check_launch("attn_fwd_kernel");
+                  static_cast<unsigned>(batch * splits));
+  launch(kern, grid, ogx::attn::kThreads, ogx::attn::SMEM_BYTES, s, mq, mk, mv, p);
+  if ((rc = check_launch("attn_fwd_kernel")) || splits == 1) return rc;
+  ogx::attn::JoinParams jp{};
+  jp.part_o = p.part_o;
+  jp.part_ml = p.part_ml;
+  jp.out = p.out;
+  jp.out_stride_b = out_stride_b;
+  jp.out_stride_t = out_stride_t;
+  jp.lse = lse;
+  jp.L = p.L;
+  jp.heads = static_cast<int>(heads);
+  jp.splits = p.splits;
+  jp.rows = batch * heads * q_tokens;
+  launch(ogx::attn::attn_join_kernel, dim3(static_cast<unsigned>(ceil_div(jp.rows, 8))), 256, 0, s, jp);
+  return check_launch("attn_join_kernel");
 }
 
 int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads,
                                 int64_t* bytes) {
   if (bytes == nullptr) return fail(OGX_EINVAL, "null_pointer");
   if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1 || kv_heads < 1) return fail(OGX_EINVAL, "shape");
-  *bytes = bwd_stats_bytes(batch, q_tokens, heads);
+  if (heads % kv_heads) return fail(OGX_EINVAL, "kv_heads: heads must be a multiple of kv_heads");
+  *bytes = bwd_workspace(batch, q_tokens, kv_tokens, heads, kv_heads).bytes;
   return OGX_OK;
 }
 
@@ -1566,10 +1682,11 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
       !row_strides_ok(kv_width, kv_tokens, batch, dk_stride_t, dk_stride_b) ||
       !row_strides_ok(kv_width, kv_tokens, batch, dv_stride_t, dv_stride_b))
     return fail(OGX_EINVAL, "gradients");
-  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < bwd_stats_bytes(batch, q_tokens, heads))
-    return fail(OGX_EINVAL, "workspace");
+  const BwdWorkspace ws = bwd_workspace(batch, q_tokens, kv_tokens, heads, kv_heads);
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < ws.bytes) return fail(OGX_EINVAL, "workspace");
   const int64_t q_tiles = bwd_tiles(q_tokens), kv_tiles = bwd_tiles(kv_tokens);
-  const int64_t dkdv_ctas = kv_tiles * kv_heads * batch, dq_ctas = q_tiles * heads * batch;
+  const int64_t dkdv_ctas = kv_tiles * kv_heads * batch * ws.dkdv_splits;
+  const int64_t dq_ctas = q_tiles * heads * batch * ws.dq_splits;
   if (dkdv_ctas + dq_ctas > INT32_MAX) return fail(OGX_EINVAL, "shape");
   CUtensorMap mq, mk, mv, mdo;
   if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BT))) return rc;
@@ -1609,6 +1726,10 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   p.q_tiles = static_cast<int>(q_tiles);
   p.kv_tiles = static_cast<int>(kv_tiles);
   p.dkdv_ctas = static_cast<unsigned>(dkdv_ctas);
+  p.dkdv_splits = static_cast<int>(ws.dkdv_splits);
+  p.dq_splits = static_cast<int>(ws.dq_splits);
+  p.dkdv_parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + ws.dkdv_at);
+  p.dq_parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + ws.dq_at);
   p.causal_block = static_cast<int>(causal_block);
   p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
@@ -1628,7 +1749,12 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   if ((rc = ensure_smem(kern, ogx::attn::BWD_SMEM))) return rc;
   launch(kern, dim3(static_cast<unsigned>(dkdv_ctas + dq_ctas)), ogx::attn::kBwdThreads, ogx::attn::BWD_SMEM, s, mq, mk,
          mv, mdo, p);
-  return check_launch("attn_bwd_kernel");
+  if ((rc = check_launch("attn_bwd_kernel"))) return rc;
+  const int64_t joined = (ws.dkdv_splits > 1 ? 2 * kv_tiles * kv_heads * batch : 0) +
+                         (ws.dq_splits > 1 ? q_tiles * heads * batch : 0);
+  if (joined == 0) return OGX_OK;
+  launch(ogx::attn::attn_bwd_join_kernel, dim3(static_cast<unsigned>(joined * 4)), 256, 0, s, p);
+  return check_launch("attn_bwd_join_kernel");
 }
 
 }  // extern "C"

@@ -33,7 +33,7 @@ def test_python_surface_refuses_cpu_tensors():
 # ogx_attention_fwd_lse arguments by name, a call that every guard accepts up to the tensor maps
 FWD = dict(q=16, k=16, v=16, batch=1, q_tokens=8, kv_tokens=8, heads=4, kv_heads=2, head_dim=128, q_stride_b=4096,
            q_stride_t=512, k_stride_b=2048, k_stride_t=256, v_stride_b=2048, v_stride_t=256, scale=0.1, causal_block=0, q_lengths=None, kv_lengths=None,
-           out=16, out_stride_b=4096, out_stride_t=512, lse=16, stream=None)
+           out=16, out_stride_b=4096, out_stride_t=512, lse=16, workspace=None, workspace_bytes=0, stream=None)
 
 
 @pytest.mark.parametrize("change,reason", [
@@ -68,6 +68,16 @@ BWD = dict(dout=16, q=16, k=16, v=16, out=16, lse=16, batch=1, q_tokens=8, kv_to
 def test_attention_gradient_entry_refusals(ogx_lib, change, reason):
     assert ogx_lib.ogx_attention_bwd(*{**BWD, **change}.values()) == -1
     assert _err(ogx_lib).split(":")[0] == reason
+
+
+def test_few_queries_over_many_keys_need_a_workspace(ogx_lib):
+    n = ctypes.c_int64(-1)
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(4, 9216, 9216, 32, ctypes.addressof(n)) == 0 and n.value == 0
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, 20000, 4, ctypes.addressof(n)) == 0 and n.value > 0
+    call = {**FWD, "q_tokens": 1, "kv_tokens": 20000, "workspace": 16, "workspace_bytes": n.value - 1}
+    assert ogx_lib.ogx_attention_fwd_lse(*call.values()) == -1 and _err(ogx_lib) == "workspace"
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 0, 20000, 4, ctypes.addressof(n)) == -1
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, 20000, 4, None) == -1
 
 
 def test_attention_gradient_workspace_size(ogx_lib):

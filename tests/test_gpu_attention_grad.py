@@ -101,6 +101,13 @@ CASES = [
     (1, 900, 900, 2, 2, 576, None, None),
     (1, 1300, 64, 2, 2, 0, (1290,), (63,)),
     (1, 64, 1300, 8, 1, 0, None, (1281,)),
+    # few tiles on one side: the sums over the other are shared by several CTAs and joined
+    (1, 1, 5000, 4, 2, 0, None, None),
+    (2, 3, 4000, 2, 1, 1, None, (3900, 70)),
+    (2, 130, 3333, 2, 2, 100, (130, 1), (3333, 1000)),
+    (1, 4000, 20, 4, 1, 0, (3950,), None),
+    (2, 5001, 130, 2, 2, 7, (5001, 3000), (130, 64)),
+    (1, 3000, 3000, 1, 1, 1, (2900,), (2950,)),
 ]
 
 
