@@ -380,7 +380,8 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
                           int64_t workspace_bytes, void* stream);
 
 /* Bytes of device workspace that ogx_attention_fwd_lse needs for these sizes on the current device. */
-int ogx_attention_fwd_lse_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t* bytes);
+int ogx_attention_fwd_lse_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
+                                    int64_t kv_heads, int64_t* bytes);
 
 /* Bytes of device workspace that ogx_attention_bwd needs for these sizes on the current device. */
 int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads,

@@ -139,7 +139,7 @@ _SIGNATURES: dict[str, list] = {
         c_int64, c_int64, c_int64, c_int64, c_float, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
         c_void_p, c_void_p, c_int64, c_void_p,
     ],
-    "ogx_attention_fwd_lse_workspace": [c_int64, c_int64, c_int64, c_int64, c_void_p],
+    "ogx_attention_fwd_lse_workspace": [c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p],
     "ogx_attention_bwd_workspace": [
         c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
     ],

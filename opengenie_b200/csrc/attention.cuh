@@ -27,6 +27,7 @@
 // the softmax, not the MMA chain, sets each tile's pace.  tcgen05.mma
 // operations issued by one thread execute in order, which makes writing
 // S_q(j+2) over P_q(j) safe.
+// With N = 1 a CTA has one Q tile, half the threads, TMEM and shared memory, and shares its SM with another.
 #pragma once
 
 #include "ogx_sm100.cuh"
@@ -48,7 +49,6 @@ constexpr int SMEM_BYTES = NQ * Q_TILE_BYTES + 2 * KV_STAGES * KV_TILE_BYTES + 1
 constexpr int kThreads = 384;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t TMEM_O = 0;      // + 128 * q
-constexpr uint32_t TMEM_S = 256;    // + 128 * q + 64 * buffer
 // A row's running max only moves when a new score exceeds it by more than
 // this many log2 units, so P <= 2^8 and most key tiles need no O rescale.
 constexpr float kRescaleThreshold = 8.0f;
@@ -60,6 +60,13 @@ constexpr int kLaunchRegs = 168;
 constexpr uint32_t kRegsProducer = 96;
 constexpr uint32_t kRegsSoftmax = 200;
 static_assert(128 * kRegsProducer + 256 * kRegsSoftmax <= kThreads * kLaunchRegs, "register split exceeds the launch");
+// The form with one Q tile per CTA and two CTAs per SM: half the threads, TMEM and shared memory.
+constexpr int KV_STAGES_ONE = 2;
+constexpr int SMEM_BYTES_ONE = Q_TILE_BYTES + 2 * KV_STAGES_ONE * KV_TILE_BYTES + 1024;
+constexpr int kThreadsOne = 256;
+constexpr int kLaunchRegsOne = 128;
+constexpr uint32_t kRegsProducerOne = 56;
+static_assert(128 * kRegsProducerOne + 128 * kRegsSoftmax <= kThreadsOne * kLaunchRegsOne, "register split exceeds the launch");
 
 struct Params {
   int L;             // query tokens
@@ -76,7 +83,9 @@ struct Params {
   int peer_tokens;
   // MASKED kernels only (Visibility below has the masks' meaning)
   float* lse;                  // [batch, heads, L]: natural log of each row's sum of exponentials
+  int heads;
   int heads_per_kv;            // query heads that share a key/value head
+  int pack_shift;              // 2^pack_shift of these make a Q tile's rows together: row = token << pack_shift | head
   int causal_block;            // 0: every key is visible
   const int* q_lengths;        // [batch] or null
   const int* kv_lengths;       // [batch] or null
@@ -214,38 +223,41 @@ __device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* map, 
 
 // MASKED adds per-batch lengths, a block-causal mask, shared key/value heads and the softmax statistics that
 // the backward pass reads (bf16 output only); without it the code is the dense kernel's.
-template <bool OUT_E4M3, bool MASKED = false>
-__global__ void __launch_bounds__(kThreads, 1)
+template <bool OUT_E4M3, bool MASKED = false, int N = NQ>
+__global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 : 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                     const __grid_constant__ CUtensorMap tv, Params p) {
   pdl_trigger();
+  constexpr int STAGES = N == NQ ? KV_STAGES : KV_STAGES_ONE;
+  constexpr uint32_t T_S = 128 * N;  // TMEM: O tiles first, then two score buffers each
   extern __shared__ uint8_t smem_raw[];
   __shared__ SharedState st;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
   // [Q0][Q1][K stages][V stages]
   uint8_t* q_tiles = smem;
-  uint8_t* k_tiles = smem + NQ * Q_TILE_BYTES;
-  uint8_t* v_tiles = k_tiles + KV_STAGES * KV_TILE_BYTES;
+  uint8_t* k_tiles = smem + N * Q_TILE_BYTES;
+  uint8_t* v_tiles = k_tiles + STAGES * KV_TILE_BYTES;
 
   const uint32_t warp = warp_idx();
   const uint32_t lane = threadIdx.x & 31;
-  const int head = blockIdx.y;
+  const int head = MASKED ? blockIdx.y << p.pack_shift : blockIdx.y;  // the block's first head
   const int batch = MASKED ? blockIdx.z / p.splits : blockIdx.z;
   const int split = MASKED ? blockIdx.z % p.splits : 0;
   // causal rows get longer with their index: the longest blocks start first
-  const int q_block0 = (MASKED ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * (NQ * BQ);
+  const int block_tokens = MASKED ? (N * BQ) >> p.pack_shift : N * BQ;
+  const int q_block0 = (MASKED ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * block_tokens;
   const int kv_head = MASKED ? head / p.heads_per_kv : head;
 
   if (threadIdx.x == 0) {
     mbar_init(&st.q_full, 1);
-    for (int s = 0; s < KV_STAGES; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(&st.k_full[s], 1);
       mbar_init(&st.k_empty[s], 1);
       mbar_init(&st.v_full[s], 1);
       mbar_init(&st.v_empty[s], 1);
     }
-    for (int q = 0; q < NQ; ++q) {
+    for (int q = 0; q < N; ++q) {
       for (int b = 0; b < 2; ++b) {
         mbar_init(&st.s_full[q][b], 1);
         mbar_init(&st.p_full[q][b], 128);
@@ -262,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&st.tmem_base, TMEM_COLS);
+    tmem_alloc(&st.tmem_base, 256 * N);
     tmem_relinquish();
   }
   pdl_wait();  // everything above touches only this CTA's shared memory and TMEM
@@ -273,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if constexpr (MASKED) {
     vis = Visibility{clamp_length(p.q_lengths, batch, p.L), clamp_length(p.kv_lengths, batch, p.L_kv), p.causal_block,
                      p.L_kv - p.L};
-    const int last = min(q_block0 + NQ * BQ, vis.q_len) - 1;  // limit() grows with the row
+    const int last = min(q_block0 + block_tokens, vis.q_len) - 1;  // limit() grows with the row
     nkv = last < q_block0 ? 0 : (vis.limit(last) + BKV - 1) / BKV;
     nkv = min(max(nkv - tile0, 0), p.split_tiles);
     const int border = vis.kv_len / BKV - tile0;
@@ -286,13 +298,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort = &st.abort;
 
   if (warp < 4) {
-    reg_dealloc<kRegsProducer>();
+    reg_dealloc<N == NQ ? kRegsProducer : kRegsProducerOne>();
     if (MASKED && nkv == 0) {
       // no row of this block sees a key: nothing to load or multiply
     } else if (MASKED && warp == 2 && fix_tile >= 0) {
       if (mbar_wait(&st.v_fix_request, 0, abort) &&
-          mbar_wait(&st.v_full[fix_tile % KV_STAGES], (fix_tile / KV_STAGES) & 1, abort)) {
-        zero_rows(v_tiles + (fix_tile % KV_STAGES) * KV_TILE_BYTES, KV_HALF_BYTES, vis.kv_len % BKV, BKV, lane);
+          mbar_wait(&st.v_full[fix_tile % STAGES], (fix_tile / STAGES) & 1, abort)) {
+        zero_rows(v_tiles + (fix_tile % STAGES) * KV_TILE_BYTES, KV_HALF_BYTES, vis.kv_len % BKV, BKV, lane);
         fence_async_shared();
       }
       __syncwarp();
@@ -302,13 +314,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_prefetch_desc(&tq);
       tma_prefetch_desc(&tk);
       tma_prefetch_desc(&tv);
-      mbar_arrive_expect_tx(&st.q_full, NQ * Q_TILE_BYTES);
-      for (int q = 0; q < NQ; ++q)
-        load_rows(q_tiles + q * Q_TILE_BYTES, &tq, &st.q_full, Q_HALF_BYTES, head, q_block0 + q * BQ, batch);
+      mbar_arrive_expect_tx(&st.q_full, N * Q_TILE_BYTES);
+      for (int q = 0; q < N; ++q)
+        load_rows(q_tiles + q * Q_TILE_BYTES, &tq, &st.q_full, Q_HALF_BYTES, head,
+                  q_block0 + (MASKED ? q * BQ >> p.pack_shift : q * BQ), batch);
       int issued = 0;  // K/V tile loads issued (K of tile j is 2j, V is 2j+1)
       for (int j = 0; j < nkv; ++j) {
-        const int s = j % KV_STAGES;
-        const uint32_t ph = (j / KV_STAGES) & 1;
+        const int s = j % STAGES;
+        const uint32_t ph = (j / STAGES) & 1;
         if (!mbar_wait(&st.k_empty[s], ph ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.k_full[s], KV_TILE_BYTES);
         load_rows(k_tiles + s * KV_TILE_BYTES, &tk, &st.k_full[s], KV_HALF_BYTES, kv_head, (tile0 + j) * BKV, batch);
@@ -322,9 +335,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // let the copies already in flight land before the CTA exits
         mbar_wait(&st.q_full, 0, nullptr);
         const int last_j = (issued - 1) / 2;
-        for (int j = last_j; j >= 0 && j > last_j - KV_STAGES; --j) {
-          const int s = j % KV_STAGES;
-          const uint32_t ph = (j / KV_STAGES) & 1;
+        for (int j = last_j; j >= 0 && j > last_j - STAGES; --j) {
+          const int s = j % STAGES;
+          const uint32_t ph = (j / STAGES) & 1;
           mbar_wait(&st.k_full[s], ph, nullptr);
           if (2 * j + 1 < issued) mbar_wait(&st.v_full[s], ph, nullptr);
         }
@@ -338,8 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t v_addr = smem_u32(v_tiles);
       auto issue_s = [&](int q, int j) {  // S_q(j) into score buffer j % 2
         const uint32_t qa = q_addr + q * Q_TILE_BYTES;
-        const uint32_t ka = k_addr + (j % KV_STAGES) * KV_TILE_BYTES;
-        const uint32_t d = tmem + TMEM_S + q * 128 + (j & 1) * 64;
+        const uint32_t ka = k_addr + (j % STAGES) * KV_TILE_BYTES;
+        const uint32_t d = tmem + T_S + q * 128 + (j & 1) * 64;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t qoff = (kk >> 2) * Q_HALF_BYTES + (kk & 3) * 32;
@@ -350,8 +363,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit(&st.s_full[q][j & 1]);
       };
       auto issue_pv = [&](int q, int j) {  // O_q += P_q(j) V(j)
-        const uint32_t va = v_addr + (j % KV_STAGES) * KV_TILE_BYTES;
-        const uint32_t pa = tmem + TMEM_S + q * 128 + (j & 1) * 64;
+        const uint32_t va = v_addr + (j % STAGES) * KV_TILE_BYTES;
+        const uint32_t pa = tmem + T_S + q * 128 + (j & 1) * 64;
 #pragma unroll
         for (int kk = 0; kk < BKV / 16; ++kk) {
           mma_f16_ts(tmem + TMEM_O + q * 128, pa + kk * 8, make_sdesc_sw128(va + kk * 2048, KV_HALF_BYTES, 1024),
@@ -363,19 +376,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = mbar_wait(&st.q_full, 0, abort);
       // prologue: the scores of key tiles 0 and 1
       for (int j = 0; j < 2 && j < nkv && ok; ++j) {
-        const int s = j % KV_STAGES;
-        if (!mbar_wait(&st.k_full[s], (j / KV_STAGES) & 1, abort)) { ok = false; break; }
+        const int s = j % STAGES;
+        if (!mbar_wait(&st.k_full[s], (j / STAGES) & 1, abort)) { ok = false; break; }
         tc_fence_after();
         issue_s(0, j);
-        issue_s(1, j);
+        if constexpr (N > 1) issue_s(1, j);
         mma_commit(&st.k_empty[s]);
       }
       for (int j = 0; j < nkv && ok; ++j) {
-        const int s = j % KV_STAGES;
-        const uint32_t ph = (j / KV_STAGES) & 1;
+        const int s = j % STAGES;
+        const uint32_t ph = (j / STAGES) & 1;
         const uint32_t pph = (j >> 1) & 1;
         const int j2 = j + 2;
-        const int s2 = j2 % KV_STAGES;
+        const int s2 = j2 % STAGES;
         if (!mbar_wait(&st.v_full[s], ph, abort) || !mbar_wait(&st.p_full[0][j & 1], pph, abort)) { ok = false; break; }
         if (MASKED && j == fix_tile) {
           mbar_arrive(&st.v_fix_request);
@@ -384,16 +397,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         issue_pv(0, j);
         if (j2 < nkv) {
-          if (!mbar_wait(&st.k_full[s2], (j2 / KV_STAGES) & 1, abort)) { ok = false; break; }
+          if (!mbar_wait(&st.k_full[s2], (j2 / STAGES) & 1, abort)) { ok = false; break; }
           tc_fence_after();
           issue_s(0, j2);
         }
-        if (!mbar_wait(&st.p_full[1][j & 1], pph, abort)) { ok = false; break; }
-        tc_fence_after();
-        issue_pv(1, j);
+        if constexpr (N > 1) {
+          if (!mbar_wait(&st.p_full[1][j & 1], pph, abort)) { ok = false; break; }
+          tc_fence_after();
+          issue_pv(1, j);
+        }
         mma_commit(&st.v_empty[s]);
         if (j2 < nkv) {
-          issue_s(1, j2);
+          if constexpr (N > 1) issue_s(1, j2);
           mma_commit(&st.k_empty[s2]);
         }
       }
@@ -412,11 +427,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m_run = -INFINITY;  // running max, already multiplied by c
     float l_run = 0.f;
     bool ok = true;
+    const int token = q_block0 + (MASKED ? (q * BQ + row) >> p.pack_shift : q * BQ + row);
     // visible keys from this CTA's first one on
-    const int limit = MASKED ? vis.limit(q_block0 + q * BQ + row) - tile0 * BKV : p.L_kv;
+    const int limit = MASKED ? vis.limit(token) - tile0 * BKV : p.L_kv;
     for (int j = 0; j < nkv; ++j) {
       const int b = j & 1;
-      const uint32_t s_tmem = tmem + lane_off + TMEM_S + q * 128 + b * 64;
+      const uint32_t s_tmem = tmem + lane_off + T_S + q * 128 + b * 64;
       if (!mbar_wait(&st.s_full[q][b], (j >> 1) & 1, abort)) { ok = false; break; }
       tc_fence_after();
       uint32_t sr[64];
@@ -493,26 +509,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       mbar_arrive(&st.p_full[q][b]);
     }
+    // this row's head, and its place among the rows of [batch][heads][L]
+    const int row_head = MASKED ? head + (row & ((1 << p.pack_shift) - 1)) : head;
+    const int64_t batch_head = static_cast<int64_t>(batch) * p.heads + row_head;
     if (MASKED && nkv == 0) {
-      const int token = q_block0 + q * BQ + row;
       if (token < p.L && p.splits > 1) {
-        p.part_ml[((static_cast<int64_t>(batch) * gridDim.y + head) * p.splits + split) * p.L + token] =
-            make_float2(-INFINITY, 0.f);
+        p.part_ml[(batch_head * p.splits + split) * p.L + token] = make_float2(-INFINITY, 0.f);
       } else if (token < p.L) {
         uint4* dst = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(batch) * p.out_stride_b +
                                               static_cast<int64_t>(token) * p.out_stride_t +
-                                              static_cast<int64_t>(head) * HD);
+                                              static_cast<int64_t>(row_head) * HD);
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
-        p.lse[(static_cast<int64_t>(batch) * gridDim.y + head) * p.L + token] = -INFINITY;
+        p.lse[batch_head * p.L + token] = -INFINITY;
       }
     } else if (ok && mbar_wait(&st.o_done[q], 0, abort)) {
       tc_fence_after();
-      const int token = q_block0 + q * BQ + row;
       const float inv_l = 1.f / l_run;
       if constexpr (MASKED) {
         if (p.splits > 1) {
-          const int64_t at = ((static_cast<int64_t>(batch) * gridDim.y + head) * p.splits + split) * p.L + token;
+          const int64_t at = (batch_head * p.splits + split) * p.L + token;
           if (token < p.L) p.part_ml[at] = limit <= 0 ? make_float2(-INFINITY, 0.f) : make_float2(m_run, l_run);
 #pragma unroll 1
           for (int oc = 0; oc < 4; ++oc) {
@@ -527,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         } else if (token < p.L)
-          p.lse[(static_cast<int64_t>(batch) * gridDim.y + head) * p.L + token] =
+          p.lse[batch_head * p.L + token] =
               limit <= 0 ? -INFINITY : (m_run + log2f(l_run)) * 0.6931471805599453f;
       }
       if constexpr (OUT_E4M3) {
@@ -591,8 +607,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_wait();
           if (token < p.L) {
             const int64_t base = static_cast<int64_t>(batch) * p.out_stride_b +
-                                 static_cast<int64_t>(token) * p.out_stride_t + static_cast<int64_t>(head) * HD +
-                                 oc * 32;
+                                 static_cast<int64_t>(token) * p.out_stride_t +
+                                 static_cast<int64_t>(row_head) * HD + oc * 32;
 #pragma unroll
             for (int v8 = 0; v8 < 4; ++v8) {
               float f[8];
@@ -612,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, TMEM_COLS);
+    tmem_dealloc(tmem, 256 * N);
   }
 }
 

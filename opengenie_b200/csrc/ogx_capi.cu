@@ -7,6 +7,7 @@
 
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -913,7 +914,7 @@ int attention_common(const void* q, const void* k, const void* v, int64_t batch,
 
 // The softmax warpgroups raise their register limit with setmaxnreg, drawing on the registers the
 // launch reserved; only launch a build whose per-thread count is the one the split was sized for.
-int attn_register_split_ok(const void* kern) {
+int attn_register_split_ok(const void* kern, int regs = ogx::attn::kLaunchRegs) {
   static std::mutex mu;
   static std::unordered_map<const void*, bool> checked;  // a kernel's register count does not change
   std::lock_guard<std::mutex> lock(mu);
@@ -921,9 +922,8 @@ int attn_register_split_ok(const void* kern) {
   cudaFuncAttributes attr;
   int rc = check_cuda(cudaFuncGetAttributes(&attr, kern), "cudaFuncGetAttributes");
   if (rc) return rc;
-  if (attr.numRegs != ogx::attn::kLaunchRegs)
-    return fail(OGX_ECUDA, "attention kernel built with %d registers per thread, the register split needs %d", attr.numRegs,
-                ogx::attn::kLaunchRegs);
+  if (attr.numRegs != regs)
+    return fail(OGX_ECUDA, "attention kernel built with %d registers per thread, the register split needs %d", attr.numRegs, regs);
   checked[kern] = true;
   return OGX_OK;
 }
@@ -1447,11 +1447,11 @@ namespace {
 
 // {d, head, token, batch} map of bf16 rows of heads * 128 columns; a box is 64 columns of `box_rows` tokens.
 int token_map(CUtensorMap* map, const void* base, int64_t heads, int64_t tokens, int64_t batch, int64_t stride_t,
-              int64_t stride_b, int box_rows) {
+              int64_t stride_b, int box_rows, int box_heads = 1) {
   const uint64_t dims[4] = {128, static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens),
                             static_cast<uint64_t>(batch)};
   const uint64_t strides[3] = {256, static_cast<uint64_t>(stride_t) * 2, static_cast<uint64_t>(stride_b) * 2};
-  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(box_rows), 1};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(box_heads), static_cast<uint32_t>(box_rows), 1};
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box);
 }
 
@@ -1495,23 +1495,46 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 constexpr int64_t kMaxSplits = 64;
 
-// CTAs per query block of the forward kernel.  In units of one 64-key tile, a CTA costs its tiles and about 8 more to
-// start and end; joining costs a launch, 6.  Few blocks over many keys are shared out until the waves of CTAs stop
-// getting shorter.  32 heads, us alone and shared: 1 query x 5000 keys 90 and 33, x 50000 832 and 201; 512 x 9216 136
-// and 86.
-int64_t fwd_splits(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads) {
-  const int64_t blocks = batch * heads * ceil_div(q_tokens, 256), tiles = ceil_div(kv_tokens, ogx::attn::BKV);
-  const int64_t sms = sm_count();
-  if (blocks >= 2 * sms) return 1;
-  int64_t best = 1, best_cost = ceil_div(blocks, sms) * (tiles + 8);
-  for (int64_t n = 2; n <= kMaxSplits && n * 4 <= tiles && batch * n <= 65535; ++n) {
-    const int64_t cost = ceil_div(blocks * n, sms) * (ceil_div(tiles, n) + 8) + 6;
-    if (cost < best_cost) {
-      best = n;
-      best_cost = cost;
+// The forward kernel's form and the CTAs that share a query block's keys.  Two Q tiles per CTA read each key tile once
+// for 256 queries; one tile per CTA, two CTAs per SM, wastes less on an odd or single tile and hides a CTA's start and
+// end behind the other's products, but the key tiles then come through L2 twice as often.  In units of a 64-key tile
+// of the first form (0.9 us) a CTA costs its tiles and 6.4 to start and end; in the second form its tiles cost 1.32
+// each, or 0.6 when no other CTA is on the SM; joining shared blocks costs a launch, 6.  Measured at 32 heads, us with
+// two tiles and one: 4736 x 256 45.6 and 37.3, 4736 x 2048 173 and 177, 9216 x 9216 1130 and 1345; without and with
+// sharing: 512 x 9216 136 and 86.
+// A power of two of query heads with the same key/value head stand together in a Q tile, token by token, so that their
+// keys are read once and a causal tile spans fewer tokens.  With 32 heads on 8, us apart and together: 1 x 50,000 120
+// and 71 (832 unshared in the first form), causal 9216 641 and 564.
+struct FwdPlan {
+  bool one;
+  int pack_shift;
+  int64_t splits;
+};
+
+FwdPlan fwd_plan(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads) {
+  const int64_t tiles = ceil_div(kv_tokens, ogx::attn::BKV), sms = sm_count();
+  FwdPlan best{};
+  int shift = 0;
+  while (shift < 7 && (int64_t{1} << shift) < heads / kv_heads) ++shift;
+  if ((int64_t{1} << shift) != heads / kv_heads) shift = 0;
+  const int64_t rows = q_tokens << shift;  // of a head's or packed group's Q tiles
+  double best_cost = 0;
+  for (int form = 0; form < 2; ++form) {
+    const bool one = form == 1;
+    const int64_t blocks = batch * (heads >> shift) * ceil_div(rows, one ? 128 : 256), slots = one ? 2 * sms : sms;
+    for (int64_t n = 1; n <= kMaxSplits && (n == 1 || (n * 4 <= tiles && blocks * (n - 1) < 2 * slots && batch * n <= 65535));
+         ++n) {
+      const double tile = !one ? 1.0 : (blocks * n <= sms ? 0.6 : 1.32);
+      const double cost = static_cast<double>(ceil_div(blocks * n, slots)) * (ceil_div(tiles, n) * tile + 6.4) +
+                          (n > 1 ? 6 : 0);
+      if ((n == 1 && !one) || cost < best_cost) {
+        best = FwdPlan{one, shift, n};
+        best_cost = cost;
+      }
     }
   }
-  return ceil_div(tiles, ceil_div(tiles, best));  // no split without a tile
+  best.splits = ceil_div(tiles, ceil_div(tiles, best.splits));  // no split without a tile
+  return best;
 }
 
 int64_t fwd_part_rows(int64_t batch, int64_t q_tokens, int64_t heads, int64_t splits) {
@@ -1578,10 +1601,11 @@ BwdWorkspace bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, i
 extern "C" {
 
 int ogx_attention_fwd_lse_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
-                                    int64_t* bytes) {
+                                    int64_t kv_heads, int64_t* bytes) {
   if (bytes == nullptr) return fail(OGX_EINVAL, "null_pointer");
-  if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1) return fail(OGX_EINVAL, "shape");
-  const int64_t splits = fwd_splits(batch, q_tokens, kv_tokens, heads);
+  if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1 || kv_heads < 1) return fail(OGX_EINVAL, "shape");
+  if (heads % kv_heads) return fail(OGX_EINVAL, "kv_heads: heads must be a multiple of kv_heads");
+  const int64_t splits = fwd_plan(batch, q_tokens, kv_tokens, heads, kv_heads).splits;
   *bytes = splits > 1 ? fwd_part_rows(batch, q_tokens, heads, splits) * (ogx::attn::HD + 2) * 4 : 0;
   return OGX_OK;
 }
@@ -1600,12 +1624,14 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
     return fail(OGX_EINVAL, "output");
   if (lse == nullptr || !aligned4(lse)) return fail(OGX_EINVAL, "lse");
   if (!aligned4(q_lengths) || !aligned4(kv_lengths)) return fail(OGX_EINVAL, "lengths");
-  const int64_t splits = fwd_splits(batch, q_tokens, kv_tokens, heads);
+  const FwdPlan plan = fwd_plan(batch, q_tokens, kv_tokens, heads, kv_heads);
+  const int64_t splits = plan.splits;
   const int64_t parts = fwd_part_rows(batch, q_tokens, heads, splits);
   if (splits > 1 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < parts * (ogx::attn::HD + 2) * 4))
     return fail(OGX_EINVAL, "workspace");
   CUtensorMap mq, mk, mv;
-  if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BQ))) return rc;
+  const int pack = 1 << plan.pack_shift;
+  if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BQ / pack, pack))) return rc;
   if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, k_stride_t, k_stride_b, ogx::attn::BKV))) return rc;
   if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, v_stride_t, v_stride_b, ogx::attn::BKV))) return rc;
   ogx::attn::Params p{};
@@ -1616,22 +1642,28 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
   p.out_stride_b = out_stride_b;
   p.out_stride_t = out_stride_t;
   p.lse = lse;
+  p.heads = static_cast<int>(heads);
   p.heads_per_kv = static_cast<int>(heads / kv_heads);
+  p.pack_shift = plan.pack_shift;
   p.causal_block = static_cast<int>(causal_block);
   p.q_lengths = q_lengths;
   p.kv_lengths = kv_lengths;
-  auto kern = ogx::attn::attn_fwd_kernel<false, true>;
-  if ((rc = attn_register_split_ok(reinterpret_cast<const void*>(kern)))) return rc;
-  if ((rc = ensure_smem(kern, ogx::attn::SMEM_BYTES))) return rc;
+  const bool one = plan.one;
+  auto kern = one ? ogx::attn::attn_fwd_kernel<false, true, 1> : ogx::attn::attn_fwd_kernel<false, true>;
+  const int smem = one ? ogx::attn::SMEM_BYTES_ONE : ogx::attn::SMEM_BYTES;
+  if ((rc = attn_register_split_ok(reinterpret_cast<const void*>(kern),
+                                   one ? ogx::attn::kLaunchRegsOne : ogx::attn::kLaunchRegs)))
+    return rc;
+  if ((rc = ensure_smem(kern, smem))) return rc;
   const int64_t tiles = ceil_div(kv_tokens, ogx::attn::BKV);
   p.splits = static_cast<int>(splits);
   p.split_tiles = static_cast<int>(ceil_div(tiles, splits));
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = splits > 1 ? reinterpret_cast<float2*>(p.part_o + parts * ogx::attn::HD) : nullptr;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>((q_tokens + 255) / 256), static_cast<unsigned>(heads),
+  const dim3 grid(static_cast<unsigned>(ceil_div(q_tokens * pack, one ? 128 : 256)), static_cast<unsigned>(heads / pack),
                   static_cast<unsigned>(batch * splits));
-  launch(kern, grid, ogx::attn::kThreads, ogx::attn::SMEM_BYTES, s, mq, mk, mv, p);
+  launch(kern, grid, one ? ogx::attn::kThreadsOne : ogx::attn::kThreads, smem, s, mq, mk, mv, p);
   if ((rc = check_launch("attn_fwd_kernel")) || splits == 1) return rc;
   ogx::attn::JoinParams jp{};
   jp.part_o = p.part_o;

@@ -1166,7 +1166,7 @@ def attention_with_lse(
     else:
         out_rows = _given_rows(out, q, "out_shape: out must be bf16 [B, L, heads*128] with unit column stride")
     lse = q.new_empty((B, heads, L), dtype=torch.float32)
-    size = _workspace_bytes("ogx_attention_fwd_lse_workspace", q.device.index, B, L, k.shape[1], heads)
+    size = _workspace_bytes("ogx_attention_fwd_lse_workspace", q.device.index, B, L, k.shape[1], heads, kv_heads)
     workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
     _call_on(
         q.device, "ogx_attention_fwd_lse", q.data_ptr(), k.data_ptr(), v.data_ptr(), B, L, k.shape[1], heads, kv_heads,

@@ -72,12 +72,13 @@ def test_attention_gradient_entry_refusals(ogx_lib, change, reason):
 
 def test_few_queries_over_many_keys_need_a_workspace(ogx_lib):
     n = ctypes.c_int64(-1)
-    assert ogx_lib.ogx_attention_fwd_lse_workspace(4, 9216, 9216, 32, ctypes.addressof(n)) == 0 and n.value == 0
-    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, 20000, 4, ctypes.addressof(n)) == 0 and n.value > 0
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(4, 9216, 9216, 32, 32, ctypes.addressof(n)) == 0 and n.value == 0
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, 20000, 4, 4, ctypes.addressof(n)) == 0 and n.value > 0
     call = {**FWD, "q_tokens": 1, "kv_tokens": 20000, "workspace": 16, "workspace_bytes": n.value - 1}
     assert ogx_lib.ogx_attention_fwd_lse(*call.values()) == -1 and _err(ogx_lib) == "workspace"
-    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 0, 20000, 4, ctypes.addressof(n)) == -1
-    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, 20000, 4, None) == -1
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 0, 20000, 4, 4, ctypes.addressof(n)) == -1
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, 20000, 4, 3, ctypes.addressof(n)) == -1
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, 20000, 4, 4, None) == -1
 
 
 def test_attention_gradient_workspace_size(ogx_lib):

@@ -108,6 +108,12 @@ CASES = [
     (1, 4000, 20, 4, 1, 0, (3950,), None),
     (2, 5001, 130, 2, 2, 7, (5001, 3000), (130, 64)),
     (1, 3000, 3000, 1, 1, 1, (2900,), (2950,)),
+    # two, four, eight and 128 query heads of a key/value head in a Q tile, and groups that are no power of two
+    (3, 1, 700, 8, 2, 1, (1, 0, 1), (700, 64, 0)),
+    (2, 65, 190, 8, 1, 3, (64, 65), (190, 129)),
+    (1, 130, 130, 4, 2, 1, None, (97,)),
+    (2, 3, 300, 128, 1, 0, (3, 2), (300, 1)),
+    (1, 129, 140, 12, 2, 5, (127,), None),
 ]
 
 
