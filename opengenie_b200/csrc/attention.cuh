@@ -27,7 +27,6 @@
 // the softmax, not the MMA chain, sets each tile's pace.  tcgen05.mma
 // operations issued by one thread execute in order, which makes writing
 // S_q(j+2) over P_q(j) safe.
-// With N = 1 a CTA has one Q tile, half the threads, TMEM and shared memory, and shares its SM with another.
 #pragma once
 
 #include "ogx_sm100.cuh"
@@ -49,6 +48,7 @@ constexpr int SMEM_BYTES = NQ * Q_TILE_BYTES + 2 * KV_STAGES * KV_TILE_BYTES + 1
 constexpr int kThreads = 384;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t TMEM_O = 0;      // + 128 * q
+constexpr uint32_t TMEM_S = 256;    // + 128 * q + 64 * buffer
 // A row's running max only moves when a new score exceeds it by more than
 // this many log2 units, so P <= 2^8 and most key tiles need no O rescale.
 constexpr float kRescaleThreshold = 8.0f;
@@ -60,13 +60,6 @@ constexpr int kLaunchRegs = 168;
 constexpr uint32_t kRegsProducer = 96;
 constexpr uint32_t kRegsSoftmax = 200;
 static_assert(128 * kRegsProducer + 256 * kRegsSoftmax <= kThreads * kLaunchRegs, "register split exceeds the launch");
-// The form with one Q tile per CTA and two CTAs per SM: half the threads, TMEM and shared memory.
-constexpr int KV_STAGES_ONE = 2;
-constexpr int SMEM_BYTES_ONE = Q_TILE_BYTES + 2 * KV_STAGES_ONE * KV_TILE_BYTES + 1024;
-constexpr int kThreadsOne = 256;
-constexpr int kLaunchRegsOne = 128;
-constexpr uint32_t kRegsProducerOne = 56;
-static_assert(128 * kRegsProducerOne + 128 * kRegsSoftmax <= kThreadsOne * kLaunchRegsOne, "register split exceeds the launch");
 
 struct Params {
   int L;             // query tokens
@@ -81,57 +74,7 @@ struct Params {
   // over NVLink instead of out_q.
   uint8_t* out_peer[8];
   int peer_tokens;
-  // MASKED kernels only (Visibility below has the masks' meaning)
-  float* lse;                  // [batch, heads, L]: natural log of each row's sum of exponentials
-  int heads;
-  int heads_per_kv;            // query heads that share a key/value head
-  int pack_shift;              // 2^pack_shift of these make a Q tile's rows together: row = token << pack_shift | head
-  int causal_block;            // 0: every key is visible
-  const int* q_lengths;        // [batch] or null
-  const int* kv_lengths;       // [batch] or null
-  // few query blocks over many keys: `splits` CTAs share a block's key tiles (split_tiles each) and leave their
-  // unnormalised rows and row statistics, [batch][heads][splits][L] x (128 | max, sum), for attn_join_kernel
-  int splits, split_tiles;
-  float* part_o;
-  float2* part_ml;
 };
-
-// Which keys a query sees.  Queries from q_len on see none; keys from kv_len on are seen by none.  With
-// block > 0 the sequences end together: query i stands at position i + shift, shift = L_kv - L, and sees the
-// keys of its own block of `block` positions and of all earlier blocks (block 1: the token-causal mask; the
-// tokens of a latent frame: a frame-causal one).  Both forms below are prefixes, so a tile needs comparing
-// only at its border.
-struct Visibility {
-  int q_len, kv_len, block, shift;
-  // keys [0, limit) are visible to query i
-  __device__ __forceinline__ int limit(int i) const {
-    if (i >= q_len) return 0;
-    if (block == 0) return kv_len;
-    const int at = i + shift;
-    if (at < 0) return 0;
-    const int64_t end = static_cast<int64_t>(at) - at % block + block;
-    return end < kv_len ? static_cast<int>(end) : kv_len;
-  }
-  // queries [first(j), q_len) see key j < kv_len
-  __device__ __forceinline__ int first(int j) const { return block == 0 ? 0 : j - j % block - shift; }
-};
-
-__device__ __forceinline__ int clamp_length(const int* lengths, int batch, int full) {
-  if (lengths == nullptr) return full;
-  const int n = lengths[batch];
-  return n < 0 ? 0 : (n > full ? full : n);
-}
-
-// Zeroes rows [row0, rows) of a tile of 128-byte rows (both 64-column halves) that a TMA load wrote, by one
-// warp: rows past a sequence's length hold whatever the caller's memory holds there, and 0 * NaN in the
-// product that sums over these rows would reach every output.  The caller has waited for the load and
-// signals the MMA issuer afterwards.  (A 128-byte row stays its own 128 bytes under the swizzle.)
-__device__ __forceinline__ void zero_rows(uint8_t* tile, int half_bytes, int row0, int rows, uint32_t lane) {
-  for (int i = static_cast<int>(lane); i < (rows - row0) * 8; i += 32) {
-    *reinterpret_cast<uint4*>(tile + row0 * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-    *reinterpret_cast<uint4*>(tile + half_bytes + row0 * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-  }
-}
 
 struct SharedState {
   uint64_t q_full;
@@ -142,9 +85,6 @@ struct SharedState {
   uint64_t o_ready[NQ];    // completes once per PV_q(j)
   uint64_t o_done[NQ];     // the last PV_q completed
   uint64_t drained;
-  // MASKED: the MMA issuer asks warp 2 to zero the rows past the keys in the last V tile, and its answer.  (A
-  // warp that waited for that tile's load by parity alone could take an earlier load of the stage for it.)
-  uint64_t v_fix_request, v_fixed;
   uint32_t tmem_base;
   int abort;
 };
@@ -181,23 +121,6 @@ __device__ __forceinline__ f2 ex2_poly2(f2 x) {
             __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23))};
 }
 
-// The same with a degree-4 polynomial (fitted in the same way, max relative error 2.7e-6) where the sum of the
-// exponentials is itself a result: with the degree-3 one the statistics of short rows are 100 times further from
-// exact than 32-bit arithmetic is.
-__device__ __forceinline__ f2 ex2_poly2_sum(f2 x) {
-  const f2 magic{12582912.0f, 12582912.0f};
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
-  const f2 t = add2(x, magic);
-  const f2 f = sub2(x, sub2(t, magic));
-  f2 p = fma2(f2{0.0095701022f, 0.0095701022f}, f, f2{0.0559178591f, 0.0559178591f});
-  p = fma2(p, f, f2{0.2402474433f, 0.2402474433f});
-  p = fma2(p, f, f2{0.6931217909f, 0.6931217909f});
-  p = fma2(p, f, f2{0.9999992847f, 0.9999992847f});
-  return f2{__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-            __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23))};
-}
-
 // The same 2^x for one lane, in scalar instructions whose constants are immediates: no registers held for
 // them across a loop that keeps a whole row of scores live.
 __device__ __forceinline__ float ex2_poly(float x) {
@@ -221,43 +144,36 @@ __device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* map, 
   tma_load_4d(dst + half_bytes, map, bar, 64, head, row0, batch);
 }
 
-// MASKED adds per-batch lengths, a block-causal mask, shared key/value heads and the softmax statistics that
-// the backward pass reads (bf16 output only); without it the code is the dense kernel's.
-template <bool OUT_E4M3, bool MASKED = false, int N = NQ>
-__global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 : 2)
+template <bool OUT_E4M3>
+__global__ void __launch_bounds__(kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                     const __grid_constant__ CUtensorMap tv, Params p) {
   pdl_trigger();
-  constexpr int STAGES = N == NQ ? KV_STAGES : KV_STAGES_ONE;
-  constexpr uint32_t T_S = 128 * N;  // TMEM: O tiles first, then two score buffers each
   extern __shared__ uint8_t smem_raw[];
   __shared__ SharedState st;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
   // [Q0][Q1][K stages][V stages]
   uint8_t* q_tiles = smem;
-  uint8_t* k_tiles = smem + N * Q_TILE_BYTES;
-  uint8_t* v_tiles = k_tiles + STAGES * KV_TILE_BYTES;
+  uint8_t* k_tiles = smem + NQ * Q_TILE_BYTES;
+  uint8_t* v_tiles = k_tiles + KV_STAGES * KV_TILE_BYTES;
 
   const uint32_t warp = warp_idx();
   const uint32_t lane = threadIdx.x & 31;
-  const int head = MASKED ? blockIdx.y << p.pack_shift : blockIdx.y;  // the block's first head
-  const int batch = MASKED ? blockIdx.z / p.splits : blockIdx.z;
-  const int split = MASKED ? blockIdx.z % p.splits : 0;
-  // causal rows get longer with their index: the longest blocks start first
-  const int block_tokens = MASKED ? (N * BQ) >> p.pack_shift : N * BQ;
-  const int q_block0 = (MASKED ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * block_tokens;
-  const int kv_head = MASKED ? head / p.heads_per_kv : head;
+  const int head = blockIdx.y;
+  const int batch = blockIdx.z;
+  const int q_block0 = blockIdx.x * (NQ * BQ);
+  const int nkv = (p.L_kv + BKV - 1) / BKV;
 
   if (threadIdx.x == 0) {
     mbar_init(&st.q_full, 1);
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < KV_STAGES; ++s) {
       mbar_init(&st.k_full[s], 1);
       mbar_init(&st.k_empty[s], 1);
       mbar_init(&st.v_full[s], 1);
       mbar_init(&st.v_empty[s], 1);
     }
-    for (int q = 0; q < N; ++q) {
+    for (int q = 0; q < NQ; ++q) {
       for (int b = 0; b < 2; ++b) {
         mbar_init(&st.s_full[q][b], 1);
         mbar_init(&st.p_full[q][b], 128);
@@ -266,31 +182,14 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
       mbar_init(&st.o_done[q], 1);
     }
     mbar_init(&st.drained, 1);
-    if (MASKED) {
-      mbar_init(&st.v_fix_request, 1);
-      mbar_init(&st.v_fixed, 1);
-    }
     st.abort = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&st.tmem_base, 256 * N);
+    tmem_alloc(&st.tmem_base, TMEM_COLS);
     tmem_relinquish();
   }
   pdl_wait();  // everything above touches only this CTA's shared memory and TMEM
-  int nkv = (p.L_kv + BKV - 1) / BKV;
-  Visibility vis{};
-  int fix_tile = -1;  // the V tile whose last rows lie past the keys' length
-  const int tile0 = MASKED ? split * p.split_tiles : 0;  // this CTA's first key tile
-  if constexpr (MASKED) {
-    vis = Visibility{clamp_length(p.q_lengths, batch, p.L), clamp_length(p.kv_lengths, batch, p.L_kv), p.causal_block,
-                     p.L_kv - p.L};
-    const int last = min(q_block0 + block_tokens, vis.q_len) - 1;  // limit() grows with the row
-    nkv = last < q_block0 ? 0 : (vis.limit(last) + BKV - 1) / BKV;
-    nkv = min(max(nkv - tile0, 0), p.split_tiles);
-    const int border = vis.kv_len / BKV - tile0;
-    if (vis.kv_len < p.L_kv && vis.kv_len % BKV != 0 && border >= 0 && border < nkv) fix_tile = border;
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -298,46 +197,35 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
   volatile int* abort = &st.abort;
 
   if (warp < 4) {
-    reg_dealloc<N == NQ ? kRegsProducer : kRegsProducerOne>();
-    if (MASKED && nkv == 0) {
-      // no row of this block sees a key: nothing to load or multiply
-    } else if (MASKED && warp == 2 && fix_tile >= 0) {
-      if (mbar_wait(&st.v_fix_request, 0, abort) &&
-          mbar_wait(&st.v_full[fix_tile % STAGES], (fix_tile / STAGES) & 1, abort)) {
-        zero_rows(v_tiles + (fix_tile % STAGES) * KV_TILE_BYTES, KV_HALF_BYTES, vis.kv_len % BKV, BKV, lane);
-        fence_async_shared();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st.v_fixed);
-    } else if (warp == 0 && elect_one()) {
+    reg_dealloc<kRegsProducer>();
+    if (warp == 0 && elect_one()) {
       // ---------------------------------------------------------- TMA producer
       tma_prefetch_desc(&tq);
       tma_prefetch_desc(&tk);
       tma_prefetch_desc(&tv);
-      mbar_arrive_expect_tx(&st.q_full, N * Q_TILE_BYTES);
-      for (int q = 0; q < N; ++q)
-        load_rows(q_tiles + q * Q_TILE_BYTES, &tq, &st.q_full, Q_HALF_BYTES, head,
-                  q_block0 + (MASKED ? q * BQ >> p.pack_shift : q * BQ), batch);
+      mbar_arrive_expect_tx(&st.q_full, NQ * Q_TILE_BYTES);
+      for (int q = 0; q < NQ; ++q)
+        load_rows(q_tiles + q * Q_TILE_BYTES, &tq, &st.q_full, Q_HALF_BYTES, head, q_block0 + q * BQ, batch);
       int issued = 0;  // K/V tile loads issued (K of tile j is 2j, V is 2j+1)
       for (int j = 0; j < nkv; ++j) {
-        const int s = j % STAGES;
-        const uint32_t ph = (j / STAGES) & 1;
+        const int s = j % KV_STAGES;
+        const uint32_t ph = (j / KV_STAGES) & 1;
         if (!mbar_wait(&st.k_empty[s], ph ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.k_full[s], KV_TILE_BYTES);
-        load_rows(k_tiles + s * KV_TILE_BYTES, &tk, &st.k_full[s], KV_HALF_BYTES, kv_head, (tile0 + j) * BKV, batch);
+        load_rows(k_tiles + s * KV_TILE_BYTES, &tk, &st.k_full[s], KV_HALF_BYTES, head, j * BKV, batch);
         ++issued;
         if (!mbar_wait(&st.v_empty[s], ph ^ 1u, abort)) break;
         mbar_arrive_expect_tx(&st.v_full[s], KV_TILE_BYTES);
-        load_rows(v_tiles + s * KV_TILE_BYTES, &tv, &st.v_full[s], KV_HALF_BYTES, kv_head, (tile0 + j) * BKV, batch);
+        load_rows(v_tiles + s * KV_TILE_BYTES, &tv, &st.v_full[s], KV_HALF_BYTES, head, j * BKV, batch);
         ++issued;
       }
       if (*abort) {
         // let the copies already in flight land before the CTA exits
         mbar_wait(&st.q_full, 0, nullptr);
         const int last_j = (issued - 1) / 2;
-        for (int j = last_j; j >= 0 && j > last_j - STAGES; --j) {
-          const int s = j % STAGES;
-          const uint32_t ph = (j / STAGES) & 1;
+        for (int j = last_j; j >= 0 && j > last_j - KV_STAGES; --j) {
+          const int s = j % KV_STAGES;
+          const uint32_t ph = (j / KV_STAGES) & 1;
           mbar_wait(&st.k_full[s], ph, nullptr);
           if (2 * j + 1 < issued) mbar_wait(&st.v_full[s], ph, nullptr);
         }
@@ -351,8 +239,8 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
       const uint32_t v_addr = smem_u32(v_tiles);
       auto issue_s = [&](int q, int j) {  // S_q(j) into score buffer j % 2
         const uint32_t qa = q_addr + q * Q_TILE_BYTES;
-        const uint32_t ka = k_addr + (j % STAGES) * KV_TILE_BYTES;
-        const uint32_t d = tmem + T_S + q * 128 + (j & 1) * 64;
+        const uint32_t ka = k_addr + (j % KV_STAGES) * KV_TILE_BYTES;
+        const uint32_t d = tmem + TMEM_S + q * 128 + (j & 1) * 64;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t qoff = (kk >> 2) * Q_HALF_BYTES + (kk & 3) * 32;
@@ -363,8 +251,8 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
         mma_commit(&st.s_full[q][j & 1]);
       };
       auto issue_pv = [&](int q, int j) {  // O_q += P_q(j) V(j)
-        const uint32_t va = v_addr + (j % STAGES) * KV_TILE_BYTES;
-        const uint32_t pa = tmem + T_S + q * 128 + (j & 1) * 64;
+        const uint32_t va = v_addr + (j % KV_STAGES) * KV_TILE_BYTES;
+        const uint32_t pa = tmem + TMEM_S + q * 128 + (j & 1) * 64;
 #pragma unroll
         for (int kk = 0; kk < BKV / 16; ++kk) {
           mma_f16_ts(tmem + TMEM_O + q * 128, pa + kk * 8, make_sdesc_sw128(va + kk * 2048, KV_HALF_BYTES, 1024),
@@ -376,39 +264,33 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
       bool ok = mbar_wait(&st.q_full, 0, abort);
       // prologue: the scores of key tiles 0 and 1
       for (int j = 0; j < 2 && j < nkv && ok; ++j) {
-        const int s = j % STAGES;
-        if (!mbar_wait(&st.k_full[s], (j / STAGES) & 1, abort)) { ok = false; break; }
+        const int s = j % KV_STAGES;
+        if (!mbar_wait(&st.k_full[s], (j / KV_STAGES) & 1, abort)) { ok = false; break; }
         tc_fence_after();
         issue_s(0, j);
-        if constexpr (N > 1) issue_s(1, j);
+        issue_s(1, j);
         mma_commit(&st.k_empty[s]);
       }
       for (int j = 0; j < nkv && ok; ++j) {
-        const int s = j % STAGES;
-        const uint32_t ph = (j / STAGES) & 1;
+        const int s = j % KV_STAGES;
+        const uint32_t ph = (j / KV_STAGES) & 1;
         const uint32_t pph = (j >> 1) & 1;
         const int j2 = j + 2;
-        const int s2 = j2 % STAGES;
+        const int s2 = j2 % KV_STAGES;
         if (!mbar_wait(&st.v_full[s], ph, abort) || !mbar_wait(&st.p_full[0][j & 1], pph, abort)) { ok = false; break; }
-        if (MASKED && j == fix_tile) {
-          mbar_arrive(&st.v_fix_request);
-          if (!mbar_wait(&st.v_fixed, 0, abort)) { ok = false; break; }
-        }
         tc_fence_after();
         issue_pv(0, j);
         if (j2 < nkv) {
-          if (!mbar_wait(&st.k_full[s2], (j2 / STAGES) & 1, abort)) { ok = false; break; }
+          if (!mbar_wait(&st.k_full[s2], (j2 / KV_STAGES) & 1, abort)) { ok = false; break; }
           tc_fence_after();
           issue_s(0, j2);
         }
-        if constexpr (N > 1) {
-          if (!mbar_wait(&st.p_full[1][j & 1], pph, abort)) { ok = false; break; }
-          tc_fence_after();
-          issue_pv(1, j);
-        }
+        if (!mbar_wait(&st.p_full[1][j & 1], pph, abort)) { ok = false; break; }
+        tc_fence_after();
+        issue_pv(1, j);
         mma_commit(&st.v_empty[s]);
         if (j2 < nkv) {
-          if constexpr (N > 1) issue_s(1, j2);
+          issue_s(1, j2);
           mma_commit(&st.k_empty[s2]);
         }
       }
@@ -427,12 +309,9 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
     float m_run = -INFINITY;  // running max, already multiplied by c
     float l_run = 0.f;
     bool ok = true;
-    const int token = q_block0 + (MASKED ? (q * BQ + row) >> p.pack_shift : q * BQ + row);
-    // visible keys from this CTA's first one on
-    const int limit = MASKED ? vis.limit(token) - tile0 * BKV : p.L_kv;
     for (int j = 0; j < nkv; ++j) {
       const int b = j & 1;
-      const uint32_t s_tmem = tmem + lane_off + T_S + q * 128 + b * 64;
+      const uint32_t s_tmem = tmem + lane_off + TMEM_S + q * 128 + b * 64;
       if (!mbar_wait(&st.s_full[q][b], (j >> 1) & 1, abort)) { ok = false; break; }
       tc_fence_after();
       uint32_t sr[64];
@@ -440,8 +319,8 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
       tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
       tmem_ld_wait();
       float* sf = reinterpret_cast<float*>(sr);
-      const int kv_valid = limit - j * BKV;
-      if (MASKED ? __any_sync(0xffffffffu, kv_valid < BKV) : kv_valid < BKV) {
+      const int kv_valid = p.L_kv - j * BKV;
+      if (kv_valid < BKV) {
 #pragma unroll
         for (int i = 0; i < BKV; ++i)
           if (i >= kv_valid) sf[i] = -INFINITY;
@@ -462,7 +341,7 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
       float alpha = 1.f;
       bool rescale = false;
       if (j == 0) {
-        m_use = (MASKED && limit <= 0) ? 0.f : m_tile;  // a row that sees any of these keys sees the first
+        m_use = m_tile;
       } else if (m_tile > m_run + kRescaleThreshold) {
         m_use = m_tile;
         alpha = ex2(m_run - m_tile);
@@ -478,7 +357,7 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const f2 a = fma2(f2{sf[cc * 16 + 2 * i], sf[cc * 16 + 2 * i + 1]}, c2, negm);
-          const f2 pr = poly ? (MASKED ? ex2_poly2_sum(a) : ex2_poly2(a)) : f2{ex2(a.x), ex2(a.y)};
+          const f2 pr = poly ? ex2_poly2(a) : f2{ex2(a.x), ex2(a.y)};
           rowsum2 = add2(rowsum2, pr);
           pk[i] = pack_bf16x2(pr.x, pr.y);
         }
@@ -509,43 +388,10 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
       tc_fence_before();
       mbar_arrive(&st.p_full[q][b]);
     }
-    // this row's head, and its place among the rows of [batch][heads][L]
-    const int row_head = MASKED ? head + (row & ((1 << p.pack_shift) - 1)) : head;
-    const int64_t batch_head = static_cast<int64_t>(batch) * p.heads + row_head;
-    if (MASKED && nkv == 0) {
-      if (token < p.L && p.splits > 1) {
-        p.part_ml[(batch_head * p.splits + split) * p.L + token] = make_float2(-INFINITY, 0.f);
-      } else if (token < p.L) {
-        uint4* dst = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(batch) * p.out_stride_b +
-                                              static_cast<int64_t>(token) * p.out_stride_t +
-                                              static_cast<int64_t>(row_head) * HD);
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
-        p.lse[batch_head * p.L + token] = -INFINITY;
-      }
-    } else if (ok && mbar_wait(&st.o_done[q], 0, abort)) {
+    if (ok && mbar_wait(&st.o_done[q], 0, abort)) {
       tc_fence_after();
+      const int token = q_block0 + q * BQ + row;
       const float inv_l = 1.f / l_run;
-      if constexpr (MASKED) {
-        if (p.splits > 1) {
-          const int64_t at = (batch_head * p.splits + split) * p.L + token;
-          if (token < p.L) p.part_ml[at] = limit <= 0 ? make_float2(-INFINITY, 0.f) : make_float2(m_run, l_run);
-#pragma unroll 1
-          for (int oc = 0; oc < 4; ++oc) {
-            uint32_t orr[32];
-            tmem_ld32(o_tmem + oc * 32, orr);
-            tmem_ld_wait();
-            if (token < p.L && limit > 0) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                reinterpret_cast<uint4*>(p.part_o + at * HD + oc * 32)[i] =
-                    make_uint4(orr[4 * i], orr[4 * i + 1], orr[4 * i + 2], orr[4 * i + 3]);
-            }
-          }
-        } else if (token < p.L)
-          p.lse[batch_head * p.L + token] =
-              limit <= 0 ? -INFINITY : (m_run + log2f(l_run)) * 0.6931471805599453f;
-      }
       if constexpr (OUT_E4M3) {
         // e4m3 rows are 128 bytes.  Each thread owns one row, so storing straight from registers
         // would scatter 32 rows per instruction; instead the warp stages its 32 quantised rows in
@@ -599,7 +445,7 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
             *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(head) * HD + g * 16u) = v;
           }
         }
-      } else if (!MASKED || p.splits == 1) {
+      } else {
 #pragma unroll 1
         for (int oc = 0; oc < 4; ++oc) {
           uint32_t orr[32];
@@ -607,14 +453,13 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
           tmem_ld_wait();
           if (token < p.L) {
             const int64_t base = static_cast<int64_t>(batch) * p.out_stride_b +
-                                 static_cast<int64_t>(token) * p.out_stride_t +
-                                 static_cast<int64_t>(row_head) * HD + oc * 32;
+                                 static_cast<int64_t>(token) * p.out_stride_t + static_cast<int64_t>(head) * HD +
+                                 oc * 32;
 #pragma unroll
             for (int v8 = 0; v8 < 4; ++v8) {
               float f[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                f[i] = (MASKED && limit <= 0) ? 0.f : __uint_as_float(orr[v8 * 8 + i]) * inv_l;
+              for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(orr[v8 * 8 + i]) * inv_l;
               *reinterpret_cast<uint4*>(p.out + base + v8 * 8) = pack8(f);
             }
           }
@@ -628,53 +473,8 @@ __global__ void __launch_bounds__(N == NQ ? kThreads : kThreadsOne, N == NQ ? 1 
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256 * N);
+    tmem_dealloc(tmem, TMEM_COLS);
   }
-}
-
-// Joins the splits of the MASKED kernel, one warp per query row: with m_i, l_i, O_i of split i and M = max m_i,
-// O = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  Splits where a row saw no key have l = 0 and an O that was never
-// written.  The splits are added in their order.
-struct JoinParams {
-  const float* part_o;
-  const float2* part_ml;
-  __nv_bfloat16* out;
-  int64_t out_stride_b, out_stride_t;
-  float* lse;
-  int L, heads, splits;
-  int64_t rows;  // batch * heads * L
-};
-
-__global__ void __launch_bounds__(256) attn_join_kernel(JoinParams p) {
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= p.rows) return;
-  const int64_t bh = row / p.L;
-  const int token = static_cast<int>(row - bh * p.L);
-  const int64_t first = bh * p.splits * p.L + token;
-  float m = -INFINITY;
-  for (int i = 0; i < p.splits; ++i) m = fmaxf(m, p.part_ml[first + static_cast<int64_t>(i) * p.L].x);
-  float l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < p.splits; ++i) {
-    const int64_t at = first + static_cast<int64_t>(i) * p.L;
-    const float2 ml = p.part_ml[at];
-    if (ml.y == 0.f) continue;  // the same for the whole warp
-    const float w = exp2f(ml.x - m);
-    const float4 v = reinterpret_cast<const float4*>(p.part_o + at * HD)[lane];
-    l = fmaf(w, ml.y, l);
-    o.x = fmaf(w, v.x, o.x);
-    o.y = fmaf(w, v.y, o.y);
-    o.z = fmaf(w, v.z, o.z);
-    o.w = fmaf(w, v.w, o.w);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t batch = bh / p.heads, head = bh - batch * p.heads;
-  reinterpret_cast<uint2*>(p.out + batch * p.out_stride_b + token * p.out_stride_t + head * HD)[lane] =
-      make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-  if (lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------------------------------

@@ -19,7 +19,7 @@
 // latency, first scores) and storing.
 #pragma once
 
-#include "attention.cuh"
+#include "attention_masked.cuh"
 #include "rows.cuh"
 
 namespace ogx {
@@ -40,7 +40,7 @@ constexpr int kSoftmaxWarps = 8;
 
 struct BwdParams {
   int L, L_kv;
-  int heads, kv_heads, heads_per_kv;
+  int batch, heads, kv_heads, heads_per_kv;
   int q_tiles, kv_tiles;
   unsigned dkdv_ctas;  // CTAs [0, dkdv_ctas) make dK and dV, the rest dQ
   int dkdv_splits, dq_splits;  // CTAs that share a tile's sum
@@ -52,6 +52,20 @@ struct BwdParams {
   const float* stats;  // [batch][heads][q_tiles][2][128]
   __nv_bfloat16 *dq, *dk, *dv;
   int64_t dq_stride_b, dq_stride_t, dk_stride_b, dk_stride_t, dv_stride_b, dv_stride_t;
+};
+
+// Which tile CTA `idx` of a role makes.  The tiles of a head follow one another, so that CTAs which run together share its
+// operands in L2; causal sums differ in length, and there the longest of all heads come first.
+struct TileOf {
+  int at, head, batch;  // at: counted from the longest sum
+  __device__ __forceinline__ TileOf(const BwdParams& p, unsigned idx, int tiles, int heads) {
+    const unsigned sums = p.causal_block > 0 ? heads * p.batch : tiles;
+    const int lo = static_cast<int>(idx % sums), hi = static_cast<int>(idx / sums);
+    at = p.causal_block > 0 ? hi : lo;
+    const int bh = p.causal_block > 0 ? lo : hi;
+    head = bh % heads;
+    batch = bh / heads;
+  }
 };
 
 struct BwdShared {
@@ -86,57 +100,6 @@ __device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a, uint32_t b, 
                (accumulate || kk > 0) ? 1u : 0u);
 }
 
-// Exchanges the pieces of four lanes: lane q of each group of four gets piece q of all four, in the lanes' order.
-__device__ __forceinline__ void transpose4(uint4 (&v)[4], uint32_t lane) {
-#pragma unroll
-  for (uint32_t bit = 1; bit <= 2; bit *= 2) {
-    const bool up = lane & bit;
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      if (i & bit) continue;
-      uint4& lo = v[i];
-      uint4& hi = v[i + bit];
-      uint4 t = up ? lo : hi;
-      t.x = __shfl_xor_sync(0xffffffffu, t.x, bit);
-      t.y = __shfl_xor_sync(0xffffffffu, t.y, bit);
-      t.z = __shfl_xor_sync(0xffffffffu, t.z, bit);
-      t.w = __shfl_xor_sync(0xffffffffu, t.w, bit);
-      if (up)
-        lo = t;
-      else
-        hi = t;
-    }
-  }
-}
-
-// `columns` fp32 columns in tensor memory of a warp's 32 rows, times `scale`, as bf16 to rows `stride` elements
-// apart, the first `rows` of them.  A lane holds a row; storing it so would send 32 rows' 16-byte pieces with every
-// instruction (one cycle of the L1 for each: 3.3 us for dK and dV of a tile), so four lanes trade pieces and store
-// 64 bytes of a row together.
-__device__ __forceinline__ void store_rows(uint32_t taddr, int columns, float scale, __nv_bfloat16* dst, int64_t stride,
-                                           int rows, uint32_t lane) {
-  __nv_bfloat16* mine = dst + static_cast<int64_t>(lane & ~3u) * stride + (lane & 3u) * 8;
-  const int left = rows - static_cast<int>(lane & ~3u);  // of this lane's four rows
-#pragma unroll 1
-  for (int oc = 0; oc < columns / 32; ++oc) {
-    uint32_t r[32];
-    tmem_ld32(taddr + oc * 32, r);
-    tmem_ld_wait();
-    uint4 piece[4];
-#pragma unroll
-    for (int v8 = 0; v8 < 4; ++v8) {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[v8 * 8 + i]) * scale;
-      piece[v8] = pack8(f);
-    }
-    transpose4(piece, lane);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) *reinterpret_cast<uint4*>(mine + i * stride + oc * 32) = piece[i];
-  }
-}
-
 // `columns` fp32 columns of a warp's 32 rows to a CTA's part of a shared sum (rows of 128, a row per lane).
 __device__ __forceinline__ void store_part(uint32_t taddr, int columns, float* dst, uint32_t lane) {
 #pragma unroll 1
@@ -147,6 +110,20 @@ __device__ __forceinline__ void store_part(uint32_t taddr, int columns, float* d
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       reinterpret_cast<uint4*>(dst + lane * HD + oc * 32)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+  }
+}
+
+// A group's 64 columns of a gradient tile (a row per thread), by a TMA store from `half`, a half tile of shared memory
+// that nothing else uses any more.  All 128 threads come here, those whose wait failed included.
+__device__ __forceinline__ void store_half(uint32_t taddr, float scale, uint8_t* half, const CUtensorMap* map, int g,
+                                           uint32_t row, int head, int row0, int batch, bool ok) {
+  if (ok) stage_row64(taddr, scale, false, half, row);
+  fence_async_shared();
+  named_bar_sync(1 + g, 128);
+  if (row == 0 && ok) {
+    tma_store_4d(map, half, g * 64, head, row0, batch);
+    tma_store_commit();
+    tma_store_wait_read();
   }
 }
 
@@ -267,8 +244,8 @@ __global__ void __launch_bounds__(256, 4) attn_bwd_stats_kernel(StatsParams p) {
 // dV and the next S.  A group of four warps takes 32 query columns of the first half and 32 of the second, and P goes
 // to the MMA issuer half by half: the first half's dV runs while the second half is still exponentials.
 __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv,
-                                         const CUtensorMap* tdo, const BwdParams& p, BwdShared& st, uint8_t* smem,
-                                         uint32_t tmem) {
+                                         const CUtensorMap* tdo, const CUtensorMap* tdk, const CUtensorMap* tdv,
+                                         const BwdParams& p, BwdShared& st, uint8_t* smem, uint32_t tmem) {
   uint8_t* k_tile = smem;
   uint8_t* v_tile = smem + T_BYTES;
   uint8_t* q_tiles = smem + 2 * T_BYTES;
@@ -280,11 +257,10 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
 
   const int split = static_cast<int>(blockIdx.x % p.dkdv_splits);
   const unsigned idx = blockIdx.x / p.dkdv_splits;
-  const int kt = static_cast<int>(idx % p.kv_tiles);
-  const int bh = static_cast<int>(idx / p.kv_tiles);
-  const int kv_head = bh % p.kv_heads;
-  const int batch = bh / p.kv_heads;
-  const int k0 = kt * BT;
+  const TileOf own(p, idx, p.kv_tiles, p.kv_heads);
+  const int kv_head = own.head;
+  const int batch = own.batch;
+  const int k0 = own.at * BT;  // the first keys are seen by the most queries
   const Visibility vis{clamp_length(p.q_lengths, batch, p.L), clamp_length(p.kv_lengths, batch, p.L_kv),
                        p.causal_block, p.L_kv - p.L};
   const int first_tile = max(vis.first(k0), 0) / BT;
@@ -511,24 +487,19 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
       warp_arrive(&st.ds_full[0], lane);
     }
     // each group stores half of the columns of both: dV while the last dK product runs, then dK
-    const int key0 = k0 + static_cast<int>(quarter * 32);
-    const int column = kv_head * HD + g * 64;
-    if (ok && mbar_wait(&st.dv_done, 0, abort)) {
-      tc_fence_after();
-      if (p.dkdv_splits > 1)
-        store_part(tmem + lane_off + 256 + g * 64, 64, part + quarter * 32 * HD + g * 64, lane);
-      else
-        store_rows(tmem + lane_off + 256 + g * 64, 64, 1.f,
-                   p.dv + batch * p.dv_stride_b + key0 * p.dv_stride_t + column, p.dv_stride_t, p.L_kv - key0, lane);
-    }
-    if (ok && mbar_wait(&st.done, 0, abort)) {
-      tc_fence_after();
-      if (p.dkdv_splits > 1)
-        store_part(tmem + lane_off + 384 + g * 64, 64, part + BT * HD + quarter * 32 * HD + g * 64, lane);
-      else
-        store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale,
-                   p.dk + batch * p.dk_stride_b + key0 * p.dk_stride_t + column, p.dk_stride_t, p.L_kv - key0, lane);
-    }
+    const uint32_t row = quarter * 32 + lane;
+    ok = ok && mbar_wait(&st.dv_done, 0, abort);
+    tc_fence_after();
+    if (p.dkdv_splits == 1)
+      store_half(tmem + lane_off + 256 + g * 64, 1.f, do_tiles + g * T_HALF_BYTES, tdv, g, row, kv_head, k0, batch, ok);
+    else if (ok)
+      store_part(tmem + lane_off + 256 + g * 64, 64, part + quarter * 32 * HD + g * 64, lane);
+    ok = ok && mbar_wait(&st.done, 0, abort);
+    tc_fence_after();
+    if (p.dkdv_splits == 1)
+      store_half(tmem + lane_off + 384 + g * 64, p.scale, q_tiles + g * T_HALF_BYTES, tdk, g, row, kv_head, k0, batch, ok);
+    else if (ok)
+      store_part(tmem + lane_off + 384 + g * 64, 64, part + BT * HD + quarter * 32 * HD + g * 64, lane);
   }
 }
 
@@ -538,8 +509,8 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
 // P never leaves the registers here.  With two score buffers S(j+1) is ready before the softmax of tile j ends,
 // and dP(j+1) runs as soon as dP(j) is in registers.
 __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv,
-                                       const CUtensorMap* tdo, const BwdParams& p, BwdShared& st, uint8_t* smem,
-                                       uint32_t tmem) {
+                                       const CUtensorMap* tdo, const CUtensorMap* tdq, const BwdParams& p,
+                                       BwdShared& st, uint8_t* smem, uint32_t tmem) {
   uint8_t* q_tile = smem;
   uint8_t* do_tile = smem + T_BYTES;
   uint8_t* k_tiles = smem + 2 * T_BYTES;
@@ -550,12 +521,11 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
 
   const int split = static_cast<int>((blockIdx.x - p.dkdv_ctas) % p.dq_splits);
   const unsigned idx = (blockIdx.x - p.dkdv_ctas) / p.dq_splits;
-  const int qt = p.q_tiles - 1 - static_cast<int>(idx % p.q_tiles);  // causal rows get longer with their index
-  const int bh = static_cast<int>(idx / p.q_tiles);
-  const int head = bh % p.heads;
-  const int batch = bh / p.heads;
+  const TileOf own(p, idx, p.q_tiles, p.heads);
+  const int head = own.head;
+  const int batch = own.batch;
   const int kv_head = head / p.heads_per_kv;
-  const int q0 = qt * BT;
+  const int q0 = (p.q_tiles - 1 - own.at) * BT;  // causal rows get longer with their index
   const Visibility vis{clamp_length(p.q_lengths, batch, p.L), clamp_length(p.kv_lengths, batch, p.L_kv),
                        p.causal_block, p.L_kv - p.L};
   const int last = min(q0 + BT, vis.q_len) - 1;
@@ -671,7 +641,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
     const int token = q0 + row;
     const uint32_t lane_off = (quarter * 32u) << 16;
     const uint32_t dp_tmem = tmem + lane_off + 256 + g * 64;
-    const float* stat = p.stats + ((static_cast<int64_t>(batch) * p.heads + head) * p.q_tiles + qt) * STAT_FLOATS + row;
+    const float* stat = p.stats + ((static_cast<int64_t>(batch) * p.heads + head) * p.q_tiles + (p.q_tiles - 1 - own.at)) * STAT_FLOATS + row;
     const float nl = stat[0], nd = stat[BT];
     const int limit = vis.limit(token);
     bool ok = true;
@@ -721,16 +691,12 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
       tmem_st_wait();
       warp_arrive(&st.ds_full[b], lane);
     }
-    if (ok && mbar_wait(&st.done, 0, abort)) {
-      tc_fence_after();
-      const int token0 = q0 + static_cast<int>(quarter * 32);
-      if (p.dq_splits > 1)
-        store_part(tmem + lane_off + 384 + g * 64, 64, part + quarter * 32 * HD + g * 64, lane);
-      else
-        store_rows(tmem + lane_off + 384 + g * 64, 64, p.scale,
-                 p.dq + batch * p.dq_stride_b + token0 * p.dq_stride_t + static_cast<int64_t>(head) * HD + g * 64,
-                 p.dq_stride_t, p.L - token0, lane);
-    }
+    ok = ok && mbar_wait(&st.done, 0, abort);
+    tc_fence_after();
+    if (p.dq_splits == 1)
+      store_half(tmem + lane_off + 384 + g * 64, p.scale, q_tile + g * T_HALF_BYTES, tdq, g, row, head, q0, batch, ok);
+    else if (ok)
+      store_part(tmem + lane_off + 384 + g * 64, 64, part + quarter * 32 * HD + g * 64, lane);
   }
 }
 
@@ -750,9 +716,8 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const __grid_constan
   if (tile < dkdv_tiles) {
     const unsigned idx = tile >> 1;
     const bool is_dk = tile & 1;
-    const int k0 = static_cast<int>(idx % p.kv_tiles) * BT;
-    const int bh = static_cast<int>(idx / p.kv_tiles);
-    const int kv_head = bh % p.kv_heads, batch = bh / p.kv_heads;
+    const TileOf own(p, idx, p.kv_tiles, p.kv_heads);
+    const int k0 = own.at * BT, kv_head = own.head, batch = own.batch;
     splits = p.dkdv_splits;
     part_stride = 2 * BT * HD;
     src = p.dkdv_parts + static_cast<int64_t>(idx) * splits * part_stride + (is_dk ? BT * HD : 0);
@@ -763,9 +728,8 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const __grid_constan
     if (!is_dk) scale = 1.f;
   } else {
     const unsigned idx = tile - dkdv_tiles;
-    const int q0 = (p.q_tiles - 1 - static_cast<int>(idx % p.q_tiles)) * BT;
-    const int bh = static_cast<int>(idx / p.q_tiles);
-    const int head = bh % p.heads, batch = bh / p.heads;
+    const TileOf own(p, idx, p.q_tiles, p.heads);
+    const int q0 = (p.q_tiles - 1 - own.at) * BT, head = own.head, batch = own.batch;
     splits = p.dq_splits;
     part_stride = BT * HD;
     src = p.dq_parts + static_cast<int64_t>(idx) * splits * part_stride;
@@ -793,7 +757,9 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const __grid_constan
 
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                    const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo, BwdParams p) {
+                    const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
+                    const __grid_constant__ CUtensorMap tdq, const __grid_constant__ CUtensorMap tdk,
+                    const __grid_constant__ CUtensorMap tdv, BwdParams p) {
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
   __shared__ BwdShared st;
@@ -834,9 +800,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   tc_fence_after();
   const uint32_t tmem = st.tmem_base;
   if (blockIdx.x < p.dkdv_ctas)
-    bwd_dkdv(&tq, &tk, &tv, &tdo, p, st, smem, tmem);
+    bwd_dkdv(&tq, &tk, &tv, &tdo, &tdk, &tdv, p, st, smem, tmem);
   else
-    bwd_dq(&tq, &tk, &tv, &tdo, p, st, smem, tmem);
+    bwd_dq(&tq, &tk, &tv, &tdo, &tdq, p, st, smem, tmem);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {

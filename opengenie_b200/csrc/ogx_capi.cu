@@ -21,6 +21,7 @@
 #include "../../include/ogx.h"
 #include "elementwise.cuh"
 #include "attention.cuh"
+#include "attention_masked.cuh"
 #include "attention_bwd.cuh"
 #include "qk_norm.cuh"
 #include "rows.cuh"
@@ -1495,16 +1496,16 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 constexpr int64_t kMaxSplits = 64;
 
-// The forward kernel's form and the CTAs that share a query block's keys.  Two Q tiles per CTA read each key tile once
-// for 256 queries; one tile per CTA, two CTAs per SM, wastes less on an odd or single tile and hides a CTA's start and
-// end behind the other's products, but the key tiles then come through L2 twice as often.  In units of a 64-key tile
-// of the first form (0.9 us) a CTA costs its tiles and 6.4 to start and end; in the second form its tiles cost 1.32
-// each, or 0.6 when no other CTA is on the SM; joining shared blocks costs a launch, 6.  Measured at 32 heads, us with
-// two tiles and one: 4736 x 256 45.6 and 37.3, 4736 x 2048 173 and 177, 9216 x 9216 1130 and 1345; without and with
-// sharing: 512 x 9216 136 and 86.
+// The masked kernel's form and the CTAs that share a query block's keys.  Two Q tiles per CTA read each key tile once for
+// 256 queries; one tile per CTA, two CTAs per SM, wastes less on an odd or single tile, but the key tiles come through
+// L2 twice as often.  In units of a 64-key tile of the first form (0.9 us) a block costs its tiles and 3.6 to change to
+// the next, and the launch 2.8; in the second form its tiles cost 1.32 each, or 0.6 when no other CTA is on the SM, a
+// change 4.5 and the launch 2; joining shared blocks costs a launch, 6.  Measured at 32 heads, us with two tiles and
+// one: 4736 x 64 24.6 and 23.9, 9216 x 64 42.3 and 48.8, 9216 x 1024 141 and 183; without and with sharing:
+// 512 x 9216 136 and 87.
 // A power of two of query heads with the same key/value head stand together in a Q tile, token by token, so that their
 // keys are read once and a causal tile spans fewer tokens.  With 32 heads on 8, us apart and together: 1 x 50,000 120
-// and 71 (832 unshared in the first form), causal 9216 641 and 564.
+// and 72 (832 unshared in the first form), causal 9216 641 and 564.
 struct FwdPlan {
   bool one;
   int pack_shift;
@@ -1525,8 +1526,8 @@ FwdPlan fwd_plan(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t hea
     for (int64_t n = 1; n <= kMaxSplits && (n == 1 || (n * 4 <= tiles && blocks * (n - 1) < 2 * slots && batch * n <= 65535));
          ++n) {
       const double tile = !one ? 1.0 : (blocks * n <= sms ? 0.6 : 1.32);
-      const double cost = static_cast<double>(ceil_div(blocks * n, slots)) * (ceil_div(tiles, n) * tile + 6.4) +
-                          (n > 1 ? 6 : 0);
+      const double waves = static_cast<double>(ceil_div(blocks * n, slots));
+      const double cost = waves * (ceil_div(tiles, n) * tile + (one ? 4.5 : 3.6)) + (one ? 2.0 : 2.8) + (n > 1 ? 6 : 0);
       if ((n == 1 && !one) || cost < best_cost) {
         best = FwdPlan{one, shift, n};
         best_cost = cost;
@@ -1629,12 +1630,13 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
   const int64_t parts = fwd_part_rows(batch, q_tokens, heads, splits);
   if (splits > 1 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < parts * (ogx::attn::HD + 2) * 4))
     return fail(OGX_EINVAL, "workspace");
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   const int pack = 1 << plan.pack_shift;
+  if ((rc = token_map(&mo, out, heads, q_tokens, batch, out_stride_t, out_stride_b, ogx::attn::BQ / pack, pack))) return rc;
   if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BQ / pack, pack))) return rc;
   if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, k_stride_t, k_stride_b, ogx::attn::BKV))) return rc;
   if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, v_stride_t, v_stride_b, ogx::attn::BKV))) return rc;
-  ogx::attn::Params p{};
+  ogx::attn::MaskedParams p{};
   p.L = static_cast<int>(q_tokens);
   p.L_kv = static_cast<int>(kv_tokens);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
@@ -1649,22 +1651,30 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
   p.q_lengths = q_lengths;
   p.kv_lengths = kv_lengths;
   const bool one = plan.one;
-  auto kern = one ? ogx::attn::attn_fwd_kernel<false, true, 1> : ogx::attn::attn_fwd_kernel<false, true>;
-  const int smem = one ? ogx::attn::SMEM_BYTES_ONE : ogx::attn::SMEM_BYTES;
-  if ((rc = attn_register_split_ok(reinterpret_cast<const void*>(kern),
-                                   one ? ogx::attn::kLaunchRegsOne : ogx::attn::kLaunchRegs)))
+  using One = ogx::attn::MaskedShape<1>;
+  using Two = ogx::attn::MaskedShape<2>;
+  auto kern = one ? ogx::attn::attn_masked_kernel<1> : ogx::attn::attn_masked_kernel<2>;
+  const int smem = one ? ogx::attn::kMaskedSmem<1> : ogx::attn::kMaskedSmem<2>;
+  if ((rc = attn_register_split_ok(reinterpret_cast<const void*>(kern), one ? One::LAUNCH_REGS : Two::LAUNCH_REGS)))
     return rc;
   if ((rc = ensure_smem(kern, smem))) return rc;
   const int64_t tiles = ceil_div(kv_tokens, ogx::attn::BKV);
-  p.splits = static_cast<int>(splits);
+  p.splits = static_cast<unsigned>(splits);
   p.split_tiles = static_cast<int>(ceil_div(tiles, splits));
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = splits > 1 ? reinterpret_cast<float2*>(p.part_o + parts * ogx::attn::HD) : nullptr;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(ceil_div(q_tokens * pack, one ? 128 : 256)), static_cast<unsigned>(heads / pack),
-                  static_cast<unsigned>(batch * splits));
-  launch(kern, grid, one ? ogx::attn::kThreadsOne : ogx::attn::kThreads, smem, s, mq, mk, mv, p);
-  if ((rc = check_launch("attn_fwd_kernel")) || splits == 1) return rc;
+  p.blocks = static_cast<unsigned>(ceil_div(q_tokens * pack, one ? 128 : 256));
+  p.head_groups = static_cast<unsigned>(heads / pack);
+  // causal blocks differ in length: the longest of all heads first (28,800 tokens, 4 heads: 745 us, head by head 827)
+  const int64_t groups = batch * splits * p.head_groups;
+  p.longest_first = causal_block > 0 && p.blocks <= 65535 && groups <= INT32_MAX;
+  const dim3 grid = p.longest_first
+                        ? dim3(static_cast<unsigned>(groups), p.blocks)
+                        : dim3(p.blocks, p.head_groups, static_cast<unsigned>(batch * splits));
+  p.one_wave = int64_t{grid.x} * grid.y * grid.z <= (one ? 2 : 1) * sm_count();
+  launch(kern, grid, one ? One::THREADS : Two::THREADS, smem, s, mq, mk, mv, mo, p);
+  if ((rc = check_launch("attn_masked_kernel")) || splits == 1) return rc;
   ogx::attn::JoinParams jp{};
   jp.part_o = p.part_o;
   jp.part_ml = p.part_ml;
@@ -1674,7 +1684,7 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
   jp.lse = lse;
   jp.L = p.L;
   jp.heads = static_cast<int>(heads);
-  jp.splits = p.splits;
+  jp.splits = static_cast<int>(splits);
   jp.rows = batch * heads * q_tokens;
   launch(ogx::attn::attn_join_kernel, dim3(static_cast<unsigned>(ceil_div(jp.rows, 8))), 256, 0, s, jp);
   return check_launch("attn_join_kernel");
@@ -1720,11 +1730,14 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   const int64_t dkdv_ctas = kv_tiles * kv_heads * batch * ws.dkdv_splits;
   const int64_t dq_ctas = q_tiles * heads * batch * ws.dq_splits;
   if (dkdv_ctas + dq_ctas > INT32_MAX) return fail(OGX_EINVAL, "shape");
-  CUtensorMap mq, mk, mv, mdo;
+  CUtensorMap mq, mk, mv, mdo, mdq, mdk, mdv;
   if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BT))) return rc;
   if ((rc = token_map(&mdo, dout, heads, q_tokens, batch, dout_stride_t, dout_stride_b, ogx::attn::BT))) return rc;
   if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, k_stride_t, k_stride_b, ogx::attn::BT))) return rc;
   if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, v_stride_t, v_stride_b, ogx::attn::BT))) return rc;
+  if ((rc = token_map(&mdq, dq, heads, q_tokens, batch, dq_stride_t, dq_stride_b, ogx::attn::BT))) return rc;
+  if ((rc = token_map(&mdk, dk, kv_heads, kv_tokens, batch, dk_stride_t, dk_stride_b, ogx::attn::BT))) return rc;
+  if ((rc = token_map(&mdv, dv, kv_heads, kv_tokens, batch, dv_stride_t, dv_stride_b, ogx::attn::BT))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 
   ogx::attn::StatsParams sp{};
@@ -1752,6 +1765,7 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   ogx::attn::BwdParams p{};
   p.L = static_cast<int>(q_tokens);
   p.L_kv = static_cast<int>(kv_tokens);
+  p.batch = static_cast<int>(batch);
   p.heads = static_cast<int>(heads);
   p.kv_heads = static_cast<int>(kv_heads);
   p.heads_per_kv = static_cast<int>(heads / kv_heads);
@@ -1780,7 +1794,7 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   auto kern = ogx::attn::attn_bwd_kernel;
   if ((rc = ensure_smem(kern, ogx::attn::BWD_SMEM))) return rc;
   launch(kern, dim3(static_cast<unsigned>(dkdv_ctas + dq_ctas)), ogx::attn::kBwdThreads, ogx::attn::BWD_SMEM, s, mq, mk,
-         mv, mdo, p);
+         mv, mdo, mdq, mdk, mdv, p);
   if ((rc = check_launch("attn_bwd_kernel"))) return rc;
   const int64_t joined = (ws.dkdv_splits > 1 ? 2 * kv_tiles * kv_heads * batch : 0) +
                          (ws.dq_splits > 1 ? q_tiles * heads * batch : 0);

@@ -144,6 +144,18 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* map, uin
       : "memory");
 }
 
+// The stores of one thread form a group; its shared memory may be written again (or the CTA end) once they are read.
+__device__ __forceinline__ void tma_store_4d(const void* map, const void* smem_src, int32_t x, int32_t y, int32_t z,
+                                             int32_t w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
+               "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
 // ---------------------------------------------------------------- CTA pairs (clusters of two)
 // The two CTAs of a pair run one 256-row tcgen05 MMA together: each holds half of the A rows and half of
 // the B rows in its shared memory and receives its half of the result in its own TMEM.  The MMA, its
