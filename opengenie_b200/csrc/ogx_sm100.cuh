@@ -144,6 +144,13 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* map, uin
       : "memory");
 }
 
+// Brings a tile to L2.
+__device__ __forceinline__ void tma_prefetch_4d(const void* map, int32_t x, int32_t y, int32_t z, int32_t w) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(x), "r"(y),
+               "r"(z), "r"(w)
+               : "memory");
+}
+
 // The stores of one thread form a group; its shared memory may be written again (or the CTA end) once they are read.
 __device__ __forceinline__ void tma_store_4d(const void* map, const void* smem_src, int32_t x, int32_t y, int32_t z,
                                              int32_t w) {
