@@ -362,22 +362,22 @@ int ogx_attention_fwd_e4m3_to_peers(const void* q, const void* k, const void* v,
 
 /* Attention with masks and shared key/value heads, keeping the softmax statistics.  q [batch, q_tokens,
  * heads*128], k and v [batch, kv_tokens, kv_heads*128] bf16 with token and batch strides (multiples of 8
- * elements); query head h reads key/value head h / (heads / kv_heads).  Query i sees key j when
+ * elements), at most 2^25 tokens; query head h reads key/value head h / (heads / kv_heads).  Query i sees key j when
  *   i < q_lengths[b], j < kv_lengths[b] (int32 device arrays, clamped to [0, tokens]; NULL: full length), and
  *   causal_block == 0 or j / causal_block <= floor((i + kv_tokens - q_tokens) / causal_block):
  * causal_block 1 is the token-causal mask with both sequences ending together, n a mask over blocks of n
  * positions (the tokens of a latent frame).  out: bf16 [batch, q_tokens, heads*128]; lse: f32 [batch, heads,
  * q_tokens], the natural log of each row's sum of exponentials.  A row that sees no key gets out = 0 and lse =
- * -inf.  Keys and values past kv_lengths may hold anything (NaN included).  Few queries over many keys are shared out
+ * -inf.  Keys and values past kv_lengths may hold anything (NaN included).  out may be q, but not k or v.  Few queries over many keys are shared out
  * over the keys and joined in a second launch; workspace (device memory, 16-byte aligned, overwritten; calls that may
  * run at the same time need one each) holds the parts: ogx_attention_fwd_lse_workspace says how much, often 0 (then
  * it may be NULL). */
 int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
                           int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
                           int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b,
-                          int64_t v_stride_t, float softmax_scale, int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
-                          int64_t out_stride_b, int64_t out_stride_t, float* lse, void* workspace,
-                          int64_t workspace_bytes, void* stream);
+                          int64_t v_stride_t, float softmax_scale, int64_t causal_block, const int* q_lengths,
+                          const int* kv_lengths, void* out, int64_t out_stride_b, int64_t out_stride_t, float* lse,
+                          void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Bytes of device workspace that ogx_attention_fwd_lse needs for these sizes on the current device. */
 int ogx_attention_fwd_lse_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
@@ -389,7 +389,7 @@ int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_toke
 
 /* Gradients of ogx_attention_fwd_lse: from dout (the gradient of out), the forward's inputs, out and lse, dq
  * [batch, q_tokens, heads*128] and dk, dv [batch, kv_tokens, kv_heads*128] (bf16, own strides), every element
- * written.  The probabilities are recomputed from lse.  Rows past q_lengths and
+ * written; they must not overlap an input.  The probabilities are recomputed from lse.  Rows past q_lengths and
  * rows that see no key get dq = 0 and give nothing to dk and dv (their q and dout may hold anything); keys past
  * kv_lengths get dk = dv = 0.  workspace: device memory, 16-byte aligned, overwritten; calls that may run at the
  * same time need one each. */
@@ -397,8 +397,8 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
                       const float* lse, int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
                       int64_t kv_heads, int64_t head_dim, int64_t dout_stride_b, int64_t dout_stride_t,
                       int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
-                      int64_t v_stride_b, int64_t v_stride_t, int64_t out_stride_b, int64_t out_stride_t, float softmax_scale,
-                      int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* workspace,
+                      int64_t v_stride_b, int64_t v_stride_t, int64_t out_stride_b, int64_t out_stride_t,
+                      float softmax_scale, int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* workspace,
                       int64_t workspace_bytes, void* dq, int64_t dq_stride_b, int64_t dq_stride_t, void* dk,
                       int64_t dk_stride_b, int64_t dk_stride_t, void* dv, int64_t dv_stride_b, int64_t dv_stride_t,
                       void* stream);

@@ -110,7 +110,8 @@ __device__ __forceinline__ void store_part(uint32_t taddr, int columns, float* d
     tmem_ld_wait();
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      reinterpret_cast<uint4*>(dst + lane * HD + oc * 32)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+      reinterpret_cast<uint4*>(dst + lane * HD + oc * 32)[i] =
+          make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
   }
 }
 
@@ -658,7 +659,8 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
     const int token = q0 + row;
     const uint32_t lane_off = (quarter * 32u) << 16;
     const uint32_t dp_tmem = tmem + lane_off + 256 + g * 64;
-    const float* stat = p.stats + ((static_cast<int64_t>(batch) * p.heads + head) * p.q_tiles + (p.q_tiles - 1 - own.at)) * STAT_FLOATS + row;
+    const float* stat =
+        p.stats + ((static_cast<int64_t>(batch) * p.heads + head) * p.q_tiles + q0 / BT) * STAT_FLOATS + row;
     const float nl = stat[0], nd = stat[BT];
     const int limit = vis.limit(token);
     bool ok = true;

@@ -1462,18 +1462,24 @@ bool row_strides_ok(int64_t width, int64_t tokens, int64_t batch, int64_t stride
   return stride_t < (int64_t{1} << 38) && (batch == 1 || stride_b < (int64_t{1} << 38)) && tokens > 0;
 }
 
+// Tokens: positions and tile ends stay far below 2^31, and the sum over one row's keys takes less time than a wait's
+// limit (0.5 s), since some warps wait for the whole of it.
+constexpr int64_t kMostTokens = int64_t{1} << 25;
+
+bool attention_sizes_ok(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads) {
+  return batch >= 1 && q_tokens >= 1 && kv_tokens >= 1 && heads >= 1 && kv_heads >= 1 && q_tokens <= kMostTokens &&
+         kv_tokens <= kMostTokens && heads <= 65535 && batch <= 65535;
+}
+
 int masked_attention_guard(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
                            int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
-                           int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b, int64_t v_stride_t,
-                           float softmax_scale, int64_t causal_block) {
+                           int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b,
+                           int64_t v_stride_t, float softmax_scale, int64_t causal_block) {
   if (q == nullptr || k == nullptr || v == nullptr) return fail(OGX_EINVAL, "null_pointer");
   if (head_dim != 128) return fail(OGX_EINVAL, "head_dim: only 128 is supported");
-  if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1 || kv_heads < 1) return fail(OGX_EINVAL, "shape");
-  // positions and tile ends stay below 2^31
-  constexpr int64_t kMost = int64_t{1} << 29;
-  if (q_tokens > kMost || kv_tokens > kMost || heads > 65535 || batch > 65535) return fail(OGX_EINVAL, "shape");
+  if (!attention_sizes_ok(batch, q_tokens, kv_tokens, heads, kv_heads)) return fail(OGX_EINVAL, "shape");
   if (heads % kv_heads) return fail(OGX_EINVAL, "kv_heads: heads must be a multiple of kv_heads");
-  if (causal_block < 0 || causal_block > kMost) return fail(OGX_EINVAL, "causal_block");
+  if (causal_block < 0 || causal_block > (int64_t{1} << 29)) return fail(OGX_EINVAL, "causal_block");
   // both ends stay far inside fp32
   if (!(softmax_scale >= 1e-30f) || softmax_scale > 1e30f) return fail(OGX_EINVAL, "softmax_scale");
   if (!row_strides_ok(heads * 128, q_tokens, batch, q_stride_t, q_stride_b) ||
@@ -1523,8 +1529,8 @@ FwdPlan fwd_plan(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t hea
   for (int form = 0; form < 2; ++form) {
     const bool one = form == 1;
     const int64_t blocks = batch * (heads >> shift) * ceil_div(rows, one ? 128 : 256), slots = one ? 2 * sms : sms;
-    for (int64_t n = 1; n <= kMaxSplits && (n == 1 || (n * 4 <= tiles && blocks * (n - 1) < 2 * slots && batch * n <= 65535));
-         ++n) {
+    for (int64_t n = 1; n <= kMaxSplits; ++n) {
+      if (n > 1 && (n * 4 > tiles || blocks * (n - 1) >= 2 * slots || batch * n > 65535)) break;
       const double tile = !one ? 1.0 : (blocks * n <= sms ? 0.6 : 1.32);
       const double waves = static_cast<double>(ceil_div(blocks * n, slots));
       const double cost = waves * (ceil_div(tiles, n) * tile + (one ? 4.5 : 3.6)) + (one ? 2.0 : 2.8) + (n > 1 ? 6 : 0);
@@ -1604,7 +1610,7 @@ extern "C" {
 int ogx_attention_fwd_lse_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
                                     int64_t kv_heads, int64_t* bytes) {
   if (bytes == nullptr) return fail(OGX_EINVAL, "null_pointer");
-  if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1 || kv_heads < 1) return fail(OGX_EINVAL, "shape");
+  if (!attention_sizes_ok(batch, q_tokens, kv_tokens, heads, kv_heads)) return fail(OGX_EINVAL, "shape");
   if (heads % kv_heads) return fail(OGX_EINVAL, "kv_heads: heads must be a multiple of kv_heads");
   const int64_t splits = fwd_plan(batch, q_tokens, kv_tokens, heads, kv_heads).splits;
   *bytes = splits > 1 ? fwd_part_rows(batch, q_tokens, heads, splits) * (ogx::attn::HD + 2) * 4 : 0;
@@ -1614,9 +1620,9 @@ int ogx_attention_fwd_lse_workspace(int64_t batch, int64_t q_tokens, int64_t kv_
 int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
                           int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
                           int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b,
-                          int64_t v_stride_t, float softmax_scale, int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* out,
-                          int64_t out_stride_b, int64_t out_stride_t, float* lse, void* workspace,
-                          int64_t workspace_bytes, void* stream) {
+                          int64_t v_stride_t, float softmax_scale, int64_t causal_block, const int* q_lengths,
+                          const int* kv_lengths, void* out, int64_t out_stride_b, int64_t out_stride_t, float* lse,
+                          void* workspace, int64_t workspace_bytes, void* stream) {
   int rc = masked_attention_guard(q, k, v, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, q_stride_b,
                                   q_stride_t, k_stride_b, k_stride_t, v_stride_b, v_stride_t, softmax_scale,
                                   causal_block);
@@ -1632,8 +1638,9 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
     return fail(OGX_EINVAL, "workspace");
   CUtensorMap mq, mk, mv, mo;
   const int pack = 1 << plan.pack_shift;
-  if ((rc = token_map(&mo, out, heads, q_tokens, batch, out_stride_t, out_stride_b, ogx::attn::BQ / pack, pack))) return rc;
-  if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BQ / pack, pack))) return rc;
+  const int box = ogx::attn::BQ / pack;
+  if ((rc = token_map(&mo, out, heads, q_tokens, batch, out_stride_t, out_stride_b, box, pack))) return rc;
+  if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, box, pack))) return rc;
   if ((rc = token_map(&mk, k, kv_heads, kv_tokens, batch, k_stride_t, k_stride_b, ogx::attn::BKV))) return rc;
   if ((rc = token_map(&mv, v, kv_heads, kv_tokens, batch, v_stride_t, v_stride_b, ogx::attn::BKV))) return rc;
   ogx::attn::MaskedParams p{};
@@ -1693,7 +1700,7 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
 int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads,
                                 int64_t* bytes) {
   if (bytes == nullptr) return fail(OGX_EINVAL, "null_pointer");
-  if (batch < 1 || q_tokens < 1 || kv_tokens < 1 || heads < 1 || kv_heads < 1) return fail(OGX_EINVAL, "shape");
+  if (!attention_sizes_ok(batch, q_tokens, kv_tokens, heads, kv_heads)) return fail(OGX_EINVAL, "shape");
   if (heads % kv_heads) return fail(OGX_EINVAL, "kv_heads: heads must be a multiple of kv_heads");
   *bytes = bwd_workspace(batch, q_tokens, kv_tokens, heads, kv_heads).bytes;
   return OGX_OK;
@@ -1703,8 +1710,8 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
                       const float* lse, int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
                       int64_t kv_heads, int64_t head_dim, int64_t dout_stride_b, int64_t dout_stride_t,
                       int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
-                      int64_t v_stride_b, int64_t v_stride_t, int64_t out_stride_b, int64_t out_stride_t, float softmax_scale,
-                      int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* workspace,
+                      int64_t v_stride_b, int64_t v_stride_t, int64_t out_stride_b, int64_t out_stride_t,
+                      float softmax_scale, int64_t causal_block, const int* q_lengths, const int* kv_lengths, void* workspace,
                       int64_t workspace_bytes, void* dq, int64_t dq_stride_b, int64_t dq_stride_t, void* dk,
                       int64_t dk_stride_b, int64_t dk_stride_t, void* dv, int64_t dv_stride_b, int64_t dv_stride_t,
                       void* stream) {

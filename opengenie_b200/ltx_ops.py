@@ -1152,7 +1152,7 @@ def attention_with_lse(
     n > 0, ``j // n <= (i + L_kv - L) // n``: n = 1 is the token-causal mask with both sequences ending
     together, the tokens of a latent frame make it frame-causal (a token sees its own and all earlier frames).
     ``lse`` is the natural log of a row's sum of exponentials.  A row that sees no key gets out 0 and lse
-    -inf; keys and values past ``kv_lengths`` may hold anything.
+    -inf; keys and values past ``kv_lengths`` may hold anything.  ``out`` may be q, but not k or v.
 
     No reference counterpart: the reference infers with dense bidirectional attention only.
     """
@@ -1165,6 +1165,8 @@ def attention_with_lse(
         out_rows = (L * C, C)
     else:
         out_rows = _given_rows(out, q, "out_shape: out must be bf16 [B, L, heads*128] with unit column stride")
+        if out.data_ptr() in (k.data_ptr(), v.data_ptr()):  # other blocks still read them
+            raise ValueError("out_alias: out must not be k or v")
     lse = q.new_empty((B, heads, L), dtype=torch.float32)
     size = _workspace_bytes("ogx_attention_fwd_lse_workspace", q.device.index, B, L, k.shape[1], heads, kv_heads)
     workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
@@ -1198,7 +1200,8 @@ def attention_backward(
     The probabilities are recomputed from ``lse``.  Every gradient is summed in one order (dk and dv over the
     query heads that share a key head), so equal inputs give equal bits.  Rows past ``q_lengths`` and rows that
     see no key get dq 0 and give nothing to dk and dv; keys past ``kv_lengths`` get 0.  ``grads`` takes (dq, dk,
-    dv) to write into, for example the slices of one packed [B, L, (heads + 2*kv_heads)*128] buffer.  No reference counterpart (the reference only infers).
+    dv) to write into, for example the slices of one packed [B, L, (heads + 2*kv_heads)*128] buffer; none of them may
+    overlap an input.  No reference counterpart (the reference only infers).
     """
     kv_heads = heads if kv_heads is None else kv_heads
     q_rows, k_rows, v_rows, scale = _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block,
@@ -1217,6 +1220,9 @@ def attention_backward(
         dq, dk, dv = grads
         reason = "grads: bf16 tensors of the shapes of q, k and v with unit column stride"
         dq_rows, dk_rows, dv_rows = (_given_rows(t, like, reason) for t, like in ((dq, q), (dk, k), (dv, v)))
+        given = {t.data_ptr() for t in (dq, dk, dv)}
+        if len(given) < 3 or given & {t.data_ptr() for t in (dout, q, k, v, out)}:
+            raise ValueError("grads_alias: dq, dk and dv must be tensors of their own")
     workspace = q.new_empty(
         (_workspace_bytes("ogx_attention_bwd_workspace", device.index, B, L, M, heads, kv_heads),), dtype=torch.uint8)
     _call_on(

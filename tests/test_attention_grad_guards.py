@@ -78,6 +78,8 @@ def test_few_queries_over_many_keys_need_a_workspace(ogx_lib):
     assert ogx_lib.ogx_attention_fwd_lse(*call.values()) == -1 and _err(ogx_lib) == "workspace"
     assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 0, 20000, 4, 4, ctypes.addressof(n)) == -1
     assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, 20000, 4, 3, ctypes.addressof(n)) == -1
+    assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, (1 << 25) + 1, 4, 4, ctypes.addressof(n)) == -1
+    assert ogx_lib.ogx_attention_bwd_workspace(1, 1 << 62, 1, 4, 4, ctypes.addressof(n)) == -1
     assert ogx_lib.ogx_attention_fwd_lse_workspace(1, 1, 20000, 4, 4, None) == -1
 
 

@@ -114,6 +114,11 @@ CASES = [
     (1, 130, 130, 4, 2, 1, None, (97,)),
     (2, 3, 300, 128, 1, 0, (3, 2), (300, 1)),
     (1, 129, 140, 12, 2, 5, (127,), None),
+    # more query blocks than CTAs at a time, with empty ones among them
+    (2, 700, 70, 64, 64, 0, (700, 300), (70, 33)),
+    (2, 700, 130, 64, 32, 7, (650, 0), (130, 100)),
+    (8, 100, 70, 64, 64, 0, (100, 0, 1, 100, 99, 100, 64, 100), (70, 70, 70, 0, 1, 64, 65, 70)),
+    (3, 1025, 1025, 20, 4, 100, (1025, 257, 1000), (1025, 300, 1000)),
 ]
 
 
@@ -217,6 +222,20 @@ def test_strided_rows_given_outputs_and_expanded_batches(ops):
     ga = ops.attention_backward(dout, q, k1, v1, a[0], a[1], heads)
     gb = ops.attention_backward(dout, q, k1.contiguous(), v1.contiguous(), b[0], b[1], heads)
     assert all(torch.equal(x, y) for x, y in zip(ga, gb))
+
+
+def test_outputs_over_inputs(ops):
+    q, k, v, dout = _case(1, 300, 300, 2, 2, seed=5)
+    want, lse = ops.attention_with_lse(q, k, v, 2)
+    grads = [torch.empty_like(q) for _ in range(3)]
+    for bad in (k, v):
+        with pytest.raises(ValueError, match="out_alias"):
+            ops.attention_with_lse(q, k, v, 2, out=bad)
+    for i, bad in ((0, q), (1, k), (2, v), (0, dout), (0, want), (1, grads[0])):
+        with pytest.raises(ValueError, match="grads_alias"):
+            ops.attention_backward(dout, q, k, v, want, lse, 2, grads=[*grads[:i], bad, *grads[i + 1:]])
+    over, _ = ops.attention_with_lse(q, k, v, 2, out=q)  # every block reads its own rows before it writes them
+    assert over is q and torch.equal(over, want)
 
 
 def test_two_streams_and_captured_graphs_share_nothing(ops):
