@@ -442,6 +442,15 @@ int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq
                          int64_t dk_stride_b, int64_t dk_stride_t, float* dq_weight, float* dk_weight, void* workspace,
                          int64_t workspace_bytes, void* stream);
 
+/* An entry point by its number, with its arguments in their order as 64-bit slots: integers and pointers as they are, a
+ * float as the bits of a double.  `count` has to be the number of its arguments.  For callers whose foreign calls cost
+ * by the argument. */
+#define OGX_CALL_ATTENTION_FWD_LSE 0
+#define OGX_CALL_ATTENTION_BWD 1
+#define OGX_CALL_QK_NORM_ROPE 2
+#define OGX_CALL_QK_NORM_ROPE_BWD 3
+int ogx_call_packed(int entry, const int64_t* slots, int64_t count);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int, c_int64, c_uint, c_void_p
 
 LIB_NAME = "libogx.so"
@@ -134,6 +135,7 @@ _SIGNATURES: dict[str, list] = {
         c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p, c_int, c_int64,
         c_int64, c_void_p,
     ],
+    "ogx_call_packed": [c_int, c_void_p, c_int64],
     "ogx_attention_fwd_lse": [
         c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
         c_int64, c_int64, c_int64, c_int64, c_float, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
@@ -199,6 +201,24 @@ def call(name: str, *args) -> None:
     """Calls an entry point and raises OgxError (reason string from the library) on failure."""
     lib = load()
     rc = getattr(lib, name)(*args)
+    if rc != OGX_OK:
+        msg = lib.ogx_last_error().decode(errors="replace")
+        raise OgxError(f"{name}: {msg}" if msg else f"{name}: error {rc}")
+
+
+# The entry points that ``call_packed`` reaches, in the order of their OGX_CALL_* numbers: (number, packer, slots).
+_PACKED = {
+    name: (i, struct.Struct("".join("d" if t is c_float else "q" for t in _SIGNATURES[name])).pack, len(_SIGNATURES[name]))
+    for i, name in enumerate(("ogx_attention_fwd_lse", "ogx_attention_bwd", "ogx_qk_norm_rope", "ogx_qk_norm_rope_bwd"))
+}
+
+
+def call_packed(name: str, *args) -> None:
+    """``call`` for the entry points of 30 and more arguments, which ctypes converts one by one (4.4 us for 45 of them;
+    packed 0.7).  Null pointers are 0 here."""
+    lib = load()
+    entry, pack, count = _PACKED[name]
+    rc = lib.ogx_call_packed(entry, pack(*args), count)
     if rc != OGX_OK:
         msg = lib.ogx_last_error().decode(errors="replace")
         raise OgxError(f"{name}: {msg}" if msg else f"{name}: error {rc}")

@@ -13,6 +13,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <type_traits>
 #include <atomic>
 #include <unordered_map>
 #include <utility>
@@ -2076,3 +2077,43 @@ int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq
 }
 
 }  // extern "C"
+
+// ------------------------------------------------------------- calls with packed arguments
+namespace {
+
+template <typename T>
+T slot_as(int64_t slot) {
+  if constexpr (std::is_pointer_v<T>) {
+    return reinterpret_cast<T>(slot);
+  } else if constexpr (std::is_floating_point_v<T>) {
+    double d;
+    std::memcpy(&d, &slot, sizeof(d));
+    return static_cast<T>(d);
+  } else {
+    return static_cast<T>(slot);
+  }
+}
+
+template <typename... A, size_t... I>
+int call_slots(int (*entry)(A...), const int64_t* slots, std::index_sequence<I...>) {
+  return entry(slot_as<A>(slots[I])...);
+}
+
+template <typename... A>
+int call_slots(int (*entry)(A...), const int64_t* slots, int64_t count) {
+  if (count != static_cast<int64_t>(sizeof...(A))) return fail(OGX_EINVAL, "argument_count");
+  return call_slots(entry, slots, std::index_sequence_for<A...>{});
+}
+
+}  // namespace
+
+extern "C" int ogx_call_packed(int entry, const int64_t* slots, int64_t count) {
+  if (slots == nullptr) return fail(OGX_EINVAL, "null_pointer");
+  switch (entry) {
+    case OGX_CALL_ATTENTION_FWD_LSE: return call_slots(ogx_attention_fwd_lse, slots, count);
+    case OGX_CALL_ATTENTION_BWD: return call_slots(ogx_attention_bwd, slots, count);
+    case OGX_CALL_QK_NORM_ROPE: return call_slots(ogx_qk_norm_rope, slots, count);
+    case OGX_CALL_QK_NORM_ROPE_BWD: return call_slots(ogx_qk_norm_rope_bwd, slots, count);
+    default: return fail(OGX_EINVAL, "entry");
+  }
+}

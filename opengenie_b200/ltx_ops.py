@@ -43,13 +43,17 @@ def _stream(t: torch.Tensor) -> int:
 
 
 def _call_on(device: torch.device, name: str, *args) -> None:
-    """Calls an entry point with ``device`` current, on its current stream (the entry's last argument)."""
+    """Calls a training-pass entry point with ``device`` current, on its current stream (the entry's last argument)."""
     index = device.index
-    if index == torch.cuda.current_device():
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    if index == torch._C._cuda_getDevice():
+        _lib.call_packed(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+            _lib.call_packed(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _at(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -1172,8 +1176,8 @@ def attention_with_lse(
     workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
     _call_on(
         q.device, "ogx_attention_fwd_lse", q.data_ptr(), k.data_ptr(), v.data_ptr(), B, L, k.shape[1], heads, kv_heads,
-        128, *q_rows, *k_rows, *v_rows, scale, causal_block, _ptr(q_lengths), _ptr(kv_lengths), out.data_ptr(), *out_rows,
-        lse.data_ptr(), _ptr(workspace), size,
+        128, *q_rows, *k_rows, *v_rows, scale, causal_block, _at(q_lengths), _at(kv_lengths), out.data_ptr(), *out_rows,
+        lse.data_ptr(), _at(workspace), size,
     )
     return out, lse
 
@@ -1229,7 +1233,7 @@ def attention_backward(
         device, "ogx_attention_bwd", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
         lse.data_ptr(), B, L, M, heads, kv_heads, 128, *dout_rows, *q_rows, *k_rows, *v_rows, *out_rows, scale,
         causal_block,
-        _ptr(q_lengths), _ptr(kv_lengths), workspace.data_ptr(), workspace.numel(), dq.data_ptr(), *dq_rows,
+        _at(q_lengths), _at(kv_lengths), workspace.data_ptr(), workspace.numel(), dq.data_ptr(), *dq_rows,
         dk.data_ptr(), *dk_rows, dv.data_ptr(), *dv_rows,
     )
     return dq, dk, dv
@@ -1339,7 +1343,7 @@ def fused_qk_norm_rope(
     q_weight, k_weight = _contiguous16(q_weight), _contiguous16(k_weight)
     _call_on(
         q.device, "ogx_qk_norm_rope", q.data_ptr(), k.data_ptr(), B, L, heads, kv_heads, hd, *q_rows, *k_rows,
-        _ptr(q_weight), _ptr(k_weight), DTYPE_F32 if q_weight is None else _code(q_weight), _NORMS[norm], eps,
+        _at(q_weight), _at(k_weight), DTYPE_F32 if q_weight is None else _code(q_weight), _NORMS[norm], eps,
         cos.data_ptr(), sin.data_ptr(), _code(cos), rotary, interleaved, *cs_strides, q_out.data_ptr(), *q_out_rows,
         k_out.data_ptr(), *k_out_rows,
     )
@@ -1387,15 +1391,16 @@ def fused_qk_norm_rope_backward(
     dqw = dkw = workspace = None
     size = 0
     if norm != "none":
-        dqw, dkw = (w.new_empty(w.shape, dtype=torch.float32) for w in (q_weight, k_weight))
+        dqw = torch.empty_like(q_weight, dtype=torch.float32)
+        dkw = torch.empty_like(k_weight, dtype=torch.float32)
         size = _workspace_bytes("ogx_qk_norm_rope_bwd_workspace", q.device.index, B, L, heads, kv_heads, hd, _NORMS[norm])
         workspace = q.new_empty((size,), dtype=torch.uint8)
     _call_on(
         q.device, "ogx_qk_norm_rope_bwd", dq_out.data_ptr(), *dq_out_rows, dk_out.data_ptr(), *dk_out_rows,
-        q.data_ptr(), k.data_ptr(), B, L, heads, kv_heads, hd, *q_rows, *k_rows, _ptr(q_weight), _ptr(k_weight),
+        q.data_ptr(), k.data_ptr(), B, L, heads, kv_heads, hd, *q_rows, *k_rows, _at(q_weight), _at(k_weight),
         DTYPE_F32 if q_weight is None else _code(q_weight), _NORMS[norm], eps, cos.data_ptr(), sin.data_ptr(),
-        _code(cos), rotary, interleaved, *cs_strides, dq.data_ptr(), *dq_rows, dk.data_ptr(), *dk_rows, _ptr(dqw),
-        _ptr(dkw), _ptr(workspace), size,
+        _code(cos), rotary, interleaved, *cs_strides, dq.data_ptr(), *dq_rows, dk.data_ptr(), *dk_rows, _at(dqw),
+        _at(dkw), _at(workspace), size,
     )
     return dq, dk, dqw, dkw
 

@@ -131,3 +131,18 @@ def test_norm_rotation_gradient_entry_refusals(ogx_lib, change, reason):
 def test_refused_calls_leave_python_errors():
     with pytest.raises(_lib.OgxError, match="null_pointer"):
         _lib.call("ogx_attention_fwd_lse", *{**FWD, "q": None}.values())
+
+
+def test_packed_calls_reach_the_entry_points(ogx_lib):
+    """The packed form hands every argument on: each refusal of the plain form comes back from it."""
+    for name, base, change, reason in [
+        ("ogx_attention_fwd_lse", FWD, dict(scale=-1.0), "softmax_scale"),
+        ("ogx_attention_fwd_lse", FWD, dict(lse=None), "lse"),
+        ("ogx_attention_bwd", BWD, dict(dv=None), "gradients"),
+        ("ogx_attention_bwd", BWD, dict(workspace_bytes=1), "workspace"),
+    ]:
+        with pytest.raises(_lib.OgxError, match=reason):
+            _lib.call_packed(name, *(0 if v is None else v for v in {**base, **change}.values()))
+    slots = (ctypes.c_int64 * 64)()
+    for entry, at, count in ((0, slots, 5), (4, slots, 29), (-1, slots, 29), (0, None, 29)):
+        assert ogx_lib.ogx_call_packed(entry, at, count) == -1
