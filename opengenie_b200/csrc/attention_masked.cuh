@@ -11,6 +11,8 @@
 // while the next block runs.  9216 x 256, 32 heads: 80 us with a CTA per block, 55 so; 2 x 2304 x 1024 86 and 76.
 //   warp 0: TMA loads, and the next block   warp 1: MMA   warp 2: zeroes V's rows past the keys' length
 //   warp 3: TMA stores                      warps 4..7 (and 8..11): softmax, a query row per thread
+// At long sums the softmax sets the pace, as in the dense kernel: 9216 x 9216, 32 heads 1.11 ms = 1250 TFLOP/s, the tensor
+// pipe active for 62 % of the cycles; causal by tokens 0.61 ms; 28,800 tokens, 4 heads, causal by 1800 0.75 ms.
 // With N = 2 (one CTA per SM) each key tile is read once for 256 rows; with N = 1 (two CTAs per SM) fewer rows are
 // wasted on an odd or single tile.
 #pragma once
