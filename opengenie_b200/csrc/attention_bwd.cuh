@@ -276,8 +276,16 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
   const int head0 = kv_head * p.heads_per_kv + (per_head > 0 ? begin / per_head : 0);
   const int tile0 = first_tile + (per_head > 0 ? begin % per_head : 0);
   float* part = p.dkdv_parts + (static_cast<int64_t>(idx) * p.dkdv_splits + split) * (2 * BT * HD);
-  // the last query tile of each head has rows past the sequence's length, holding the caller's memory
-  const bool fix = vis.q_len < p.L && vis.q_len % BT != 0;
+  // Rows that hold the caller's memory, whatever that is: those past the sequence's length in each head's last query
+  // tile, and in its first one those that causality leaves without keys (more queries than keys).  0 * NaN in the dV and
+  // dK products, which sum over these rows, would reach every key, so warp 2 zeroes them.
+  const int tail = vis.q_len < p.L ? vis.q_len % BT : 0;  // the first row past the length, 0: none in the tile
+  const int blind = p.causal_block > 0 ? max(-vis.shift - first_tile * BT, 0) : 0;  // rows [0, blind) see no key
+  const auto zeroes = [&](int j) {  // whether this CTA's tile j has such rows
+    if (tail == 0 && blind == 0) return false;
+    const int at = (begin + j) % per_head;
+    return (blind > 0 && at == 0) || (tail > 0 && at == per_head - 1);
+  };
 
   if (n == 0) {
     if (warp >= 4 && p.dkdv_splits > 1) {
@@ -356,11 +364,11 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
       const uint32_t k_addr = smem_u32(k_tile), v_addr = smem_u32(v_tile);
       const uint32_t q_addr = smem_u32(q_tiles), do_addr = smem_u32(do_tiles);
       uint32_t requests = 0;
-      // Q of tile j in shared memory; in a head's last tile with its rows and dO's past the length zeroed
+      // Q of tile j in shared memory, the rows of Q and dO that hold anything zeroed
       auto q_ready = [&](int j) {
         const int s = j % B_STAGES;
         if (!mbar_wait(&st.a_full[s], (j / B_STAGES) & 1, abort)) return false;
-        if (fix && (begin + j + 1) % per_head == 0) {
+        if (zeroes(j)) {
           if (!mbar_wait(&st.b_full[s], (j / B_STAGES) & 1, abort)) return false;
           mbar_arrive(&st.zero_request);
           if (!mbar_wait(&st.zeroed, requests++ & 1, abort)) return false;
@@ -412,16 +420,20 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
       mbar_wait(&st.done, 0, nullptr);
     }
   } else if (warp == 2) {
-    if (fix) {
-      // ---------------------------------------------------------- zeroes the rows past the queries' length
+    if (tail > 0 || blind > 0) {
+      // ---------------------------------------------------------- zeroes the query rows that hold anything
       uint32_t request = 0;
-      for (int j = per_head - 1 - begin % per_head; j < n; j += per_head) {
+      for (int j = 0; j < n; ++j) {
+        if (!zeroes(j)) continue;
         const int s = j % B_STAGES;
         const uint32_t ph = (j / B_STAGES) & 1;
         if (!mbar_wait(&st.zero_request, request++ & 1, abort)) break;
         if (!mbar_wait(&st.a_full[s], ph, abort) || !mbar_wait(&st.b_full[s], ph, abort)) break;
-        zero_rows(q_tiles + s * T_BYTES, T_HALF_BYTES, vis.q_len % BT, BT, lane);
-        zero_rows(do_tiles + s * T_BYTES, T_HALF_BYTES, vis.q_len % BT, BT, lane);
+        const int at = (begin + j) % per_head;
+        for (uint8_t* tile : {q_tiles + s * T_BYTES, do_tiles + s * T_BYTES}) {
+          if (at == 0) zero_rows(tile, T_HALF_BYTES, 0, blind, lane);
+          if (tail > 0 && at == per_head - 1) zero_rows(tile, T_HALF_BYTES, tail, BT, lane);
+        }
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&st.zeroed);
