@@ -168,6 +168,21 @@ __device__ __forceinline__ f2 ex2_poly2_sum(f2 x) {
             __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23))};
 }
 
+// The running maximum of a row before its first score: the lowest finite one, so that scores of -inf add nothing.
+constexpr float kNoScore = -3.40282347e38f;
+
+// Maxima that are NaN where an operand is (fmaxf and max3 drop it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // A thread's row of 64 fp32 columns in tensor memory, times `scale`, as bf16 into its place of a 64-column half tile
 // that a TMA store takes (128-byte rows, 128-byte swizzle).  Stored straight from registers, every instruction would
 // touch 32 rows: 4800 cycles for a 256-row block at 8 KB between rows; the staging takes 1700, and the store (2100, 30
@@ -516,7 +531,7 @@ __global__ void __launch_bounds__(MaskedShape<N>::THREADS, N == 2 ? 1 : 2)
       const int64_t batch_head = static_cast<int64_t>(blk.batch) * p.heads + row_head;
       // visible keys from this CTA's first one on
       const int limit = blk.vis.limit(token) - blk.tile0 * BKV;
-      float m_run = -INFINITY;  // running max, already multiplied by c
+      float m_run = kNoScore;  // running max, already multiplied by c
       float l_run = 0.f;
       for (int j = 0; j < nkv; ++j) {
         const int t = base + j;
@@ -542,25 +557,22 @@ __global__ void __launch_bounds__(MaskedShape<N>::THREADS, N == 2 ? 1 : 2)
         float mq[4];
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-          float m = fmaxf(sf[h * 16], sf[h * 16 + 15]);
+          float m = max_nan(sf[h * 16], sf[h * 16 + 15]);
 #pragma unroll
-          for (int i = 1; i < 15; i += 2) m = max3(m, sf[h * 16 + i], sf[h * 16 + i + 1]);
+          for (int i = 1; i < 15; i += 2) m = max3_nan(m, sf[h * 16 + i], sf[h * 16 + i + 1]);
           mq[h] = m;
         }
-        const float m_tile = max3(fmaxf(mq[0], mq[1]), mq[2], mq[3]) * c;
-        float m_use = m_run;
+        const float m_tile = max3_nan(max_nan(mq[0], mq[1]), mq[2], mq[3]) * c;
         float alpha = 1.f;
         bool rescale = false;
-        if (j == 0) {
-          m_use = limit <= 0 ? 0.f : m_tile;  // a row that sees any of these keys sees the first
-        } else if (m_tile > m_run + kRescaleThreshold) {
-          m_use = m_tile;
-          alpha = ex2(m_run - m_tile);
-          rescale = true;
+        if (!(m_tile <= m_run + kRescaleThreshold)) {  // NaN, too, becomes the maximum, and stays it
+          alpha = ex2(m_run - m_tile);  // 0 at a row's first score
+          m_run = m_tile;
+          rescale = j > 0;
         }
         f2 rowsum2{0.f, 0.f};
         const f2 c2{c, c};
-        const f2 negm{-m_use, -m_use};
+        const f2 negm{-m_run, -m_run};
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
           uint32_t pk[8];
@@ -579,7 +591,6 @@ __global__ void __launch_bounds__(MaskedShape<N>::THREADS, N == 2 ? 1 : 2)
               : "memory");
         }
         l_run = l_run * alpha + (rowsum2.x + rowsum2.y);
-        m_run = m_use;
         if (__any_sync(0xffffffffu, rescale)) {
           // O must hold PV_q(t-1) before it is rescaled.  o_ready completes once per PV_q; S_q(t) was issued after
           // PV_q(t-2), so it is at most one phase behind phase t-1 here.
@@ -615,9 +626,13 @@ __global__ void __launch_bounds__(MaskedShape<N>::THREADS, N == 2 ? 1 : 2)
         }
       } else if ((ok = ok && mbar_wait(&st.o_done[q], live & 1, abort))) {
         tc_fence_after();
+        // A row without a key, or of scores of -inf alone (its sum is 0, and out 0 / 0); a row with a score of NaN or +inf
+        // is NaN (inf - inf), the log of its sum NaN or +inf.
+        if (limit <= 0 || m_run == kNoScore) m_run = -INFINITY;
+        if (!(fabsf(m_run) < INFINITY)) l_run = NAN;
         if (p.splits > 1) {
           const int64_t at_row = (batch_head * p.splits + blk.split) * p.L + token;
-          if (token < p.L) p.part_ml[at_row] = limit <= 0 ? make_float2(-INFINITY, 0.f) : make_float2(m_run, l_run);
+          if (token < p.L) p.part_ml[at_row] = make_float2(m_run, limit <= 0 ? 0.f : l_run);
 #pragma unroll 1
           for (int oc = 0; oc < 4; ++oc) {
             uint32_t orr[32];
@@ -633,7 +648,7 @@ __global__ void __launch_bounds__(MaskedShape<N>::THREADS, N == 2 ? 1 : 2)
         } else {
           if (token < p.L)
             p.lse[batch_head * p.L + token] =
-                limit <= 0 ? -INFINITY : (m_run + log2f(l_run)) * 0.6931471805599453f;
+                fabsf(m_run) == INFINITY ? m_run : (m_run + log2f(l_run)) * 0.6931471805599453f;
           // into this block's Q tile, idle since its last S_q
           uint8_t* stage = q_tiles + ((live % QB) * N + q) * Q_TILE_BYTES;
 #pragma unroll 1
@@ -660,7 +675,7 @@ __global__ void __launch_bounds__(MaskedShape<N>::THREADS, N == 2 ? 1 : 2)
 
 // Joins the splits, one warp per query row: with m_i, l_i, O_i of split i and M = max m_i,
 // O = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  Splits where a row saw no key have l = 0 and an O that was never
-// written.  The splits are added in their order.
+// written; where it saw scores of -inf alone, m = -inf and l = NaN.  The splits are added in their order.
 struct JoinParams {
   const float* part_o;
   const float2* part_ml;
@@ -681,13 +696,13 @@ __global__ void __launch_bounds__(256) attn_join_kernel(JoinParams p) {
   const int token = static_cast<int>(row - bh * p.L);
   const int64_t first = bh * p.splits * p.L + token;
   float m = -INFINITY;
-  for (int i = 0; i < p.splits; ++i) m = fmaxf(m, p.part_ml[first + static_cast<int64_t>(i) * p.L].x);
+  for (int i = 0; i < p.splits; ++i) m = max_nan(m, p.part_ml[first + static_cast<int64_t>(i) * p.L].x);
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = 0; i < p.splits; ++i) {
     const int64_t at = first + static_cast<int64_t>(i) * p.L;
     const float2 ml = p.part_ml[at];
-    if (ml.y == 0.f) continue;  // the same for the whole warp
+    if (ml.y == 0.f || (ml.x == -INFINITY && m > ml.x)) continue;  // the same for the whole warp
     const float w = exp2f(ml.x - m);
     const float4 v = reinterpret_cast<const float4*>(p.part_o + at * HD)[lane];
     l = fmaf(w, ml.y, l);
@@ -700,7 +715,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(JoinParams p) {
   const int64_t batch = bh / p.heads, head = bh - batch * p.heads;
   reinterpret_cast<uint2*>(p.out + batch * p.out_stride_b + token * p.out_stride_t + head * HD)[lane] =
       make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-  if (lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  if (lane == 0) p.lse[row] = fabsf(m) == INFINITY ? m : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 

@@ -55,3 +55,68 @@ def test_rows_that_causality_leaves_without_keys_may_hold_anything(ops, B, L, M,
     for got in results[1:]:
         for x, y in zip(got, results[0]):
             assert torch.equal(x, y)
+
+
+FORMS = [
+    # B, L, L_kv, heads, kv_heads, causal_block: one and two Q tiles per CTA, packed heads, shared key sums
+    (1, 90, 200, 2, 2, 0),
+    (2, 300, 300, 2, 1, 1),
+    (1, 1, 5000, 8, 2, 0),
+    (1, 1300, 700, 32, 32, 0),
+    (1, 1100, 1100, 32, 8, 100),
+]
+
+
+def _sees(L, M, block, key):
+    """The rows that see `key`."""
+    i = torch.arange(L, device="cuda")
+    return key // block <= torch.div(i + M - L, block, rounding_mode="floor") if block else i >= 0
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("key", [5, 50, 63, 64 + 49, -1])
+def test_a_score_that_is_nan_or_infinite_reaches_every_row_that_sees_it(ops, form, bad, key):
+    """softmax of a row with a NaN or +inf score is NaN in every column (inf - inf), and the log of its sum NaN or +inf,
+    wherever the key lies in its tile; rows that do not see the key are as they were, bit for bit."""
+    B, L, M, heads, kv_heads, block = form
+    q, k, v = _randn(M + key, (B, L, heads * D), (B, M, kv_heads * D), (B, M, kv_heads * D))
+    q[..., ::D] = q[..., ::D].abs() + 0.5  # column 0 of each head: a positive times +inf
+    args = dict(kv_heads=kv_heads, causal_block=block)
+    out, lse = ops.attention_with_lse(q, k, v, heads, **args)
+    assert torch.isfinite(lse).logical_or(lse == -math.inf).all() and torch.isfinite(out).all()
+    k[0, key, ::D] = bad
+    got, got_lse = ops.attention_with_lse(q, k, v, heads, **args)
+    assert status_clean()
+    hit = torch.zeros((B, L), dtype=torch.bool, device="cuda")
+    hit[0] = _sees(L, M, block, key % M)
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], out[~hit])
+    rows = hit[:, None].expand_as(lse)
+    assert (torch.isnan(got_lse[rows]) if math.isnan(bad) else got_lse[rows] == math.inf).all()
+    assert torch.equal(got_lse[~rows], lse[~rows])
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_scores_of_minus_infinity_weigh_nothing(ops, form):
+    """A first tile and more of scores of -inf: the other keys are what counts.  A row of nothing else is 0 / 0."""
+    B, L, M, heads, kv_heads, block = form
+    q, k, v = _randn(M, (B, L, heads * D), (B, M, kv_heads * D), (B, M, kv_heads * D))
+    q[..., ::D] = q[..., ::D].abs() + 0.5
+    k[:, :130, ::D] = -math.inf
+    out, lse = ops.attention_with_lse(q, k, v, heads, kv_heads=kv_heads, causal_block=block)
+    assert status_clean()
+    sees = torch.stack([_sees(L, M, block, j) for j in range(M)], -1)
+    one = lambda x, h: x.double().unflatten(-1, (-1, D))[..., h, :]  # noqa: E731
+    for h in range(heads):
+        s = one(q, h) @ one(k, h * kv_heads // heads).transpose(-1, -2) * D ** -0.5
+        s = s.masked_fill(~sees, -math.inf)
+        p, values = torch.softmax(s, -1), one(v, h * kv_heads // heads)
+        none = ~(s > -math.inf).any(-1)
+        blind = ~sees.any(-1).expand_as(none)
+        assert torch.isnan(one(out, h)[none & ~blind]).all() and not one(out, h)[blind].any()
+        # P and the output are rounded to bf16 once each (2^-8 at most), and an eighth of it for the rest
+        tol = 2.0 ** -8 * 9 / 8 * ((p @ values).abs() + p @ values.abs())
+        assert ((one(out, h) - p @ values).abs() <= tol)[~none].all()
+        want = torch.logsumexp(s, -1)
+        assert torch.equal(lse[:, h] == -math.inf, none)
+        assert ((lse[:, h].double() - want).abs() <= 2.0 ** -12)[~none].all()
