@@ -140,6 +140,19 @@ __device__ __forceinline__ void zero_row(__nv_bfloat16* dst, int columns) {
   for (int i = 0; i < columns / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
 }
 
+// ex2_poly2 whose power of two is a factor: added to the bits of a NaN, as there, it would make a finite number of it.
+__device__ __forceinline__ f2 ex2_poly2_nan(f2 x) {
+  const f2 magic{12583039.0f, 12583039.0f};  // 1.5 * 2^23 and the exponent's bias
+  x.x = max_nan(x.x, -126.0f);
+  x.y = max_nan(x.y, -126.0f);
+  const f2 t = add2(x, magic);
+  const f2 f = sub2(x, sub2(t, magic));
+  f2 p = fma2(f2{0.0551716648f, 0.0551716648f}, f, f2{0.2426111251f, 0.2426111251f});
+  p = fma2(p, f, f2{0.6932609677f, 0.6932609677f});
+  p = fma2(p, f, f2{0.9999280572f, 0.9999280572f});
+  return mul2(p, f2{__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23)});
+}
+
 // 32 scores of a row to probabilities: exp2(score * c + offset), three quarters on the MUFU and one on the FMA pipe.
 // offset(i): the offsets of columns i .. i + 3.
 template <typename Offset>
@@ -150,8 +163,8 @@ __device__ __forceinline__ void probabilities(float* s, float c, Offset offset) 
     const bool poly = i >= 24;
     const f2 a = fma2(f2{s[i], s[i + 1]}, f2{c, c}, f2{o.x, o.y});
     const f2 b = fma2(f2{s[i + 2], s[i + 3]}, f2{c, c}, f2{o.z, o.w});
-    const f2 pa = poly ? ex2_poly2(a) : f2{ex2(a.x), ex2(a.y)};
-    const f2 pb = poly ? ex2_poly2(b) : f2{ex2(b.x), ex2(b.y)};
+    const f2 pa = poly ? ex2_poly2_nan(a) : f2{ex2(a.x), ex2(a.y)};
+    const f2 pb = poly ? ex2_poly2_nan(b) : f2{ex2(b.x), ex2(b.y)};
     s[i] = pa.x;
     s[i + 1] = pa.y;
     s[i + 2] = pb.x;

@@ -120,3 +120,41 @@ def test_scores_of_minus_infinity_weigh_nothing(ops, form):
         want = torch.logsumexp(s, -1)
         assert torch.equal(lse[:, h] == -math.inf, none)
         assert ((lse[:, h].double() - want).abs() <= 2.0 ** -12)[~none].all()
+
+
+@pytest.mark.parametrize("L,M", [(200, 200), (40, 700), (4000, 40), (1000, 300)])
+@pytest.mark.parametrize("at", [3, 27, 31])
+def test_values_that_are_not_finite_reach_the_gradients(ops, L, M, at):
+    """What one row or key that is NaN makes of the gradients, by their formulas: a query's NaN reaches its dq and every dk
+    and dv, a key's every gradient, a value's dq and dk (dv = P^T dout does not read it), an infinite score all but the dv
+    of keys whose P = exp(s - inf) is 0.  The other batch and head keep their bits."""
+    heads = 2
+    clean = _randn(L + M, (2, L, heads * D), (2, M, heads * D), (2, M, heads * D), (2, L, heads * D))
+    clean[0][..., ::D] = clean[0][..., ::D].abs() + 0.5
+
+    def gradients(q, k, v, dout):
+        out, lse = ops.attention_with_lse(q, k, v, heads)
+        grads = ops.attention_backward(dout, q, k, v, out, lse, heads)
+        assert status_clean()
+        return grads
+
+    want = gradients(*clean)
+    for n, column, value, finite in ((0, slice(D), math.nan, (True, False, False)),
+                                     (1, slice(D), math.nan, (False, False, False)),
+                                     (2, slice(D), math.nan, (False, False, True)),
+                                     (1, slice(1), math.inf, (False, False, None)),
+                                     (3, slice(D), math.nan, (True, False, False))):
+        given = [t.clone() for t in clean]
+        given[n][1, at, column] = value
+        for i, (got, ref) in enumerate(zip(gradients(*given), want)):
+            assert torch.equal(got[0], ref[0]) and torch.equal(got[1, :, D:], ref[1, :, D:])
+            here = got[1, :, :D]
+            if finite[i]:  # dq but for the query's own row, or all of dv
+                rest = torch.arange(here.shape[0], device="cuda") != at if i == 0 else slice(None)
+                assert torch.equal(here[rest], ref[1, :, :D][rest])
+                assert i == 2 or torch.isnan(here[at]).all()
+            elif finite[i] is None:
+                rest = torch.arange(M, device="cuda") != at
+                assert torch.isnan(here[at]).all() and here[rest].abs().max() < 1e-30
+            else:
+                assert torch.isnan(here).all()
