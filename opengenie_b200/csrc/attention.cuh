@@ -95,9 +95,15 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// Maxima that are NaN where an operand is (fmaxf drops it).
+__device__ __forceinline__ float max_nan(float a, float b) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -330,19 +336,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       float mq[4];
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        float m = fmaxf(sf[h * 16], sf[h * 16 + 15]);
+        float m = max_nan(sf[h * 16], sf[h * 16 + 15]);
 #pragma unroll
-        for (int i = 1; i < 15; i += 2) m = max3(m, sf[h * 16 + i], sf[h * 16 + i + 1]);
+        for (int i = 1; i < 15; i += 2) m = max3_nan(m, sf[h * 16 + i], sf[h * 16 + i + 1]);
         mq[h] = m;
       }
-      float mx = max3(fmaxf(mq[0], mq[1]), mq[2], mq[3]);
+      float mx = max3_nan(max_nan(mq[0], mq[1]), mq[2], mq[3]);
       const float m_tile = mx * c;
       float m_use = m_run;
       float alpha = 1.f;
       bool rescale = false;
       if (j == 0) {
         m_use = m_tile;
-      } else if (m_tile > m_run + kRescaleThreshold) {
+      } else if (!(m_tile <= m_run + kRescaleThreshold)) {  // NaN, too, becomes the maximum, and stays it
         m_use = m_tile;
         alpha = ex2(m_run - m_tile);
         rescale = true;
@@ -391,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && mbar_wait(&st.o_done[q], 0, abort)) {
       tc_fence_after();
       const int token = q_block0 + q * BQ + row;
-      const float inv_l = 1.f / l_run;
+      // a row with a score of NaN or +inf is NaN (inf - inf)
+      const float inv_l = fabsf(m_run) < INFINITY ? 1.f / l_run : NAN;
       if constexpr (OUT_E4M3) {
         // e4m3 rows are 128 bytes.  Each thread owns one row, so storing straight from registers
         // would scatter 32 rows per instruction; instead the warp stages its 32 quantised rows in
@@ -798,18 +805,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       float mq[8];
 #pragma unroll
       for (int h = 0; h < 8; ++h) {
-        float m = fmaxf(sf[h * 16], sf[h * 16 + 15]);
+        float m = max_nan(sf[h * 16], sf[h * 16 + 15]);
 #pragma unroll
-        for (int i = 1; i < 15; i += 2) m = max3(m, sf[h * 16 + i], sf[h * 16 + i + 1]);
+        for (int i = 1; i < 15; i += 2) m = max3_nan(m, sf[h * 16 + i], sf[h * 16 + i + 1]);
         mq[h] = m;
       }
-      const float m_tile = fmaxf(max3(mq[0], mq[1], mq[2]), max3(mq[3], mq[4], max3(mq[5], mq[6], mq[7]))) * c;
+      const float m_tile = max_nan(max3_nan(mq[0], mq[1], mq[2]), max3_nan(mq[3], mq[4], max3_nan(mq[5], mq[6], mq[7]))) * c;
       float m_use = m_run;
       float alpha = 1.f;
       bool rescale = false;
       if (j == g) {
         m_use = m_tile;
-      } else if (m_tile > m_run + kRescaleThreshold) {
+      } else if (!(m_tile <= m_run + kRescaleThreshold)) {  // NaN, too, becomes the maximum, and stays it
         m_use = m_tile;
         alpha = ex2(m_run - m_tile);
         rescale = true;
@@ -868,7 +875,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     named_bar_sync(1, 256);
     const bool two = nkv > 1;  // group 1 has key tiles (else its O was never written)
     const float m0 = st.red[0][0][row], m1 = st.red[1][0][row];
-    const float m = two ? fmaxf(m0, m1) : m0;
+    const float m = two ? max_nan(m0, m1) : m0;
     const float a0 = ex2(m0 - m);
     const float a1 = two ? ex2(m1 - m) : 0.f;
     const float inv_l = 1.f / (st.red[0][1][row] * a0 + st.red[1][1][row] * a1);

@@ -171,18 +171,6 @@ __device__ __forceinline__ f2 ex2_poly2_sum(f2 x) {
 // The running maximum of a row before its first score: the lowest finite one, so that scores of -inf add nothing.
 constexpr float kNoScore = -3.40282347e38f;
 
-// Maxima that are NaN where an operand is (fmaxf and max3 drop it).
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 // A thread's row of 64 fp32 columns in tensor memory, times `scale`, as bf16 into its place of a 64-column half tile
 // that a TMA store takes (128-byte rows, 128-byte swizzle).  Stored straight from registers, every instruction would
 // touch 32 rows: 4800 cycles for a 256-row block at 8 KB between rows; the staging takes 1700, and the store (2100, 30

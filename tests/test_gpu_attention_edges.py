@@ -158,3 +158,17 @@ def test_values_that_are_not_finite_reach_the_gradients(ops, L, M, at):
                 assert torch.isnan(here[at]).all() and here[rest].abs().max() < 1e-30
             else:
                 assert torch.isnan(here).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("key", [5, 50, 120, 199])
+def test_dense_attention_with_a_score_that_is_nan_or_infinite(ops, bad, key):
+    """The dense attention, too: NaN in every row of that head and batch, the others as they were."""
+    q, k, v = _randn(key, (2, 300, 2 * D), (2, 200, 2 * D), (2, 200, 2 * D))
+    q[..., ::D] = q[..., ::D].abs() + 0.5
+    want = ops.attention(q, k, v, 2)
+    k[1, key, D] = bad
+    got = ops.attention(q, k, v, 2)
+    assert status_clean()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1, :, :D], want[1, :, :D])
+    assert torch.isnan(got[1, :, D:]).all()
