@@ -368,10 +368,11 @@ int ogx_attention_fwd_e4m3_to_peers(const void* q, const void* k, const void* v,
  * causal_block 1 is the token-causal mask with both sequences ending together, n a mask over blocks of n
  * positions (the tokens of a latent frame).  out: bf16 [batch, q_tokens, heads*128]; lse: f32 [batch, heads,
  * q_tokens], the natural log of each row's sum of exponentials.  A row that sees no key gets out = 0 and lse =
- * -inf.  Keys and values past kv_lengths may hold anything (NaN included).  out may be q, but not k or v.  Few queries over many keys are shared out
- * over the keys and joined in a second launch; workspace (device memory, 16-byte aligned, overwritten; calls that may
- * run at the same time need one each) holds the parts: ogx_attention_fwd_lse_workspace says how much, often 0 (then
- * it may be NULL). */
+ * -inf; a score of NaN or +inf among those a row sees makes its out NaN and its lse NaN or +inf.  Keys and values past
+ * kv_lengths may hold anything (NaN included).  out may be q with its strides; any other overlap of the memory that is
+ * written with an input is refused.  Few queries over many keys are shared out over the keys and joined in a second
+ * launch; workspace (device memory, 16-byte aligned, overwritten; calls that may run at the same time need one each)
+ * holds the parts: ogx_attention_fwd_lse_workspace says how much, often 0 (then it may be NULL). */
 int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t batch, int64_t q_tokens,
                           int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,
                           int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t, int64_t v_stride_b,
@@ -389,10 +390,10 @@ int ogx_attention_bwd_workspace(int64_t batch, int64_t q_tokens, int64_t kv_toke
 
 /* Gradients of ogx_attention_fwd_lse: from dout (the gradient of out), the forward's inputs, out and lse, dq
  * [batch, q_tokens, heads*128] and dk, dv [batch, kv_tokens, kv_heads*128] (bf16, own strides), every element
- * written; they must not overlap an input.  The probabilities are recomputed from lse.  Rows past q_lengths and
- * rows that see no key get dq = 0 and give nothing to dk and dv (their q and dout may hold anything); keys past
- * kv_lengths get dk = dv = 0.  workspace: device memory, 16-byte aligned, overwritten; calls that may run at the
- * same time need one each. */
+ * written; overlaps with an input or one another are refused.  The probabilities are recomputed from lse.  Rows past
+ * q_lengths and rows that see no key get dq = 0 and give nothing to dk and dv (their q and dout may hold anything);
+ * keys past kv_lengths get dk = dv = 0.  workspace: device memory, 16-byte aligned, overwritten; calls that may run at
+ * the same time need one each. */
 int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
                       const float* lse, int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
                       int64_t kv_heads, int64_t head_dim, int64_t dout_stride_b, int64_t dout_stride_t,
@@ -414,8 +415,8 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
  * 16) turn by the token's angles: columns (j, j + rotary/2), or (2j, 2j + 1) with interleaved != 0, by entry j of
  * cos and sin.  The tables are bf16 or f32 with unit column stride and strides cs_stride_b (0: shared by the
  * batch), cs_stride_h (0: shared by the heads; otherwise heads == kv_heads) and cs_stride_t, multiples of 8.
- * The outputs may be the inputs (in place).  With OGX_NORM_ROW and the half layout this is the arithmetic of
- * ogx_video_qk_rmsnorm_rope at other widths, batches and head counts. */
+ * An output may be its input with its strides (in place); any other overlap is refused.  With OGX_NORM_ROW and the half
+ * layout this is the arithmetic of ogx_video_qk_rmsnorm_rope at other widths, batches and head counts. */
 int ogx_qk_norm_rope(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                      int64_t head_dim, int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
                      const void* q_weight, const void* k_weight, int weight_dtype, int norm, float eps,
@@ -430,8 +431,8 @@ int ogx_qk_norm_rope_bwd_workspace(int64_t batch, int64_t tokens, int64_t heads,
                                    int norm, int64_t* bytes);
 
 /* Gradients of ogx_qk_norm_rope: from those of its outputs (dq_out, dk_out) and its inputs, dq and dk (bf16, own
- * strides; they may be dq_out and dk_out) and the weights' dq_weight, dk_weight (f32, summed over all rows; not
- * written for OGX_NORM_NONE).  workspace as for ogx_attention_bwd (may be NULL for OGX_NORM_NONE). */
+ * strides; each may be the output gradient or the input it belongs to, with its strides, other overlaps are refused) and
+ * the weights' dq_weight, dk_weight (f32, summed over all rows; not written for OGX_NORM_NONE).  workspace as for ogx_attention_bwd (may be NULL for OGX_NORM_NONE). */
 int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq_out_stride_t, const void* dk_out,
                          int64_t dk_out_stride_b, int64_t dk_out_stride_t, const void* q, const void* k, int64_t batch,
                          int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,

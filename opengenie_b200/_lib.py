@@ -16,6 +16,7 @@ LIB_NAME = "libogx.so"
 LIB_PATH = os.environ.get("OPENGENIE_B200_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 
 OGX_OK = 0
+OGX_EINVAL = -1
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
 DTYPE_F16 = 2
@@ -176,6 +177,10 @@ class OgxError(RuntimeError):
     """A C-ABI call returned an error; the message is ogx_last_error()."""
 
 
+class OgxArgumentError(OgxError, ValueError):
+    """The call was turned down for its arguments, before anything ran."""
+
+
 def load() -> ctypes.CDLL:
     """Loads libogx.so from the package directory (built by ``opengenie_b200.build``)."""
     global _LIB
@@ -197,13 +202,18 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+def _error(lib: ctypes.CDLL, name: str, rc: int) -> OgxError:
+    msg = lib.ogx_last_error().decode(errors="replace")
+    return (OgxArgumentError if rc == OGX_EINVAL else OgxError)(f"{name}: {msg}" if msg else f"{name}: error {rc}")
+
+
 def call(name: str, *args) -> None:
-    """Calls an entry point and raises OgxError (reason string from the library) on failure."""
+    """Calls an entry point and raises OgxError (reason string from the library) on failure, OgxArgumentError where a
+    guard turned the arguments down."""
     lib = load()
     rc = getattr(lib, name)(*args)
     if rc != OGX_OK:
-        msg = lib.ogx_last_error().decode(errors="replace")
-        raise OgxError(f"{name}: {msg}" if msg else f"{name}: error {rc}")
+        raise _error(lib, name, rc)
 
 
 # The entry points that ``call_packed`` reaches, in the order of their OGX_CALL_* numbers: (number, packer, slots).
@@ -220,8 +230,7 @@ def call_packed(name: str, *args) -> None:
     entry, pack, count = _PACKED[name]
     rc = lib.ogx_call_packed(entry, pack(*args), count)
     if rc != OGX_OK:
-        msg = lib.ogx_last_error().decode(errors="replace")
-        raise OgxError(f"{name}: {msg}" if msg else f"{name}: error {rc}")
+        raise _error(lib, name, rc)
 
 
 OGX_ERR_TIMEOUT = 1  # device status bit: a bounded device-side wait gave up

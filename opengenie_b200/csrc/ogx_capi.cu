@@ -28,6 +28,7 @@
 #include "rows.cuh"
 #include "fp8_gemm.cuh"
 #include "peer.cuh"
+#include "regions.h"
 
 namespace {
 
@@ -1447,6 +1448,12 @@ int ogx_peer_barrier_static(int rank, int world, const int* devices, unsigned in
 // ------------------------------------------------------------- training pass: attention with statistics, gradients
 namespace {
 
+using ogx::flat_region;
+using ogx::Output;
+using ogx::outputs_ok;
+using ogx::Region;
+using ogx::rows_region;
+
 // {d, head, token, batch} map of bf16 rows of heads * 128 columns; a box is 64 columns of `box_rows` tokens.
 int token_map(CUtensorMap* map, const void* base, int64_t heads, int64_t tokens, int64_t batch, int64_t stride_t,
               int64_t stride_b, int box_rows, int box_heads = 1) {
@@ -1637,6 +1644,17 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
   const int64_t parts = fwd_part_rows(batch, q_tokens, heads, splits);
   if (splits > 1 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < parts * (ogx::attn::HD + 2) * 4))
     return fail(OGX_EINVAL, "workspace");
+  const int64_t width = heads * 128, kv_width = kv_heads * 128;
+  const Region inputs[] = {rows_region(q, 2, width, batch, q_stride_b, q_tokens, q_stride_t),
+                           rows_region(k, 2, kv_width, batch, k_stride_b, kv_tokens, k_stride_t),
+                           rows_region(v, 2, kv_width, batch, v_stride_b, kv_tokens, v_stride_t),
+                           flat_region(q_lengths, batch * 4), flat_region(kv_lengths, batch * 4)};
+  // every block reads its own rows of q before it writes those of out
+  const Output outputs[] = {{rows_region(out, 2, width, batch, out_stride_b, q_tokens, out_stride_t), {0, -1}},
+                            {flat_region(lse, batch * heads * q_tokens * 4), {-1, -1}},
+                            {flat_region(splits > 1 ? workspace : nullptr, parts * (ogx::attn::HD + 2) * 4), {-1, -1}}};
+  if (!outputs_ok(outputs, inputs))
+    return fail(OGX_EINVAL, "out_alias: out must be memory of its own, or q with its strides");
   CUtensorMap mq, mk, mv, mo;
   const int pack = 1 << plan.pack_shift;
   const int box = ogx::attn::BQ / pack;
@@ -1738,6 +1756,18 @@ int ogx_attention_bwd(const void* dout, const void* q, const void* k, const void
   const int64_t dkdv_ctas = kv_tiles * kv_heads * batch * ws.dkdv_splits;
   const int64_t dq_ctas = q_tiles * heads * batch * ws.dq_splits;
   if (dkdv_ctas + dq_ctas > INT32_MAX) return fail(OGX_EINVAL, "shape");
+  const Region inputs[] = {rows_region(dout, 2, width, batch, dout_stride_b, q_tokens, dout_stride_t),
+                           rows_region(q, 2, width, batch, q_stride_b, q_tokens, q_stride_t),
+                           rows_region(k, 2, kv_width, batch, k_stride_b, kv_tokens, k_stride_t),
+                           rows_region(v, 2, kv_width, batch, v_stride_b, kv_tokens, v_stride_t),
+                           rows_region(out, 2, width, batch, out_stride_b, q_tokens, out_stride_t),
+                           flat_region(lse, batch * heads * q_tokens * 4), flat_region(q_lengths, batch * 4),
+                           flat_region(kv_lengths, batch * 4)};
+  const Output outputs[] = {{rows_region(dq, 2, width, batch, dq_stride_b, q_tokens, dq_stride_t), {-1, -1}},
+                            {rows_region(dk, 2, kv_width, batch, dk_stride_b, kv_tokens, dk_stride_t), {-1, -1}},
+                            {rows_region(dv, 2, kv_width, batch, dv_stride_b, kv_tokens, dv_stride_t), {-1, -1}},
+                            {flat_region(workspace, ws.bytes), {-1, -1}}};
+  if (!outputs_ok(outputs, inputs)) return fail(OGX_EINVAL, "grads_alias: dq, dk and dv must be memory of their own");
   CUtensorMap mq, mk, mv, mdo, mdq, mdk, mdv;
   if ((rc = token_map(&mq, q, heads, q_tokens, batch, q_stride_t, q_stride_b, ogx::attn::BT))) return rc;
   if ((rc = token_map(&mdo, dout, heads, q_tokens, batch, dout_stride_t, dout_stride_b, ogx::attn::BT))) return rc;
@@ -1979,6 +2009,19 @@ ogx::qkn::Params qk_params(const void* q, const void* k, int64_t batch, int64_t 
   return p;
 }
 
+// cos or sin
+Region qk_table(const void* base, int64_t batch, int64_t tokens, int64_t heads, int cs_dtype, int64_t rotary,
+                int64_t stride_b, int64_t stride_h, int64_t stride_t) {
+  const int64_t size = cs_dtype == OGX_DTYPE_F32 ? 4 : 2;
+  return Region{static_cast<const char*>(base), rotary / 2 * size,
+                {stride_b ? batch : 1, stride_h ? heads : 1, stride_t ? tokens : 1},
+                {stride_b * size, stride_h * size, stride_t * size}};
+}
+Region qk_weight(const void* base, int weight_dtype, int norm, int64_t heads, int64_t head_dim) {
+  return flat_region(norm == kNone ? nullptr : base,
+                     qk_weight_columns(norm, heads, head_dim) * (weight_dtype == OGX_DTYPE_F32 ? 4 : 2));
+}
+
 int qk_outputs(ogx::qkn::Params& p, const QkShape (&sh)[2], void* y_q, int64_t q_stride_b, int64_t q_stride_t, void* y_k,
                int64_t k_stride_b, int64_t k_stride_t) {
   if (y_q == nullptr || y_k == nullptr || !aligned16(y_q) || !aligned16(y_k) || q_stride_b % 8 || q_stride_t % 8 ||
@@ -2010,6 +2053,18 @@ int ogx_qk_norm_rope(const void* q, const void* k, int64_t batch, int64_t tokens
                                  k_stride_t, q_weight, k_weight, weight_dtype, norm, eps, cos, sin, cs_dtype, rotary,
                                  cs_stride_b, cs_stride_h, cs_stride_t, false, sh, &steps);
   if ((rc = qk_outputs(p, sh, q_out, q_out_stride_b, q_out_stride_t, k_out, k_out_stride_b, k_out_stride_t))) return rc;
+  const int64_t width = heads * head_dim, kv_width = kv_heads * head_dim;
+  const Region inputs[] = {
+      rows_region(q, 2, width, batch, q_stride_b, tokens, q_stride_t),
+      rows_region(k, 2, kv_width, batch, k_stride_b, tokens, k_stride_t),
+      qk_weight(q_weight, weight_dtype, norm, heads, head_dim), qk_weight(k_weight, weight_dtype, norm, kv_heads, head_dim),
+      qk_table(cos, batch, tokens, heads, cs_dtype, rotary, cs_stride_b, cs_stride_h, cs_stride_t),
+      qk_table(sin, batch, tokens, heads, cs_dtype, rotary, cs_stride_b, cs_stride_h, cs_stride_t)};
+  // the lane that writes a column has read it before
+  const Output outputs[] = {{rows_region(q_out, 2, width, batch, q_out_stride_b, tokens, q_out_stride_t), {0, -1}},
+                            {rows_region(k_out, 2, kv_width, batch, k_out_stride_b, tokens, k_out_stride_t), {1, -1}}};
+  if (!outputs_ok(outputs, inputs))
+    return fail(OGX_EINVAL, "out_alias: each output must be memory of its own, or its input with its strides");
   qk_dispatch<false>(p, head_dim, interleaved, steps, norm, static_cast<cudaStream_t>(stream));
   return check_launch("qk_norm_rope_kernel");
 }
@@ -2060,6 +2115,24 @@ int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq
     p.t[0].partials = static_cast<float*>(workspace);
     p.t[1].partials = p.t[0].partials + q_bytes / 4;
   }
+  const bool weights = norm != kNone;
+  const int64_t width = heads * head_dim, kv_width = kv_heads * head_dim;
+  const Region inputs[] = {
+      rows_region(dq_out, 2, width, batch, dq_out_stride_b, tokens, dq_out_stride_t),
+      rows_region(dk_out, 2, kv_width, batch, dk_out_stride_b, tokens, dk_out_stride_t),
+      rows_region(q, 2, width, batch, q_stride_b, tokens, q_stride_t),
+      rows_region(k, 2, kv_width, batch, k_stride_b, tokens, k_stride_t),
+      qk_weight(q_weight, weight_dtype, norm, heads, head_dim), qk_weight(k_weight, weight_dtype, norm, kv_heads, head_dim),
+      qk_table(cos, batch, tokens, heads, cs_dtype, rotary, cs_stride_b, cs_stride_h, cs_stride_t),
+      qk_table(sin, batch, tokens, heads, cs_dtype, rotary, cs_stride_b, cs_stride_h, cs_stride_t)};
+  const Output outputs[] = {
+      {rows_region(dq, 2, width, batch, dq_stride_b, tokens, dq_stride_t), {0, 2}},
+      {rows_region(dk, 2, kv_width, batch, dk_stride_b, tokens, dk_stride_t), {1, 3}},
+      {flat_region(weights ? dq_weight : nullptr, qk_weight_columns(norm, heads, head_dim) * 4), {-1, -1}},
+      {flat_region(weights ? dk_weight : nullptr, qk_weight_columns(norm, kv_heads, head_dim) * 4), {-1, -1}},
+      {flat_region(weights ? workspace : nullptr, q_bytes + qk_partial_bytes(sh[1], norm, kv_heads, head_dim)), {-1, -1}}};
+  if (!outputs_ok(outputs, inputs))
+    return fail(OGX_EINVAL, "out_alias: each output must be memory of its own, or its input with its strides");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   qk_dispatch<true>(p, head_dim, interleaved, steps, norm, s);
   if ((rc = check_launch("qk_norm_rope_kernel"))) return rc;

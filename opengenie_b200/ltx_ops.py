@@ -1156,7 +1156,8 @@ def attention_with_lse(
     n > 0, ``j // n <= (i + L_kv - L) // n``: n = 1 is the token-causal mask with both sequences ending
     together, the tokens of a latent frame make it frame-causal (a token sees its own and all earlier frames).
     ``lse`` is the natural log of a row's sum of exponentials.  A row that sees no key gets out 0 and lse
-    -inf; keys and values past ``kv_lengths`` may hold anything.  ``out`` may be q, but not k or v.
+    -inf; keys and values past ``kv_lengths`` may hold anything.  ``out`` may be q itself; any other overlap with an
+    input is refused.  A row with a score of NaN or +inf among those it sees gets out NaN and lse NaN or +inf.
 
     No reference counterpart: the reference infers with dense bidirectional attention only.
     """
@@ -1169,8 +1170,6 @@ def attention_with_lse(
         out_rows = (L * C, C)
     else:
         out_rows = _given_rows(out, q, "out_shape: out must be bf16 [B, L, heads*128] with unit column stride")
-        if out.data_ptr() in (k.data_ptr(), v.data_ptr()):  # other blocks still read them
-            raise ValueError("out_alias: out must not be k or v")
     lse = q.new_empty((B, heads, L), dtype=torch.float32)
     size = _workspace_bytes("ogx_attention_fwd_lse_workspace", q.device.index, B, L, k.shape[1], heads, kv_heads)
     workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
@@ -1204,8 +1203,8 @@ def attention_backward(
     The probabilities are recomputed from ``lse``.  Every gradient is summed in one order (dk and dv over the
     query heads that share a key head), so equal inputs give equal bits.  Rows past ``q_lengths`` and rows that
     see no key get dq 0 and give nothing to dk and dv; keys past ``kv_lengths`` get 0.  ``grads`` takes (dq, dk,
-    dv) to write into, for example the slices of one packed [B, L, (heads + 2*kv_heads)*128] buffer; none of them may
-    overlap an input.  No reference counterpart (the reference only infers).
+    dv) to write into, for example the slices of one packed [B, L, (heads + 2*kv_heads)*128] buffer; overlaps with
+    an input or one another are refused.  No reference counterpart (the reference only infers).
     """
     kv_heads = heads if kv_heads is None else kv_heads
     q_rows, k_rows, v_rows, scale = _masked_attention_args(q, k, v, heads, kv_heads, softmax_scale, causal_block,
@@ -1224,9 +1223,6 @@ def attention_backward(
         dq, dk, dv = grads
         reason = "grads: bf16 tensors of the shapes of q, k and v with unit column stride"
         dq_rows, dk_rows, dv_rows = (_given_rows(t, like, reason) for t, like in ((dq, q), (dk, k), (dv, v)))
-        given = {t.data_ptr() for t in (dq, dk, dv)}
-        if len(given) < 3 or given & {t.data_ptr() for t in (dout, q, k, v, out)}:
-            raise ValueError("grads_alias: dq, dk and dv must be tensors of their own")
     workspace = q.new_empty(
         (_workspace_bytes("ogx_attention_bwd_workspace", device.index, B, L, M, heads, kv_heads),), dtype=torch.uint8)
     _call_on(
@@ -1326,7 +1322,8 @@ def fused_qk_norm_rope(
     [heads*d] and [kv_heads*d], the video block's norm), "none" only rotates (weights None).  The first
     R = 2 * cos.shape[-1] columns of each head turn by the token's angles: columns (j, j + R/2), or (2j, 2j + 1)
     with ``interleaved``.  cos/sin (bf16 or fp32): [1|B, L, R/2] shared by the heads or [1|B, heads, L, R/2]
-    (then kv_heads == heads).  ``out`` may be (q, k) for an in-place update.
+    (then kv_heads == heads).  ``out`` may be (q, k) for an in-place update; any other overlap with an input, or of
+    the two outputs, is refused.  heads + kv_heads is at most 128.
 
     ``fused_video_qk_rmsnorm_rope`` (ltx_serve/triton_ltx_ops.py:320-378) is the case norm="row", 32 heads of
     128, B = 1; ``fused_qk_norm_rope_backward`` gives the gradients of all of them.
@@ -1370,9 +1367,9 @@ def fused_qk_norm_rope_backward(
     """Gradients of ``fused_qk_norm_rope`` (and of ``fused_video_qk_rmsnorm_rope``: norm="row"): from the
     gradients of its outputs and its inputs, (dq, dk, dq_weight, dk_weight).
 
-    dq and dk are bf16 (``out`` may be (dq_out, dk_out) for an in-place update); the weights' gradients are fp32
-    sums over all rows (and, for norm="head", heads), whatever the weights' type, and None for norm="none".  The
-    sums run in a fixed order.  No reference counterpart (the reference only infers).
+    dq and dk are bf16 (``out`` may be (dq_out, dk_out) or (q, k) for an in-place update, other overlaps are
+    refused); the weights' gradients are fp32 sums over all rows (and, for norm="head", heads), whatever the weights'
+    type, and None for norm="none".  The sums run in a fixed order.  No reference counterpart (the reference only infers).
     """
     kv_heads = heads if kv_heads is None else kv_heads
     hd, rotary, q_rows, k_rows, cs_strides = _qk_norm_rope_args(q, k, q_weight, k_weight, cos, sin, heads, kv_heads, norm)
