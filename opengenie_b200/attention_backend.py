@@ -168,6 +168,11 @@ def _linear_tensors(m) -> list:
     return [getattr(m, name, None) for name in ("weight", "weight_scale", "input_scale", "bias")]
 
 
+def _needs_gradient(*tensors) -> bool:
+    """Whether a graph has to run through these activations, which the fused branches have none of."""
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
 _MSA_BRANCH_CALLS = 0
 _MSA_BRANCH_FALLBACK_REASONS: Counter = Counter()
 _MSA_BLOCKS = _BranchCache()
@@ -187,7 +192,9 @@ def video_msa_branch(block, video, vx: torch.Tensor, *, token_counts: set[int] |
     out-projection -> bias + gate(2) + residual as five sm_100a kernels.  ``block`` provides
     ``scale_shift_table``, ``norm_eps`` and ``attn1`` (FP8 linears ``to_q/to_k/to_v/to_out[0]`` with
     ``weight``/``weight_scale``/``input_scale``/``bias``, and ``q_norm``/``k_norm`` with ``weight``/``eps``);
-    ``video`` provides ``timesteps`` and ``positional_embeddings`` (cos, sin).
+    ``video`` provides ``timesteps`` and ``positional_embeddings`` (cos, sin).  The kernels have no backward pass: where
+    ``vx`` or ``timesteps`` requires a gradient (and gradients are enabled) the branch declines, too
+    (`requires_grad`), and the caller's path runs, its attention differentiable with the ``b200-native`` backend.
     """
     global _MSA_BRANCH_CALLS
     from .synthetic import BlockWeights, Fp8Linear
@@ -206,6 +213,8 @@ def video_msa_branch(block, video, vx: torch.Tensor, *, token_counts: set[int] |
     pe = getattr(video, "positional_embeddings", None)
     if pe is None:
         return _decline("missing_rope")
+    if _needs_gradient(vx, getattr(video, "timesteps", None)):
+        return _decline("requires_grad")
     attn = block.attn1
 
     def build():
@@ -266,8 +275,9 @@ def video_text_cross_attention_branch(block, x: torch.Tensor, context: torch.Ten
     same arguments.  Declines (the caller keeps the reference's path) when the block has no cross-attention
     AdaLN or no prompt table (`no_cross_attention_adaln`, `no_prompt_table`; the reference's own branches
     :2821-2835), on shapes other than batch 1 x 4096 (`shape`, `context_shape`), a table of fewer than 9
-    slots (`table_shape`), a context mask (`mask`: pass the prompt's valid tokens as the context instead) and
-    gated attention (`gated_attention`).  Otherwise the eight launches of ``VideoTextCrossAttention``, built
+    slots (`table_shape`), a context mask (`mask`: pass the prompt's valid tokens as the context instead),
+    gated attention (`gated_attention`) and activations that require a gradient, which the kernels do not have
+    (`requires_grad`).  Otherwise the eight launches of ``VideoTextCrossAttention``, built
     once per block from its modules (and again when one of their tensors is replaced or changed in place).
     """
     global _TEXT_BRANCH_CALLS
@@ -287,6 +297,8 @@ def video_text_cross_attention_branch(block, x: torch.Tensor, context: torch.Ten
         return _decline_text("mask")
     if getattr(attn, "to_gate_logits", None) is not None:
         return _decline_text("gated_attention")
+    if _needs_gradient(x, context, timestep, prompt_timestep):
+        return _decline_text("requires_grad")
     sources = [t for m in (attn.to_q, attn.to_k, attn.to_v, attn.to_out[0]) for t in _linear_tensors(m)]
     sources += [attn.q_norm.weight, attn.k_norm.weight, block.scale_shift_table,
                 getattr(block, "prompt_scale_shift_table", None)]
