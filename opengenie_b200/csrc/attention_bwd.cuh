@@ -440,7 +440,7 @@ __device__ __forceinline__ void bwd_dkdv(const CUtensorMap* tq, const CUtensorMa
         if (!zeroes(j)) continue;
         const int s = j % B_STAGES;
         const uint32_t ph = (j / B_STAGES) & 1;
-        if (!mbar_wait(&st.zero_request, request++ & 1, abort)) break;
+        if (!mbar_wait(&st.zero_request, request++ & 1, abort, kSumWaitLimitNs)) break;
         if (!mbar_wait(&st.a_full[s], ph, abort) || !mbar_wait(&st.b_full[s], ph, abort)) break;
         const int at = (begin + j) % per_head;
         for (uint8_t* tile : {q_tiles + s * T_BYTES, do_tiles + s * T_BYTES}) {
@@ -669,7 +669,7 @@ __device__ __forceinline__ void bwd_dq(const CUtensorMap* tq, const CUtensorMap*
     if (fix_tile >= 0) {
       // ---------------------------------------------------------- zeroes the K rows past the keys' length
       const int s = fix_tile % DQ_K_STAGES;
-      if (mbar_wait(&st.zero_request, 0, abort) && mbar_wait(&st.a_full[s], (fix_tile / DQ_K_STAGES) & 1, abort)) {
+      if (mbar_wait(&st.zero_request, 0, abort, kSumWaitLimitNs) && mbar_wait(&st.a_full[s], (fix_tile / DQ_K_STAGES) & 1, abort)) {
         zero_rows(k_tiles + s * T_BYTES, T_HALF_BYTES, vis.kv_len % BT, BT, lane);
         fence_async_shared();
       }

@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(MaskedShape<N>::THREADS, N == 2 ? 1 : 2)
   // The block after item `i`, for every warp but the producer's.
   auto advance = [&](int i) {
     if (p.one_wave) return false;
-    if (!mbar_wait(&st.next_full[i & 1], (i >> 1) & 1, abort)) return false;
+    if (!mbar_wait(&st.next_full[i & 1], (i >> 1) & 1, abort, kSumWaitLimitNs)) return false;
     const bool more = read_next(&st.next[i & 1], &at);
     __syncwarp();
     if (lane == 0) mbar_arrive(&st.next_empty[i & 1]);
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(MaskedShape<N>::THREADS, N == 2 ? 1 : 2)
         const Block<N> b(p, at);
         if (b.fix_tile >= 0) {
           const int t = base + b.fix_tile;
-          if (mbar_wait(&st.v_fix_request, fixes & 1, abort) &&
+          if (mbar_wait(&st.v_fix_request, fixes & 1, abort, kSumWaitLimitNs) &&
               mbar_wait(&st.v_full[t % STAGES], (t / STAGES) & 1, abort)) {
             zero_rows(v_tiles + (t % STAGES) * KV_TILE_BYTES, KV_HALF_BYTES, b.vis.kv_len % BKV, BKV, lane);
             fence_async_shared();
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(MaskedShape<N>::THREADS, N == 2 ? 1 : 2)
             const int qb = live % QB;
             bool ok = true;
             for (int q = 0; q < N; ++q) {
-              ok = ok && mbar_wait(&st.o_read[q], live & 1, abort);
+              ok = ok && mbar_wait(&st.o_read[q], live & 1, abort, kSumWaitLimitNs);
               const int token = b.token0 + (q * BQ >> p.pack_shift);
               if (!ok || p.splits > 1 || token >= p.L) continue;
               for (int h = 0; h < 2; ++h)

@@ -1470,8 +1470,9 @@ bool row_strides_ok(int64_t width, int64_t tokens, int64_t batch, int64_t stride
   return stride_t < (int64_t{1} << 38) && (batch == 1 || stride_b < (int64_t{1} << 38)) && tokens > 0;
 }
 
-// Tokens: positions and tile ends stay far below 2^31, and the sum over one row's keys takes less time than a wait's
-// limit (0.5 s), since some warps wait for the whole of it.
+// Tokens: positions and tile ends stay far below 2^31, and a sum over one row's keys, which some warps wait for as a whole,
+// takes far less than such a wait's limit of 8 s (kSumWaitLimitNs): at 2^25 keys 0.52 s with two Q tiles per CTA and 0.62 s
+// with one (0.99 us per 64 keys, and 1.32 x 0.9 us), an eighth more under the power cap; lower clocks have the rest.
 constexpr int64_t kMostTokens = int64_t{1} << 25;
 
 bool attention_sizes_ok(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads) {

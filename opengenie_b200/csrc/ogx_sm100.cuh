@@ -26,6 +26,9 @@ namespace ogx {
 
 // A wait gives up after this many nanoseconds of polling (about one second).
 constexpr unsigned long long kWaitLimitNs = 1000000000ull;
+// The limit of a wait for a whole sum over a sequence, which the warps that make the sum wait for step by step: where one
+// of those steps runs out, the abort flag ends this wait too, long before its own limit.
+constexpr unsigned long long kSumWaitLimitNs = 8 * kWaitLimitNs;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -97,14 +100,15 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // Waits until the phase with the given parity of `bar` has completed.
 // `abort` (shared memory, may be null) lets a CTA that already failed stop
 // waiting early.  Returns false (and records a timeout) if the wait ran out.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort = nullptr) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort = nullptr,
+                                          unsigned long long limit_ns = kWaitLimitNs) {
   if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long t0 = global_ns();
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 63u) == 0u) {
       if (abort != nullptr && *abort) return false;
-      if (global_ns() - t0 > kWaitLimitNs) {
+      if (global_ns() - t0 > limit_ns) {
         atomicOr(&g_ogx_status, OGX_ERR_TIMEOUT);
         if (abort != nullptr) *abort = 1;
         return false;

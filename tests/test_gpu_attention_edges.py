@@ -172,3 +172,27 @@ def test_dense_attention_with_a_score_that_is_nan_or_infinite(ops, bad, key):
     assert status_clean()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1, :, :D], want[1, :, :D])
     assert torch.isnan(got[1, :, D:]).all()
+
+
+def test_rows_of_the_largest_length(ops):
+    """2^25 keys, the most that is taken, with enough queries that no row's sum is shared out: some warps wait for the
+    whole of it.  Equal scores: P = 1, the sum 2^25 and the mean of the values, which are 1 or -1 by turns of 64 keys and
+    3 at one key in 1024."""
+    n, rows = 1 << 25, 148 * 256
+    if torch.cuda.mem_get_info()[0] < 3 * n * D * 2:
+        pytest.skip("not enough free memory")
+    q = torch.zeros((1, rows, D), device="cuda", dtype=BF)
+    k = torch.zeros((1, n, D), device="cuda", dtype=BF)
+    v = torch.ones((1, n, D), device="cuda", dtype=BF)
+    v.view(1, n // 128, 2, 64, D)[:, :, 1] = -1
+    v.view(1, n // 1024, 1024, D)[:, :, 5] = 3  # 1 before
+    from opengenie_b200 import _lib
+
+    assert ops._workspace_bytes("ogx_attention_fwd_lse_workspace", 0, 1, rows, n, 1, 1) == 0
+    lengths = torch.tensor([n - 3], device="cuda", dtype=torch.int32)  # and a last tile with rows to zero
+    out, lse = ops.attention_with_lse(q, k, v, 1, kv_lengths=lengths)
+    assert _lib.device_status() == 0
+    # the products' sums are whole numbers below 2^24; the sum of P, 2^19 tiles in 32 bits, is off by 2^19 2^-24 at most
+    assert (lse - math.log(n - 3)).abs().max() <= 2.0 ** -5
+    mean = (2 * (n / 1024) + 3) / (n - 3)
+    assert ((out.double() - mean).abs() <= mean * (2.0 ** -8 + 2.0 ** -5)).all()
