@@ -196,3 +196,21 @@ def test_rows_of_the_largest_length(ops):
     assert (lse - math.log(n - 3)).abs().max() <= 2.0 ** -5
     mean = (2 * (n / 1024) + 3) / (n - 3)
     assert ((out.double() - mean).abs() <= mean * (2.0 ** -8 + 2.0 ** -5)).all()
+
+
+@pytest.mark.parametrize("chunk", range(4))
+@pytest.mark.parametrize("L,M", [(40, 64), (1300, 64), (40, 5000)])
+def test_statistics_of_short_rows_are_as_exact_as_32_bits(ops, chunk, L, M):
+    """Rows whose weight lies in one chunk of 16 keys, one of which has its exponentials from a polynomial (off by 2.7e-6 at
+    most; hardware's by 2^-22).  The scores are exact: small whole numbers and a scale of 1/8.  Scaling, the maximum and
+    the logarithm round values of up to (1 + |lse|) log2(e) four times, by 2^-24 each."""
+    g = torch.Generator(device="cuda").manual_seed(chunk)
+    q = torch.zeros((1, L, D), device="cuda", dtype=BF)
+    k, v = torch.zeros((1, M, D), device="cuda", dtype=BF), torch.ones((1, M, D), device="cuda", dtype=BF)
+    q[..., 1:9] = torch.randint(-2, 3, (1, L, 8), device="cuda", generator=g).to(BF)
+    k[..., 1:9] = torch.randint(-2, 3, (1, M, 8), device="cuda", generator=g).to(BF)
+    q[..., 0], k[..., 0] = 1, -2000  # the other keys' weight is e^-250
+    k[:, 16 * chunk:16 * chunk + 16, 0] = 0
+    _, lse = ops.attention_with_lse(q, k, v, 1, softmax_scale=0.125)
+    want = torch.logsumexp(q.double() @ k.double().transpose(-1, -2) * 0.125, -1)
+    assert ((lse[:, 0].double() - want).abs() <= 2.7e-6 + 4 * 1.45 * 2.0 ** -24 * (1 + want.abs())).all()
