@@ -8,11 +8,15 @@
 // loading Q, its first scores and storing, against 1500 a tile.  So the CTAs stay, and take over blocks whose CTA has
 // not started yet (cluster launch control): the next block's Q and first keys are loaded and its first scores are
 // computed behind the last tiles of the current one, and a TMA store sends the output, staged in the block's Q tile,
-// while the next block runs.  9216 x 256, 32 heads: 80 us with a CTA per block, 55 so; 2 x 2304 x 1024 86 and 76.
+// while the next block runs.  9216 x 256, 32 heads: 83 us with a CTA per block, 55 so; 2 x 2304 x 1024 91 and 76.
 //   warp 0: TMA loads, and the next block   warp 1: MMA   warp 2: zeroes V's rows past the keys' length
 //   warp 3: TMA stores                      warps 4..7 (and 8..11): softmax, a query row per thread
-// At long sums the softmax sets the pace, as in the dense kernel: 9216 x 9216, 32 heads 1.11 ms = 1250 TFLOP/s, the tensor
-// pipe active for 62 % of the cycles; causal by tokens 0.61 ms; 28,800 tokens, 4 heads, causal by 1800 0.75 ms.
+// At long sums the softmax sets the pace, as in the dense kernel: 9216 x 9216, 32 heads 1.14 ms = 1220 TFLOP/s, the tensor
+// pipe active for 62 % of the cycles; causal by tokens 0.62 ms; 28,800 tokens, 4 heads, causal by 1800 0.77 ms.  These are
+// the kernel's time in a burst of a few ms; back to back, under the 1000 W cap, 1.28, 0.71 and 0.86 ms.
+// P is rounded to bf16, the type that the instruction wants where V is bf16: each term of O by 2^-8 at most, which leaves
+// O 0.0021 to 0.0024 of its norm from the exact one where the rounding of O alone leaves 0.0017.  A second product with
+// what the rounding dropped would cost half of the tensor work again.  The sum of the exponentials takes P unrounded.
 // With N = 2 (one CTA per SM) each key tile is read once for 256 rows; with N = 1 (two CTAs per SM) fewer rows are
 // wasted on an odd or single tile.
 #pragma once

@@ -1516,11 +1516,14 @@ constexpr int64_t kMaxSplits = 64;
 // L2 twice as often.  In units of a 64-key tile of the first form (0.9 us) a block costs its tiles and 3.6 to change to
 // the next, and the launch 2.8; in the second form its tiles cost 1.32 each, or 0.6 when no other CTA is on the SM, a
 // change 4.5 and the launch 2; joining shared blocks costs a launch, 6.  Measured at 32 heads, us with two tiles and
-// one: 4736 x 64 24.6 and 23.9, 9216 x 64 42.3 and 48.8, 9216 x 1024 141 and 183; without and with sharing:
-// 512 x 9216 136 and 87.
+// one, the kernels alone over inputs larger than L2: 64 x 64 6.9 and 6.4, 100 x 100 7.9 and 7.7, 9216 x 64 41 and 48,
+// 9216 x 256 55 and 71, 9216 x 1024 146 and 188.  The units flatter the second form where it is not a matter of a few
+// tiles: it is taken, too, at 4736 x 64 (24.9 and 28.0; 23.7 and 22.9 back to back out of L2), 128 x 1024 (17.0 and 19.4),
+// 1024 x 1024 with 8 heads (20.4 and 25.3) and 1 x 50,000 (64.7 and 71.4).  Without and with sharing: 512 x 9216 142
+// and 88.
 // A power of two of query heads with the same key/value head stand together in a Q tile, token by token, so that their
-// keys are read once and a causal tile spans fewer tokens.  With 32 heads on 8, us apart and together: 1 x 50,000 120
-// and 72 (832 unshared in the first form), causal 9216 641 and 564.
+// keys are read once and a causal tile spans fewer tokens.  With 32 heads on 8, us apart and together: 1 x 50,000 126
+// and 71 (832 unshared in the first form), causal 9216 590 and 580.
 struct FwdPlan {
   bool one;
   int pack_shift;
@@ -1561,8 +1564,8 @@ int64_t fwd_part_rows(int64_t batch, int64_t q_tokens, int64_t heads, int64_t sp
 // pairs and 6 more to start and store; a dK/dV pair costs 1.5, or 2.2 where its operands come from HBM, as for a CTA
 // whose tiles few others read.  The dK/dV CTAs start first, so the launch takes the longest of them, or an SM's share of
 // everything, or an SM's share of dK/dV and then the longest dQ sum; joining costs 10 and 2 per part.  Without causality,
-// us alone and as chosen here: 2304 x 2304 with 2 key/value heads of 16 queries each 417 and 226 (4 CTAs per dK/dV
-// tile), 28800 x 64, 16 heads 508 and 242 (4), 100 x 9216, 16 heads 133 and 89 (6 per dQ tile).
+// us alone and as chosen here: 2304 x 2304 with 2 key/value heads of 16 queries each 432 and 232 (4 CTAs per dK/dV
+// tile), 28800 x 64, 16 heads 518 and 253 (4), 100 x 9216, 16 heads 136 and 91 (6 per dQ tile).
 void bwd_splits(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t* dkdv,
                 int64_t* dq) {
   static const int64_t counts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kMaxSplits};
@@ -1693,7 +1696,7 @@ int ogx_attention_fwd_lse(const void* q, const void* k, const void* v, int64_t b
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   p.blocks = static_cast<unsigned>(ceil_div(q_tokens * pack, one ? 128 : 256));
   p.head_groups = static_cast<unsigned>(heads / pack);
-  // causal blocks differ in length: the longest of all heads first (28,800 tokens, 4 heads: 745 us, head by head 827)
+  // causal blocks differ in length: the longest of all heads first (28,800 tokens, 4 heads: 770 us, head by head 1003)
   const int64_t groups = batch * splits * p.head_groups;
   p.longest_first = causal_block > 0 && p.blocks <= 65535 && groups <= INT32_MAX;
   const dim3 grid = p.longest_first

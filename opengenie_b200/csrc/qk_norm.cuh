@@ -305,8 +305,8 @@ __device__ __forceinline__ void elements(const Lane& v, float (&e)[8]) {
 
 // ------------------------------------------------------------------------- norm of each head, or no norm
 // A group's heads are independent; UNROLL of them are loaded before the first is used.  Bound by HBM: 9216 tokens of
-// 32 + 32 heads 51.5 us = 5.9 TB/s (91 % of a plain copy), their gradient 83 us = 5.5 TB/s with its sums of the weights'
-// gradients; 4 tokens 3 us.
+// 32 + 32 heads 51 us = 6.0 TB/s (92 % of a plain copy), their gradient 82 us = 5.6 TB/s with its sums of the weights'
+// gradients; 4 tokens 2 us.
 template <int HD, int NORM, bool INTER, bool PER_HEAD, bool BACKWARD>
 __global__ void __launch_bounds__(kThreads, head_ctas(BACKWARD)) qk_head_kernel(const __grid_constant__ Params p) {
   constexpr int LANES = HD / 8;
@@ -410,7 +410,9 @@ __global__ void __launch_bounds__(kThreads, head_ctas(BACKWARD)) qk_head_kernel(
 // ------------------------------------------------------------------------- norm over all heads of a row
 // A team holds its token's columns (STEPS heads per group) until the row's sums are known.  Bound by instructions and the
 // wait for those sums (16 warps on an SM, a half of the issue slots used): 9216 tokens of 32 + 32 heads with tables for
-// each head 113 us = 3.3 TB/s, the gradient 150 us = 3.5 TB/s.
+// each head 111 us = 3.4 TB/s, the gradient 150 us = 3.5 TB/s.  More than 64 heads of 128 take four heads to a
+// group, and their gradient spills registers (0.5 KB a thread): 4608 tokens with tables for all heads, 64 + 64 heads 98
+// and 144 us, 96 + 32 heads, the same bytes, 208 and 445.
 template <int HD, int THREADS, int STEPS, bool INTER, bool PER_HEAD, bool BACKWARD>
 __global__ void __launch_bounds__(THREADS, row_ctas(THREADS, STEPS)) qk_row_kernel(const __grid_constant__ Params p) {
   constexpr int LANES = HD / 8;
