@@ -1952,6 +1952,14 @@ void qk_dispatch(const ogx::qkn::Params& p, int64_t head_dim, int interleaved, i
                      : qk_launch<64, false, BACKWARD>(p, steps, norm, s);
 }
 
+bool qk_sizes_ok(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads) {
+  if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || heads > kQkMaxHeads || kv_heads > kQkMaxHeads ||
+      heads + kv_heads > kQkMaxHeads)
+    return false;
+  // row numbers, and those a step past the last, stay below 2^31
+  return tokens <= (1 << 30) && batch <= (1 << 30) && tokens * batch <= (1 << 30);
+}
+
 int qk_norm_guard(const void* q, const void* k, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                   int64_t head_dim, int64_t q_stride_b, int64_t q_stride_t, int64_t k_stride_b, int64_t k_stride_t,
                   const void* q_weight, const void* k_weight, int weight_dtype, int norm, float eps, const void* cos,
@@ -1959,11 +1967,7 @@ int qk_norm_guard(const void* q, const void* k, int64_t batch, int64_t tokens, i
                   int64_t cs_stride_t) {
   if (q == nullptr || k == nullptr) return fail(OGX_EINVAL, "null_pointer");
   if (head_dim != 64 && head_dim != 128) return fail(OGX_EINVAL, "head_dim: 64 or 128");
-  if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || heads > kQkMaxHeads || kv_heads > kQkMaxHeads ||
-      heads + kv_heads > kQkMaxHeads)
-    return fail(OGX_EINVAL, "qk_shape");
-  // row numbers, and those a step past the last, stay below 2^31
-  if (tokens > (1 << 30) || batch > (1 << 30) || tokens * batch > (1 << 30)) return fail(OGX_EINVAL, "qk_shape");
+  if (!qk_sizes_ok(batch, tokens, heads, kv_heads)) return fail(OGX_EINVAL, "qk_shape");
   if (q_stride_b % 8 || q_stride_t % 8 || k_stride_b % 8 || k_stride_t % 8) return fail(OGX_EINVAL, "qk_noncontiguous");
   if (norm != kNone && norm != kHead && norm != kRow) return fail(OGX_EINVAL, "norm");
   if (norm != kNone && (q_weight == nullptr || k_weight == nullptr || !dtype_ok(weight_dtype)))
@@ -2076,8 +2080,7 @@ int ogx_qk_norm_rope(const void* q, const void* k, int64_t batch, int64_t tokens
 int ogx_qk_norm_rope_bwd_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                    int norm, int64_t* bytes) {
   if (bytes == nullptr) return fail(OGX_EINVAL, "null_pointer");
-  if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || heads > kQkMaxHeads || kv_heads > kQkMaxHeads ||
-      heads + kv_heads > kQkMaxHeads || (head_dim != 64 && head_dim != 128))
+  if (!qk_sizes_ok(batch, tokens, heads, kv_heads) || (head_dim != 64 && head_dim != 128))
     return fail(OGX_EINVAL, "qk_shape");
   if (norm != kNone && norm != kHead && norm != kRow) return fail(OGX_EINVAL, "norm");
   *bytes = qk_partial_bytes(qk_shape(heads, kv_heads, head_dim, norm, true, batch * tokens), norm, heads, head_dim) +

@@ -1,6 +1,7 @@
 """How the training-pass operators reach the library (no GPU): the device and the stream of a call."""
 
 import contextlib
+import ctypes
 
 import pytest
 import torch
@@ -46,6 +47,13 @@ def test_workspace_sizes_are_kept_for_each_device(monkeypatch):
         ltx_ops._workspace_bytes("entry", index, 3, 4)
     ltx_ops._workspace_bytes.cache_clear()
     assert asked == [(0, "entry", (3, 4)), (1, "entry", (3, 4))]
+
+
+@pytest.mark.parametrize("batch,tokens", [(1, (1 << 30) + 1), (1 << 16, 1 << 15), (1 << 40, 1 << 40), ((1 << 30) + 1, 1)])
+def test_workspace_query_refuses_sizes_that_the_call_refuses(ogx_lib, batch, tokens):
+    size = ctypes.c_int64(-1)
+    assert ogx_lib.ogx_qk_norm_rope_bwd_workspace(batch, tokens, 4, 2, 128, 1, ctypes.addressof(size)) == -1
+    assert ogx_lib.ogx_last_error().decode().split(":")[0] == "qk_shape" and size.value == -1
 
 
 @pytest.mark.gpu
