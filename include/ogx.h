@@ -432,7 +432,8 @@ int ogx_qk_norm_rope_bwd_workspace(int64_t batch, int64_t tokens, int64_t heads,
 
 /* Gradients of ogx_qk_norm_rope: from those of its outputs (dq_out, dk_out) and its inputs, dq and dk (bf16, own
  * strides; each may be the output gradient or the input it belongs to, with its strides, other overlaps are refused) and
- * the weights' dq_weight, dk_weight (f32, summed over all rows; not written for OGX_NORM_NONE).  workspace as for ogx_attention_bwd (may be NULL for OGX_NORM_NONE). */
+ * the weights' dq_weight, dk_weight (f32, summed over all rows; not written for OGX_NORM_NONE).  workspace as for
+ * ogx_attention_bwd (may be NULL for OGX_NORM_NONE). */
 int ogx_qk_norm_rope_bwd(const void* dq_out, int64_t dq_out_stride_b, int64_t dq_out_stride_t, const void* dk_out,
                          int64_t dk_out_stride_b, int64_t dk_out_stride_t, const void* q, const void* k, int64_t batch,
                          int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_b,

@@ -195,6 +195,8 @@ def video_msa_branch(block, video, vx: torch.Tensor, *, token_counts: set[int] |
     ``video`` provides ``timesteps`` and ``positional_embeddings`` (cos, sin).  The kernels have no backward pass: where
     ``vx`` or ``timesteps`` requires a gradient (and gradients are enabled) the branch declines, too
     (`requires_grad`), and the caller's path runs, its attention differentiable with the ``b200-native`` backend.
+    The block's weights count as constants, whether they are parameters or not: a step that trains its norms or its
+    table takes the caller's path.
     """
     global _MSA_BRANCH_CALLS
     from .synthetic import BlockWeights, Fp8Linear
@@ -277,8 +279,9 @@ def video_text_cross_attention_branch(block, x: torch.Tensor, context: torch.Ten
     :2821-2835), on shapes other than batch 1 x 4096 (`shape`, `context_shape`), a table of fewer than 9
     slots (`table_shape`), a context mask (`mask`: pass the prompt's valid tokens as the context instead),
     gated attention (`gated_attention`) and activations that require a gradient, which the kernels do not have
-    (`requires_grad`).  Otherwise the eight launches of ``VideoTextCrossAttention``, built
-    once per block from its modules (and again when one of their tensors is replaced or changed in place).
+    (`requires_grad`; weights count as constants, as in ``video_msa_branch``).  Otherwise the eight launches of
+    ``VideoTextCrossAttention``, built once per block from its modules (and again when one of their tensors is
+    replaced or changed in place).
     """
     global _TEXT_BRANCH_CALLS
     from .video_text_attention import VideoTextCrossAttention

@@ -9,8 +9,8 @@
 // 128 queries of a head (dQ, over all key tiles).  S and dP are computed in both: seven tile products instead of
 // five.  In return every gradient is summed in one CTA's tensor memory in a fixed order: no fp32 buffer for dQ, no
 // atomics, and the same bits on every run.  (The five-product form adds its dQ tiles to HBM, a 64 KB reduction per
-// tile pair, in whatever order the CTAs reach it.)  Where one side has so few tiles that the GPU would idle behind
-// long sums, several CTAs share a sum and attn_bwd_join_kernel adds their parts, in their order.
+// tile pair, in whatever order the CTAs reach it unless each waits for its turn.)  Where one side has so few tiles that
+// the GPU would idle behind long sums, several CTAs share a sum and attn_bwd_join_kernel adds their parts, in their order.
 //
 // What bounds it, at 9216 x 9216 x 32 heads: 3.71 ms back to back, under the 1000 W cap (1.43 GHz) 1312 TFLOP/s of
 // its seven products, 96 % of what cuBLAS sustains there; 3.20 ms in a burst.  Per tile pair the two roles take 2700
